@@ -1,0 +1,157 @@
+"""Mixture-of-experts operators: what they refuse, checked without a GPU.
+
+Shapes, types and ranges are checked before the device is touched, so plain CPU tensors reach
+every refusal; a call that passes them all is refused for its device."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from tileccl_b200 import _native, ops
+
+
+def _slots(tokens=4, top_k=2, experts=3):
+    n = tokens * top_k
+    return ops.ExpertSlots(torch.zeros(experts + 1, dtype=torch.int32),
+                           torch.zeros(n, dtype=torch.int32),
+                           torch.zeros(tokens, top_k, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("kwargs, error", [
+    (dict(top_k=0), ValueError), (dict(top_k=9), ValueError), (dict(score="relu"), ValueError),
+    (dict(groups=3), ValueError), (dict(groups=0), ValueError),
+    (dict(groups=4, top_groups=5), ValueError), (dict(groups=4, top_groups=0), ValueError),
+    (dict(groups=4, group_score="mean"), ValueError),
+    (dict(bias=torch.zeros(7)), ValueError),
+    (dict(bias=torch.zeros(8, dtype=torch.float16)), TypeError),
+    (dict(bias=torch.zeros(16)[::2]), ValueError),
+    (dict(mask=torch.ones(4)), TypeError), (dict(mask=torch.ones(3, dtype=torch.bool)), ValueError),
+    (dict(), ValueError),                                        # right, but on the CPU
+])
+def test_route_refusals(kwargs, error):
+    kwargs.setdefault("top_k", 2)
+    with pytest.raises(error):
+        ops.route_experts(torch.zeros(4, 8), **kwargs)
+
+
+def test_route_refuses_other_layouts_and_types():
+    with pytest.raises(ValueError):
+        ops.route_experts(torch.zeros(8), 2)
+    with pytest.raises(TypeError):
+        ops.route_experts(torch.zeros(4, 8, dtype=torch.float64), 2)
+    with pytest.raises(ValueError):
+        ops.route_experts(torch.zeros(8, 4).t(), 2)              # unit stride along tokens
+    with pytest.raises(ValueError, match="overlap"):
+        ops.route_experts(torch.zeros(1, 8).expand(4, 8), 2)
+    with pytest.raises(ValueError, match="experts"):
+        ops.route_experts(torch.zeros(4, 513), 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.route_experts(torch.zeros(4, 8), 2)
+
+
+def test_route_backward_refusals():
+    logits, ids = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32)
+    for g, i in [(torch.zeros(4, 3), ids), (torch.zeros(3, 2), ids),
+                 (torch.zeros(4, 2), torch.zeros(5, 2, dtype=torch.int32)),
+                 (torch.zeros(4, 4)[:, ::2], ids)]:
+        with pytest.raises(ValueError):
+            ops.route_experts_backward(g, logits, i)
+    with pytest.raises(TypeError):
+        ops.route_experts_backward(torch.zeros(4, 2), logits, ids.long())
+    with pytest.raises(TypeError):
+        ops.route_experts_backward(torch.zeros(4, 2).half(), logits, ids)
+
+
+def test_slot_refusals():
+    ids = torch.zeros(4, 2, dtype=torch.int32)
+    for bad in (ids[0], ids[:, :0], ids.t()):
+        with pytest.raises(ValueError):
+            ops.expert_slots(bad, 3)
+    with pytest.raises(TypeError):
+        ops.expert_slots(ids.long(), 3)
+    for n, first in ((0, 0), (1025, 0), (3, -1)):
+        with pytest.raises(ValueError):
+            ops.expert_slots(ids, n, first_expert=first)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.expert_slots(ids, 3)
+    with pytest.raises(ValueError):
+        ops.ExpertSlots(torch.zeros(4, dtype=torch.int32), torch.zeros(7, dtype=torch.int32), ids)
+    with pytest.raises(TypeError):
+        ops.ExpertSlots(torch.zeros(4), torch.zeros(8, dtype=torch.int32), ids)
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(rows="experts"), ValueError), (dict(epilogue="gelu"), ValueError),
+    (dict(epilogue="silu_gate"), ValueError),                    # N is no multiple of 256
+    (dict(b_is_nk=True), ValueError),                            # inner dimensions differ
+    (dict(rows="slots"), ValueError),                            # 4 rows for 8 slots
+    (dict(W=torch.zeros(2, 16, 24).half()), ValueError),         # experts differ
+    (dict(W=torch.zeros(3, 16, 24).bfloat16()), TypeError),
+    (dict(W=torch.zeros(16, 24).half()), ValueError),
+    (dict(X=torch.zeros(4, 16)), TypeError),
+    (dict(X=torch.zeros(4, 12).half(), W=torch.zeros(3, 12, 24).half()), ValueError),
+    (dict(W=torch.zeros(3, 16, 20).half()), ValueError),
+    (dict(out=torch.zeros(8, 23).half()), ValueError),
+    (dict(out=torch.zeros(8, 24)), TypeError),
+    (dict(out=torch.zeros(8, 28).half()[:, :24]), ValueError),   # rows not 16-byte aligned
+    (dict(slots=None), ValueError),
+    (dict(), ValueError),                                        # right, but on the CPU
+])
+def test_product_refusals(change, error):
+    args = dict(X=torch.zeros(4, 16).half(), W=torch.zeros(3, 16, 24).half(), slots=_slots())
+    args.update(change)
+    with pytest.raises(error):
+        ops.expert_gemm(**args)
+
+
+def test_backward_and_combine_refusals():
+    s = _slots()
+    X, W = torch.zeros(4, 16).half(), torch.zeros(3, 16, 24).half()
+    with pytest.raises(ValueError):
+        ops.expert_gemm_backward(torch.zeros(4, 24).half(), X, W, s)      # 8 slots
+    with pytest.raises(TypeError):
+        ops.expert_gemm_backward(torch.zeros(8, 24), X, W, s)
+    H, w = torch.zeros(8, 16).half(), torch.zeros(4, 2)
+    for args, kw in [((H[:4], s, w), {}), ((H, s, w[:3]), {}), ((H, s, w[:, :1]), {}),
+                     ((torch.zeros(8, 12).half(), s, w), {}),
+                     ((H, s, w), dict(add=torch.zeros(8, 16).half())),
+                     ((H, s, w), dict(out=torch.zeros(4, 8).half())),
+                     ((H, None, w), {}), ((H, s, w), {})]:
+        with pytest.raises(ValueError):
+            ops.expert_combine(*args, **kw)
+    with pytest.raises(TypeError):
+        ops.expert_combine(H.float(), s, w)
+    with pytest.raises(TypeError):
+        ops.expert_combine(H, s, w.half())
+    with pytest.raises(ValueError):
+        ops.expert_combine_backward(torch.zeros(4, 16).half(), H, s, None)
+    with pytest.raises(ValueError):
+        ops.expert_combine_backward(torch.zeros(8, 16).half(), H, s, w)
+
+
+def test_native_entries_check_their_arguments():
+    """The C entries refuse on their own (another binding may call them)."""
+    lib = _native.load()
+    ok = [64, 8, 0, 0, 64, 64, 4, 8, 2, 2, 0, 1, 1, 0, 1, 1.0, 0]
+    for i, v in [(0, 0), (1, 4), (6, -1), (7, 0), (7, 513), (8, 0), (8, 9), (9, 3), (11, 3),
+                 (12, 2)]:
+        args = list(ok)
+        args[i] = v
+        assert lib.tccl_expert_route(*args) == 1, (i, v)
+    d = _native.ExpertGemm()
+    fields = dict(dtype=0, epilogue=0, experts=3, w_nk=0, k=16, n=24, slots=8, x_rows=4, offsets=64,
+                  token_of_slot=64, x=64, w=64, out=64, dh=0, ldx=16, ldw=24, w_expert=384, ldo=24)
+    for name, bad in [("dtype", 2), ("epilogue", 3), ("epilogue", 1), ("experts", 0),
+                      ("experts", 1025), ("k", 12), ("n", 20), ("k", 0), ("ldx", 12), ("x", 72),
+                      ("slots", -1), ("slots", 1 << 31), ("x", 0), ("offsets", 0)]:
+        for k, v in fields.items():
+            setattr(d, k, v)
+        setattr(d, name, bad)
+        assert lib.tccl_expert_gemm(C.byref(d), 0) == 1, (name, bad)
+    assert lib.tccl_expert_slots(64, 4, 2, 1025, 0, 64, 64, 64, 0, 0) == 1
+    assert lib.tccl_expert_slots(64, 1 << 30, 2, 8, 0, 64, 64, 64, 0, 0) == 1
+    assert lib.tccl_expert_slots(64, 1 << 16, 2, 8, 0, 64, 64, 64, 0, 0) == 1   # no workspace
+    assert lib.tccl_expert_combine(64, 16, 64, 64, 0, 0, 64, 16, 4, 8, 2, 12, 0, 0) == 1
+    assert lib.tccl_expert_combine(64, 16, 64, 64, 0, 0, 64, 16, 4, 8, 2, 16, 2, 0) == 1
+    assert b"" != lib.tccl_last_error()

@@ -1,0 +1,625 @@
+"""Mixture-of-experts operators against plain 64-bit formulas (one GPU)."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _randn(g, *shape, std=1.0, dtype=torch.float32):
+    return (torch.randn(*shape, device="cuda", generator=g) * std).to(dtype)
+
+
+def _within(got, want, bound):
+    """|got - want| <= bound elementwise (NaNs nowhere)."""
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst " \
+                          f"{err[bad].max().item():.3e} at bound {bound[bad].min().item():.3e}"
+
+
+# ------------------------------------------------------------------------------ routing
+def _route64(logits, k, score, bias, groups, top_groups, group_score, renormalize, scale, mask):
+    """Row by row in Python floats; returns (weights, ids) as tensors."""
+    T, E = logits.shape
+    w = torch.zeros(T, k, dtype=torch.float64)
+    ids = torch.full((T, k), -1, dtype=torch.int32)
+    rows = logits.double().cpu()
+    b = [0.0] * E if bias is None else bias.double().cpu().tolist()
+    for t in range(T):
+        if mask is not None and not bool(mask[t]):
+            continue
+        l = rows[t].tolist()
+        if all(v == -math.inf for v in l):
+            continue
+        if score == "softmax":
+            m = max(l)
+            e = [math.exp(v - m) for v in l]
+            s = math.fsum(e)
+            p = [v / s for v in e]
+        else:
+            p = [1 / (1 + math.exp(-v)) if v > -700 else 0.0 for v in l]
+        alive = {e: p[e] + b[e] for e in range(E) if l[e] != -math.inf and b[e] != -math.inf}
+        if groups > 1:
+            per = E // groups
+            score_of = {}
+            for e, key in alive.items():
+                score_of.setdefault(e // per, []).append(key)
+            rank = sorted(score_of, key=lambda g: (-sum(sorted(score_of[g])[-(1 if group_score == "max" else 2):]), g))
+            alive = {e: key for e, key in alive.items() if e // per in rank[:top_groups]}
+        best = sorted(alive, key=lambda e: (-alive[e], e))[:k]
+        total = math.fsum(p[e] for e in best) if renormalize else 1.0
+        for j, e in enumerate(best):
+            ids[t, j] = e
+            w[t, j] = scale * p[e] / total
+    return w.cuda(), ids.cuda()
+
+
+ROUTE_CASES = [
+    # tokens, experts, k, score, bias, groups, top_groups, group_score, renorm, scale
+    (1, 8, 2, "softmax", False, 1, 1, "top2", True, 1.0),
+    (1, 1, 1, "sigmoid", True, 1, 1, "top2", True, 1.0),
+    (7, 33, 5, "softmax", True, 1, 1, "top2", False, 1.0),
+    (130, 64, 8, "sigmoid", False, 1, 1, "top2", False, 2.5),
+    (65, 256, 8, "sigmoid", True, 8, 4, "top2", True, 2.5),
+    (33, 160, 6, "softmax", False, 8, 3, "max", False, 16.0),
+    (29, 96, 6, "softmax", False, 4, 2, "top2", True, 1.0),
+    (17, 512, 32, "softmax", False, 1, 1, "top2", True, 1.0),
+    (9, 32, 3, "sigmoid", True, 32, 5, "top2", True, 1.0),       # groups of one expert
+]
+
+
+@pytest.mark.parametrize("case", ROUTE_CASES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_route_matches_formula(case, dtype):
+    from tileccl_b200 import ops
+
+    T, E, k, score, with_bias, groups, top_groups, gs, renorm, scale = case
+    g = _gen(T + E)
+    logits = _randn(g, T, E, std=2.0).to(dtype)
+    bias = _randn(g, E, std=0.1) if with_bias else None
+    w, ids = ops.route_experts(logits, k, score=score, bias=bias, groups=groups,
+                               top_groups=top_groups, group_score=gs, renormalize=renorm,
+                               scale=scale)
+    ref_w, ref_ids = _route64(logits, k, score, bias, groups, top_groups, gs, renorm, scale, None)
+    assert w.dtype == torch.float32 and torch.equal(ids, ref_ids)
+    # exp within 2 ulp, its argument's rounding |l - m| 2^-24 (< 20 here), a sum of at most 512
+    # positive terms, a division and a product: below 2^-24 * (4 + 20 + 10 + 2)
+    _within(w, ref_w, ref_w * 36 * 2 ** -24)
+
+
+def test_route_tells_close_keys_apart():
+    """Scores that agree in 32 bits are told apart; equal ones go to the lower index."""
+    from tileccl_b200 import ops
+
+    logits = torch.full((3, 16), -4.0, device="cuda")
+    logits[0, 5], logits[0, 9] = 9.0, 9.0000019          # sigmoids differ by 2^-32 or so
+    logits[1, 9], logits[1, 5] = 9.0, 9.0000019
+    logits[2, 3] = logits[2, 11] = 1.0
+    bias = torch.full((16,), 0.25, device="cuda")
+    for score in ("sigmoid", "softmax"):
+        _, ids = ops.route_experts(logits, 3, score=score, bias=bias)
+        assert ids[:, :2].tolist() == [[9, 5], [5, 9], [3, 11]]
+        assert ids[:, 2].tolist() == [0, 0, 0]
+
+
+def test_route_masks_and_unavailable_experts():
+    from tileccl_b200 import ops
+
+    inf, nan = math.inf, math.nan
+    logits = torch.tensor([[1.0, 2.0, 3.0, 4.0],
+                           [nan, inf, nan, 2.0],          # masked row
+                           [-inf, 1.0, -inf, -inf],       # fewer experts than k
+                           [-inf, -inf, -inf, -inf],
+                           [0.0, nan, 1.0, -inf],
+                           [-200.0, -201.0, -300.0, -inf]], device="cuda")
+    mask = torch.tensor([True, False, True, True, True, True], device="cuda")
+    for score in ("softmax", "sigmoid"):
+        w, ids = ops.route_experts(logits, 3, score=score, mask=mask)
+        assert ids.tolist() == [[3, 2, 1], [-1] * 3, [1, -1, -1], [-1] * 3, [2, 0, 1], [0, 1, 2]]
+        assert w[1].tolist() == [0.0] * 3 and w[3].tolist() == [0.0] * 3
+        assert w[2].tolist() == [1.0, 0.0, 0.0]
+        assert torch.isnan(w[4]).all()
+        # renormalised scores keep their ratio e where the scores themselves underflow
+        assert abs(w[5, 0].item() - 1 / (1 + math.exp(-1))) < 1e-6
+    bias = torch.tensor([0.0, 0.0, -inf, -inf], device="cuda")
+    _, ids = ops.route_experts(logits[:1], 3, bias=bias)
+    assert ids.tolist() == [[1, 0, -1]]
+    # groups without an available expert stay behind
+    grouped = torch.tensor([[-inf, -inf, -5.0, -inf]], device="cuda")
+    _, ids = ops.route_experts(grouped, 2, score="sigmoid", groups=2, top_groups=1)
+    assert ids.tolist() == [[2, -1]]
+    w, ids = ops.route_experts(logits[:0], 2)
+    assert tuple(w.shape) == tuple(ids.shape) == (0, 2)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("shape", [(1, 8, 2), (67, 33, 5), (40, 300, 8), (5, 64, 1)])
+def test_route_backward(score, renorm, shape):
+    from tileccl_b200 import ops
+
+    T, E, k = shape
+    g = _gen(E)
+    big = _randn(g, T, E + 5, std=1.5)
+    logits = big[:, :E]                                   # strided rows
+    _, ids = ops.route_experts(logits, k, score=score, renormalize=renorm, scale=1.5)
+    grad = _randn(g, T, k)
+    if T > 2:
+        ids[2, -1] = -1                                   # a place without an expert
+    got = ops.route_experts_backward(grad, logits, ids, score=score, renormalize=renorm, scale=1.5)
+    l = logits.double().requires_grad_(True)
+    p = torch.softmax(l, 1) if score == "softmax" else torch.sigmoid(l)
+    here = ids >= 0
+    c = p.gather(1, ids.clamp(min=0).long()) * here
+    none = ~here.any(1, keepdim=True)                     # (a token without any expert: 0 / 1)
+    w = 1.5 * (c / (c.sum(1, keepdim=True) + none) if renorm else c)
+    (w * grad.double()).sum().backward()
+    # terms are at most scale * |p| * (|g| + sum |g w|); each carries the 36 half steps of a
+    # weight and as many again for the dot product
+    size = 1.5 * p.detach() * (2 + grad.double().abs().sum(1, keepdim=True))
+    if renorm:
+        size = size / (c.detach().sum(1, keepdim=True) + none)
+    _within(got, l.grad, 80 * 2 ** -24 * size)
+    # and against differences of the forward pass in 64 bits, in one direction
+    d = _randn(g, T, E).double() * 1e-5
+
+    def loss(x):
+        q = torch.softmax(x, 1) if score == "softmax" else torch.sigmoid(x)
+        cc = q.gather(1, ids.clamp(min=0).long()) * here
+        return (1.5 * (cc / (cc.sum(1, keepdim=True) + none) if renorm else cc) * grad.double()).sum()
+
+    diff = (loss(logits.double() + d) - loss(logits.double() - d)) / 2
+    want = (got.double() * d).sum()
+    assert abs(diff - want) <= 1e-5 * (got.double().abs() * d.abs()).sum()
+
+
+def test_route_backward_unrouted_rows_are_zero():
+    from tileccl_b200 import ops
+
+    logits = torch.full((2, 40), math.nan, device="cuda")
+    logits[1] = 0.5
+    logits[1, 3] = -math.inf
+    ids = torch.tensor([[-1, -1], [4, 7]], dtype=torch.int32, device="cuda")
+    for score in ("softmax", "sigmoid"):
+        for renorm in (False, True):
+            d = ops.route_experts_backward(torch.ones(2, 2, device="cuda"), logits, ids, score=score,
+                                           renormalize=renorm)
+            assert (d[0] == 0).all() and d[1, 3] == 0 and torch.isfinite(d).all()
+
+
+# ------------------------------------------------------------------------------ slot map
+@pytest.mark.parametrize("tokens, k, experts, first, local", [
+    (0, 2, 4, 0, 4), (1, 1, 1, 0, 1), (1, 8, 64, 0, 64), (37, 3, 5, 1, 3), (512, 8, 8, 0, 8),
+    (513, 8, 8, 2, 2), (2049, 2, 1024, 0, 1024), (5000, 6, 61, 60, 1), (20011, 8, 256, 128, 128)])
+def test_slots(tokens, k, experts, first, local):
+    from tileccl_b200 import ops
+
+    g = _gen(tokens + 1)
+    ids = torch.randint(-1, experts, (tokens, k), device="cuda", generator=g).int()
+    s = ops.expert_slots(ids, local, first_expert=first)
+    flat = ids.reshape(-1).long().cpu() - first
+    here = (flat >= 0) & (flat < local)
+    order = sorted(torch.nonzero(here).flatten().tolist(), key=lambda i: (int(flat[i]), i))
+    counts = torch.bincount(flat[here], minlength=local)
+    assert s.offsets.tolist() == [0] + counts.cumsum(0).tolist()
+    tok = torch.full((tokens * k,), -1, dtype=torch.int32)
+    tok[:len(order)] = torch.tensor([i // k for i in order], dtype=torch.int32)
+    slot = torch.full((tokens * k,), -1, dtype=torch.int32)
+    if order:
+        slot[torch.tensor(order)] = torch.arange(len(order), dtype=torch.int32)
+    assert torch.equal(s.token_of_slot.cpu(), tok)
+    assert torch.equal(s.slot_of.cpu().reshape(-1), slot)
+
+
+# ----------------------------------------------------------------------------- products
+def _make_slots(g, tokens, k, experts, lost=0.0):
+    from tileccl_b200 import ops
+
+    ids = _randn(g, tokens, experts).topk(k, 1).indices.int()
+    if lost:
+        drop = torch.rand(tokens, k, device="cuda", generator=g) < lost
+        ids = torch.where(drop, torch.full_like(ids, -1), ids)
+    return ops.expert_slots(ids, experts)
+
+
+def _sum_bound(a, b, terms):
+    """Error of an fp32 sum of `terms` products in any order, the tensor cores' truncating
+    additions (2^-23 each) included."""
+    return terms * 2 ** -23 * (a.abs() @ b.abs())
+
+
+def _pairs(N):
+    """Columns of gate and up in packed order."""
+    c = torch.arange(N // 2, device="cuda")
+    gate = (c // 128) * 256 + c % 128
+    return gate, gate + 128
+
+
+def _ref_product(x, w, gate):
+    """(out, bound before rounding) of one expert in 64 bits; w is [K, N]."""
+    x, w = x.double(), w.double()
+    y, dy = x @ w, _sum_bound(x, w, x.shape[1])
+    if not gate:
+        return y, dy
+    cg, cu = _pairs(w.shape[1])
+    a, u, da, du = y[:, cg], y[:, cu], dy[:, cg], dy[:, cu]
+    s = torch.sigmoid(a)
+    out = a * s * u
+    # |silu'| < 1.1; exp and the division of the epilogue carry a few 2^-22 of relative error
+    # (the fast exponential's grows with its argument: |a| 2^-23)
+    return out, 1.1 * u.abs() * da + (a * s).abs() * du + da * du * 1.1 + \
+        out.abs() * (8 + a.abs()) * 2 ** -22
+
+
+PRODUCT_CASES = [
+    # tokens, k, experts, K, N, lost
+    (1, 1, 1, 8, 256, 0.0),
+    (1, 2, 8, 64, 256, 0.0),
+    (3, 2, 4, 72, 512, 0.3),
+    (40, 4, 16, 136, 256, 0.0),
+    (200, 2, 3, 320, 768, 0.0),
+    (700, 3, 5, 1024, 512, 0.1),
+    (1100, 1, 2, 512, 1024, 0.0),
+]
+
+
+@pytest.mark.parametrize("case", PRODUCT_CASES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b_is_nk", [False, True])
+@pytest.mark.parametrize("rows", ["tokens", "slots"])
+@pytest.mark.parametrize("epilogue", ["none", "silu_gate"])
+def test_expert_gemm(case, dtype, b_is_nk, rows, epilogue):
+    from tileccl_b200 import ops
+
+    T, k, E, K, N, lost = case
+    gate = epilogue == "silu_gate"
+    if not gate:
+        N -= 8 * (E % 4)                                  # odd widths without the gate
+    g = _gen(T + K)
+    slots = _make_slots(g, T, k, E, lost)
+    X = _randn(g, T if rows == "tokens" else T * k, K, std=K ** -0.5, dtype=dtype)
+    W = _randn(g, E, N, K, dtype=dtype) if b_is_nk else _randn(g, E, K, N, dtype=dtype)
+    out = torch.full((T * k, N // 2 if gate else N), 7.0, dtype=dtype, device="cuda")
+    got = ops.expert_gemm(X, W, slots, out, rows=rows, b_is_nk=b_is_nk, epilogue=epilogue)
+    assert got is out
+    off, tok = slots.offsets.tolist(), slots.token_of_slot.long()
+    for e in range(E):
+        a, b = off[e], off[e + 1]
+        x = X[tok[a:b]] if rows == "tokens" else X[a:b]
+        want, bound = _ref_product(x, W[e].t() if b_is_nk else W[e], gate)
+        _within(out[a:b], want, bound + (want.abs() + bound) * _half_step(dtype) + 2 ** -25)
+    assert (out[off[E]:] == 7.0).all()                    # behind the last slot
+
+
+def test_expert_gemm_strided_operands_and_poisoned_neighbours():
+    """Row pitches and expert pitches beyond the width; NaN in every place that must not be
+    read into a result: other tokens' rows, rows behind the last slot, columns beside a view."""
+    from tileccl_b200 import ops
+
+    dtype, T, k, E, K, N = torch.bfloat16, 50, 2, 4, 200, 264
+    g = _gen(3)
+    ids = torch.randint(0, E, (T, k), device="cuda", generator=g).int()
+    ids[:, 1] = -1
+    ids[10:20] = -1                                       # tokens that no expert takes
+    slots = ops.expert_slots(ids, E)
+    big_x = torch.full((T, K + 64), math.nan, dtype=dtype, device="cuda")
+    big_w = torch.full((E, K + 8, N + 24), math.nan, dtype=dtype, device="cuda")
+    X, W = big_x[:, 8:8 + K], big_w[:, 8:, 8:8 + N]
+    X.copy_(_randn(g, T, K, std=K ** -0.5))
+    X[10:20] = math.nan
+    W.copy_(_randn(g, E, K, N))
+    big_out = torch.full((T * k, N + 16), 5.0, dtype=dtype, device="cuda")
+    out = big_out[:, 8:8 + N]
+    ops.expert_gemm(X, W, slots, out)
+    off, tok = slots.offsets.tolist(), slots.token_of_slot.long()
+    for e in range(E):
+        a, b = off[e], off[e + 1]
+        want, bound = _ref_product(X[tok[a:b]], W[e], False)
+        _within(out[a:b], want, bound + (want.abs() + bound) * _half_step(dtype))
+    assert (big_out[:, :8] == 5.0).all() and (big_out[:, 8 + N:] == 5.0).all()
+    assert (out[off[E]:] == 5.0).all()
+    # slot rows: the same with NaN behind the last slot and in the neighbours' rows
+    Xs = torch.full((T * k, K), math.nan, dtype=dtype, device="cuda")
+    Xs[:off[E]] = X[tok[:off[E]]]
+    again = ops.expert_gemm(Xs, W, slots, rows="slots")
+    assert torch.equal(again[:off[E]], out[:off[E]])
+
+
+def test_expert_gemm_empty_experts_and_tokens():
+    from tileccl_b200 import ops
+
+    W = torch.randn(3, 64, 256, device="cuda").half()
+    none = ops.expert_slots(torch.empty(0, 2, dtype=torch.int32, device="cuda"), 3)
+    X = torch.empty(0, 64, device="cuda").half()
+    assert tuple(ops.expert_gemm(X, W, none).shape) == (0, 256)
+    gx, gw = ops.expert_gemm_backward(torch.empty(0, 256, device="cuda").half(), X, W, none)
+    assert tuple(gx.shape) == (0, 64) and (gw == 0).all()
+    assert tuple(ops.expert_combine(torch.empty(0, 256, device="cuda").half(), none).shape) == (0, 256)
+    lost = ops.expert_slots(torch.full((5, 2), -1, dtype=torch.int32, device="cuda"), 3)
+    X = torch.randn(5, 64, device="cuda").half()
+    out = torch.ones(10, 256, device="cuda").half()
+    ops.expert_gemm(X, W, lost, out)
+    assert (out == 1).all()
+    gx, gw = ops.expert_gemm_backward(out, X, W, lost)
+    assert (gx == 0).all() and (gw == 0).all()
+
+
+@pytest.mark.parametrize("case", [(1, 1, 1, 64, 256, 0.0), (70, 2, 4, 136, 512, 0.2),
+                                  (300, 3, 7, 256, 256, 0.0), (900, 2, 3, 512, 768, 0.0)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b_is_nk", [False, True])
+@pytest.mark.parametrize("rows", ["tokens", "slots"])
+@pytest.mark.parametrize("epilogue", ["none", "silu_gate"])
+def test_expert_gemm_backward(case, dtype, b_is_nk, rows, epilogue):
+    from tileccl_b200 import ops
+
+    T, k, E, K, N, lost = case
+    gate = epilogue == "silu_gate"
+    if not gate:
+        N -= 8 * (E % 4)
+    g = _gen(T + K + 1)
+    slots = _make_slots(g, T, k, E, lost)
+    S = T * k
+    X = _randn(g, T if rows == "tokens" else S, K, std=K ** -0.5, dtype=dtype)
+    W = _randn(g, E, N, K, dtype=dtype) if b_is_nk else _randn(g, E, K, N, dtype=dtype)
+    dY = _randn(g, S, N // 2 if gate else N, std=0.25, dtype=dtype)
+    off, tok = slots.offsets.tolist(), slots.token_of_slot.long()
+    dY[off[E]:] = math.nan                                # behind the last slot: never read
+    gx, gw = ops.expert_gemm_backward(dY, X, W, slots, rows=rows, b_is_nk=b_is_nk,
+                                      epilogue=epilogue)
+    u = _half_step(dtype)
+    want_x = torch.zeros(X.shape, dtype=torch.float64, device="cuda")
+    bound_x = torch.zeros_like(want_x)
+    for e in range(E):
+        a, b = off[e], off[e + 1]
+        w = (W[e].t() if b_is_nk else W[e]).double()
+        at = tok[a:b] if rows == "tokens" else torch.arange(a, b, device="cuda")
+        x, dy = X[at].double(), dY[a:b].double()
+        err = torch.zeros(b - a, N, dtype=torch.float64, device="cuda")
+        if gate:
+            y, ey = x @ w, _sum_bound(x, w, K)
+            cg, cu = _pairs(N)
+            ga, up, eg, eu = y[:, cg], y[:, cu], ey[:, cg], ey[:, cu]
+            s = torch.sigmoid(ga)
+            d = torch.zeros(b - a, N, dtype=torch.float64, device="cuda")
+            d[:, cg] = dy * up * s * (1 + ga * (1 - s))
+            d[:, cu] = dy * ga * s
+            # |silu'| < 1.1, |silu''| <= 0.5; then the rounding of the operand to 16 bits
+            fast = (8 + ga.abs()) * 2 ** -22
+            err[:, cg] = dy.abs() * (1.1 * eu + 0.5 * up.abs() * eg
+                                     + up.abs() * (1 + ga.abs()) * fast)
+            err[:, cu] = dy.abs() * (1.1 * eg + (ga * s).abs() * fast)
+            dy, err = d, err * 1.01 + (d.abs() + err) * u + 2 ** -25
+        dx = dy @ w.t()
+        bx = _sum_bound(dy.abs() + err, w.t(), N) + err @ w.t().abs()
+        bx = bx + (dx.abs() + bx) * u                     # slot rows are held in 16 bits
+        dw = x.t() @ dy
+        bw = _sum_bound(x.t(), dy.abs() + err, b - a) + x.t().abs() @ err
+        got_w = gw[e].t() if b_is_nk else gw[e]
+        _within(got_w, dw, bw + (dw.abs() + bw) * u + 2 ** -25)
+        if rows == "tokens":
+            want_x.index_add_(0, at, dx)
+            bound_x.index_add_(0, at, bx)
+        else:
+            want_x[a:b], bound_x[a:b] = dx, bx
+    if rows == "tokens":
+        _within(gx, want_x, bound_x * 1.001 + want_x.abs() * u + 2 ** -25)
+    else:
+        _within(gx[:off[E]], want_x[:off[E]], bound_x[:off[E]] + 2 ** -25)
+
+
+def test_backward_against_differences():
+    """Directional derivative of a scalar of the gated product against the gradients."""
+    from tileccl_b200 import ops
+
+    g = _gen(11)
+    T, k, E, K, N, dtype = 60, 2, 3, 64, 256, torch.float16
+    slots = _make_slots(g, T, k, E)
+    X, W = _randn(g, T, K, std=K ** -0.5, dtype=dtype), _randn(g, E, K, N, dtype=dtype)
+    dY = _randn(g, T * k, N // 2, dtype=dtype)
+    gx, gw = ops.expert_gemm_backward(dY, X, W, slots, epilogue="silu_gate")
+    off, tok = slots.offsets.tolist(), slots.token_of_slot.long()
+    cg, cu = _pairs(N)
+
+    def loss(x, w):
+        total = 0.0
+        for e in range(E):
+            y = x[tok[off[e]:off[e + 1]]] @ w[e]
+            total += (torch.nn.functional.silu(y[:, cg]) * y[:, cu] * dY[off[e]:off[e + 1]].double()).sum()
+        return total
+
+    x, w = X.double(), W.double()
+    dx, dw = _randn(g, T, K).double() * 1e-4, _randn(g, E, K, N).double() * 1e-4
+    diff = (loss(x + dx, w + dw) - loss(x - dx, w - dw)) / 2
+    mine = (gx.double() * dx).sum() + (gw.double() * dw).sum()
+    # two 16-bit roundings on the way to every gradient, signs at random over many terms
+    size = math.sqrt((gx.double() * dx).square().sum() + (gw.double() * dw).square().sum())
+    assert abs(diff - mine) <= 8 * 2 * _half_step(dtype) * size
+
+
+# ------------------------------------------------------------------------------ combine
+@pytest.mark.parametrize("tokens, k, n, lost, weighted, add", [
+    (1, 1, 8, 0.0, True, False), (1, 8, 4096, 0.0, True, True), (5, 3, 264, 0.5, False, False),
+    (300, 6, 1032, 0.2, True, True), (33, 2, 9000, 0.0, True, False)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_combine(tokens, k, n, lost, weighted, add, dtype):
+    from tileccl_b200 import ops
+
+    g = _gen(tokens + n)
+    slots = _make_slots(g, tokens, k, 16, lost)
+    used = int(slots.offsets[-1])
+    H = _randn(g, tokens * k, n, dtype=dtype)
+    H[used:] = math.nan
+    w = _randn(g, tokens, k) if weighted else None
+    base = _randn(g, tokens, n, dtype=dtype) if add else None
+    keep = None if base is None else base.clone()
+    got = ops.expert_combine(H, slots, w, add=base)
+    here = slots.slot_of >= 0
+    ww = (torch.ones(tokens, k, device="cuda") if w is None else w).double() * here
+    rows = H[slots.slot_of.clamp(min=0).long()].double()
+    rows = torch.where(here[:, :, None], rows, torch.zeros_like(rows))
+    want = torch.einsum("tj,tjn->tn", ww, rows)
+    size = torch.einsum("tj,tjn->tn", ww.abs(), rows.abs())
+    if base is not None:
+        want, size = want + base.double(), size + base.double().abs()
+    bound = (k + 1) * 2 ** -24 * size
+    bound = bound + (want.abs() + bound) * _half_step(dtype) + 2 ** -25
+    _within(got, want, bound)
+    if base is not None:                                  # in place over the residual
+        ops.expert_combine(H, slots, w, base, add=base)
+        assert torch.equal(base, got) and not torch.equal(base, keep)
+
+
+@pytest.mark.parametrize("tokens, k, n, lost", [(1, 1, 8, 0.0), (3, 8, 4096, 0.0),
+                                               (200, 6, 1032, 0.3), (17, 2, 20000, 0.0)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_combine_backward(tokens, k, n, lost, dtype):
+    from tileccl_b200 import ops
+
+    g = _gen(tokens + n)
+    slots = _make_slots(g, tokens, k, 16, lost)
+    used = int(slots.offsets[-1])
+    big = _randn(g, tokens * k, n + 16, dtype=dtype)
+    H = big[:, 8:8 + n]
+    H[used:] = math.nan
+    w = _randn(g, tokens, k)
+    w[slots.slot_of < 0] = math.nan
+    dy = _randn(g, tokens, n, dtype=dtype)
+    gh, gw = ops.expert_combine_backward(dy, H, slots, w)
+    here = slots.slot_of >= 0
+    at = slots.slot_of[here].long()
+    want_h = torch.zeros(tokens * k, n, dtype=torch.float64, device="cuda")
+    tok = torch.arange(tokens, device="cuda")[:, None].expand(tokens, k)[here]
+    want_h[at] = w[here].double()[:, None] * dy[tok].double()
+    u = _half_step(dtype)
+    _within(gh[:used], want_h[:used], want_h[:used].abs() * (u + 2 ** -23) + 2 ** -25)
+    want_w = torch.zeros(tokens, k, dtype=torch.float64, device="cuda")
+    prod = dy[tok].double() * H[at].double()
+    want_w[here] = prod.sum(1)
+    size = torch.zeros_like(want_w)
+    size[here] = prod.abs().sum(1)
+    _within(gw, want_w, n * 2 ** -24 * size)
+
+
+# --------------------------------------------------------------------- as used together
+def _layer(ops, logits, x, w_gu, w_down, k):
+    weights, ids = ops.route_experts(logits, k)
+    slots = ops.expert_slots(ids, w_gu.shape[0])
+    h = ops.expert_gemm(x, w_gu, slots, epilogue="silu_gate")
+    y = ops.expert_gemm(h, w_down, slots, rows="slots")
+    return ops.expert_combine(y, slots, weights, add=x), weights, slots, h, y
+
+
+def _layer_ref(logits, x, w_gu, w_down, k):
+    """The layer in 64 bits, differentiable, every expert applied to every token."""
+    p = torch.softmax(logits, 1)
+    top = p.topk(k, 1)
+    w = torch.zeros_like(p).scatter(1, top.indices, top.values / top.values.sum(1, keepdim=True))
+    cg, cu = _pairs(w_gu.shape[2])
+    out = x
+    for e in range(w_gu.shape[0]):
+        y = x @ w_gu[e]
+        out = out + w[:, e:e + 1] * ((torch.nn.functional.silu(y[:, cg]) * y[:, cu]) @ w_down[e])
+    return out
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 257])
+def test_layer_forward_and_backward(tokens):
+    from tileccl_b200 import ops
+
+    dtype, k, E, H, F = torch.float16, 2, 6, 256, 384
+    g = _gen(tokens)
+    logits, x = _randn(g, tokens, E, std=1.5), _randn(g, tokens, H, dtype=dtype)
+    w_gu, w_down = _randn(g, E, H, 2 * F, std=H ** -0.5, dtype=dtype), _randn(g, E, F, H, std=F ** -0.5, dtype=dtype)
+    out, weights, slots, h, y = _layer(ops, logits, x, w_gu, w_down, k)
+    leaves = [t.double().requires_grad_(True) for t in (logits, x, w_gu, w_down)]
+    ref = _layer_ref(*leaves, k)
+    dout = _randn(g, tokens, H, dtype=dtype)
+    ref.backward(dout.double())
+    dy, dweights = ops.expert_combine_backward(dout, y, slots, weights)
+    dh, dw_down = ops.expert_gemm_backward(dy, h, w_down, slots, rows="slots")
+    dx, dw_gu = ops.expert_gemm_backward(dh, x, w_gu, slots, epilogue="silu_gate")
+    dx = dx.double() + dout.double()
+    dlogits = ops.route_experts_backward(dweights, logits, ops.route_experts(logits, k)[1])
+    # at most five 16-bit roundings lie on any path, each half a step of a value that the
+    # following sums mix with random signs: five half steps of the result's size, times 4
+    # for the largest of some 10^5 normal deviates
+    for got, want in ((out, ref.detach()), (dx, leaves[1].grad), (dw_gu, leaves[2].grad),
+                      (dw_down, leaves[3].grad), (dlogits, leaves[0].grad)):
+        rms = want.square().mean().sqrt()
+        err = (got.double() - want).abs()
+        assert (err <= 5 * 4 * _half_step(dtype) * (want.abs() + rms) + 1e-9).all(), err.max().item()
+
+
+def test_layer_in_a_graph_on_another_stream_and_twice_at_once():
+    """Captured and replayed on new inputs; two graphs and an eager layer at the same time."""
+    from tileccl_b200 import ops
+
+    dtype, k, E, H, F, T = torch.bfloat16, 2, 8, 512, 256, 40
+    g = _gen(9)
+    w_gu, w_down = _randn(g, E, H, 2 * F, std=H ** -0.5, dtype=dtype), _randn(g, E, F, H, std=F ** -0.5, dtype=dtype)
+    data = [(_randn(g, T, E), _randn(g, T, H, dtype=dtype)) for _ in range(6)]
+    want = [_layer(ops, l, x, w_gu, w_down, k)[0].clone() for l, x in data]
+    graphs = []
+    for i in range(2):
+        l, x = data[i][0].clone(), data[i][1].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _layer(ops, l, x, w_gu, w_down, k)[0]
+        graphs.append((graph, l, x, out))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for rep in range(3):
+        for i, (graph, l, x, out) in enumerate(graphs):
+            with torch.cuda.stream(streams[i]):
+                l.copy_(data[2 * rep + i][0])
+                x.copy_(data[2 * rep + i][1])
+        torch.cuda.synchronize()
+        eager = []
+        for i, (graph, l, x, out) in enumerate(graphs):
+            with torch.cuda.stream(streams[i]):
+                graph.replay()
+        for l, x in data[:2]:
+            weights, ids = ops.route_experts(l, k, stream=streams[2])
+            s = ops.expert_slots(ids, E, stream=streams[2])
+            h = ops.expert_gemm(x, w_gu, s, epilogue="silu_gate", stream=streams[2])
+            y = ops.expert_gemm(h, w_down, s, rows="slots", stream=streams[2])
+            eager.append(ops.expert_combine(y, s, weights, add=x, stream=streams[2]))
+        torch.cuda.synchronize()
+        for i, (graph, l, x, out) in enumerate(graphs):
+            assert torch.equal(out, want[2 * rep + i])
+        assert torch.equal(eager[0], want[0]) and torch.equal(eager[1], want[1])
+
+
+def test_backward_repeats_and_captures():
+    from tileccl_b200 import ops
+
+    g = _gen(21)
+    T, k, E, K, N, dtype = 300, 2, 4, 256, 512, torch.bfloat16
+    slots = _make_slots(g, T, k, E)
+    X, W = _randn(g, T, K, dtype=dtype), _randn(g, E, K, N, std=K ** -0.5, dtype=dtype)
+    dY = _randn(g, T * k, N // 2, dtype=dtype)
+    first = [t.clone() for t in ops.expert_gemm_backward(dY, X, W, slots, epilogue="silu_gate")]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gx, gw = ops.expert_gemm_backward(dY, X, W, slots, epilogue="silu_gate")
+    for _ in range(3):
+        graph.replay()
+        again = ops.expert_gemm_backward(dY, X, W, slots, epilogue="silu_gate")
+        torch.cuda.synchronize()
+        assert torch.equal(gx, first[0]) and torch.equal(gw, first[1])
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])

@@ -154,6 +154,51 @@ class GemmPlanInfo(C.Structure):
     ]
 
 
+class ExpertGemm(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("epilogue", C.c_int32),
+        ("experts", C.c_int32),
+        ("w_nk", C.c_int32),
+        ("k", C.c_int64),
+        ("n", C.c_int64),
+        ("slots", C.c_int64),
+        ("x_rows", C.c_int64),
+        ("offsets", C.c_uint64),
+        ("token_of_slot", C.c_uint64),
+        ("x", C.c_uint64),
+        ("w", C.c_uint64),
+        ("out", C.c_uint64),
+        ("dh", C.c_uint64),
+        ("ldx", C.c_int64),
+        ("ldw", C.c_int64),
+        ("w_expert", C.c_int64),
+        ("ldo", C.c_int64),
+        ("ld_dh", C.c_int64),
+    ]
+
+
+class ExpertWeightGrad(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("experts", C.c_int32),
+        ("gather_a", C.c_int32),
+        ("gather_b", C.c_int32),
+        ("m", C.c_int64),
+        ("n", C.c_int64),
+        ("slots", C.c_int64),
+        ("a_rows", C.c_int64),
+        ("b_rows", C.c_int64),
+        ("offsets", C.c_uint64),
+        ("token_of_slot", C.c_uint64),
+        ("a", C.c_uint64),
+        ("b", C.c_uint64),
+        ("out", C.c_uint64),
+        ("lda", C.c_int64),
+        ("ldb", C.c_int64),
+    ]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -170,7 +215,7 @@ def lib_path() -> Path:
 
 
 def _declare(lib: C.CDLL) -> None:
-    u64, i32, u32, vp = C.c_uint64, C.c_int32, C.c_uint32, C.c_void_p
+    u64, i64, i32, u32, vp = C.c_uint64, C.c_int64, C.c_int32, C.c_uint32, C.c_void_p
     lib.tccl_last_error.restype = C.c_char_p
     lib.tccl_version.restype = C.c_char_p
     sigs = {
@@ -216,6 +261,17 @@ def _declare(lib: C.CDLL) -> None:
         "tccl_emul_gemm_reducescatter_ex": [i32, i32, i32, i32, C.c_void_p, C.c_void_p, C.c_void_p, i32,
                                             i32, i32, i32, i32, i32, i32, i32, i32, i32, C.POINTER(i32)],
         "tccl_preload_kernels": [],
+        "tccl_expert_route": [u64, i64, u64, u64, u64, u64, i64, i32, i32, i32, i32, i32, i32, i32,
+                              i32, C.c_float, u64],
+        "tccl_expert_route_backward": [u64, u64, i64, u64, u64, i64, i32, i32, i32, i32, i32,
+                                       C.c_float, u64],
+        "tccl_expert_slots_workspace": [i64, i32, C.POINTER(i64)],
+        "tccl_expert_slots": [u64, i64, i32, i32, i32, u64, u64, u64, u64, u64],
+        "tccl_expert_gemm": [C.POINTER(ExpertGemm), u64],
+        "tccl_expert_weight_grad": [C.POINTER(ExpertWeightGrad), u64],
+        "tccl_expert_combine": [u64, i64, u64, u64, u64, i64, u64, i64, i64, i64, i32, i32, i32, u64],
+        "tccl_expert_combine_backward": [u64, i64, u64, i64, u64, u64, u64, i64, u64, i64, i64, i32,
+                                         i32, i32, u64],
         "tccl_plan_tile_order": [i32, i32, i32, i32, i32, i32, C.POINTER(i32), i32],
         "tccl_plan_tile_order_ex": [i32, i32, i32, i32, i32, i32, i32, C.POINTER(i32), i32],
         "tccl_bootstrap_allgather": [i32, i32, C.c_char_p, i32, u64, i32, C.POINTER(u64),

@@ -303,6 +303,57 @@ int tccl_prim_test(int32_t op, int32_t sub_op, int32_t rank, int32_t world_size,
                    uint64_t stream);
 
 // --------------------------------------------------------------------------
+// Mixture-of-experts operators (csrc/kernels/expert_{route,slots,gemm,combine}.cu).
+// Matrices are row-major with unit column stride; dtype codes: 0 fp16, 1 bf16, 2 fp32.
+// --------------------------------------------------------------------------
+// weights / ids: [tokens, top_k]; bias (fp32, per expert) and mask (bytes, per token, 0 = not
+// routed) may be 0; sigmoid 0 = softmax scores; groups 1 = every expert competes; group_max 0 =
+// a group counts by the sum of its two largest keys, 1 = by its largest.
+int tccl_expert_route(uint64_t logits, int64_t ld, uint64_t bias, uint64_t mask, uint64_t weights,
+                      uint64_t ids, int64_t tokens, int32_t experts, int32_t top_k, int32_t dtype,
+                      int32_t sigmoid, int32_t groups, int32_t top_groups, int32_t group_max,
+                      int32_t renormalize, float scale, uint64_t stream);
+// grad_logits: [tokens, experts] contiguous, in the logits' type.
+int tccl_expert_route_backward(uint64_t grad_weights, uint64_t logits, int64_t ld, uint64_t ids,
+                               uint64_t grad_logits, int64_t tokens, int32_t experts,
+                               int32_t top_k, int32_t dtype, int32_t sigmoid, int32_t renormalize,
+                               float scale, uint64_t stream);
+// Bytes of device scratch tccl_expert_slots needs for tokens * top_k entries (0 = none).
+int tccl_expert_slots_workspace(int64_t entries, int32_t experts, int64_t* bytes);
+// ids outside [first, first + experts) get no slot.
+int tccl_expert_slots(uint64_t ids, int64_t tokens, int32_t top_k, int32_t experts, int32_t first,
+                      uint64_t offsets, uint64_t token_of_slot, uint64_t slot_of,
+                      uint64_t workspace, uint64_t stream);
+
+typedef struct TcclExpertGemm {
+  int32_t dtype, epilogue;    // epilogue: 0 none, 1 SiLU gate, 2 gradient of the SiLU gate
+  int32_t experts, w_nk;      // w_nk: W is [experts, N, K], else [experts, K, N]
+  int64_t k, n, slots, x_rows;
+  uint64_t offsets;           // int32[experts + 1]
+  uint64_t token_of_slot;     // int32[slots]; 0 = row s of x belongs to slot s
+  uint64_t x, w, out, dh;     // dh: epilogue 2 only
+  int64_t ldx, ldw, w_expert, ldo, ld_dh;   // pitches in elements
+} TcclExpertGemm;
+int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream);
+
+// out[e] = sum over the slots of expert e of a[row(s)]^T b[row(s)]: [experts, m, n] contiguous.
+typedef struct TcclExpertWeightGrad {
+  int32_t dtype, experts, gather_a, gather_b;   // a gathered operand has one row per token
+  int64_t m, n, slots, a_rows, b_rows;
+  uint64_t offsets, token_of_slot, a, b, out;
+  int64_t lda, ldb;
+} TcclExpertWeightGrad;
+int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_t stream);
+
+int tccl_expert_combine(uint64_t h, int64_t h_ld, uint64_t slot_of, uint64_t weights, uint64_t add,
+                        int64_t add_ld, uint64_t out, int64_t out_ld, int64_t tokens,
+                        int64_t slots, int32_t top_k, int32_t n, int32_t dtype, uint64_t stream);
+int tccl_expert_combine_backward(uint64_t dy, int64_t dy_ld, uint64_t h, int64_t h_ld,
+                                 uint64_t slot_of, uint64_t weights, uint64_t dh, int64_t dh_ld,
+                                 uint64_t dw, int64_t tokens, int64_t slots, int32_t top_k,
+                                 int32_t n, int32_t dtype, uint64_t stream);
+
+// --------------------------------------------------------------------------
 // Debug build (-DTILECCL_DEBUG_CHECKS, libtileccl_b200_debug.so): the record of bounds
 // violations of the current device (tileccl::DebugRecord in device/symm_ptr.cuh, 40 bytes:
 // count, code, rank, from_rank, to_rank, enabled, addr, bytes), one per translation unit

@@ -1,0 +1,172 @@
+// Weighted sum of a token's expert outputs and its gradient.
+//
+//   y[t] = add[t] + sum_j w[t][j] * h[slot_of[t][j]]        (choices without a slot add nothing)
+//   dh[slot_of[t][j]] = w[t][j] * dy[t]      dw[t][j] = <dy[t], h[slot_of[t][j]]>
+//
+// Sums run in fp32 in the order of the choices and are rounded once.
+#include <cuda_runtime.h>
+
+#include "../api.h"
+#include "../device/tile_compute.cuh"
+#include "../runtime/errors.h"
+
+namespace tileccl {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct CombineParams {
+  const uint4* h;            // [slots] rows of `n` 16-bit values
+  int64_t h_ld;              // 16-byte vectors between rows, likewise below
+  const int32_t* slot_of;    // [tokens][top_k]
+  const float* weights;      // [tokens][top_k] or null (all ones)
+  const uint4* add;          // [tokens] rows or null
+  int64_t add_ld;
+  uint4* out;                // forward
+  int64_t out_ld;
+  const uint4* dy;           // backward
+  int64_t dy_ld;
+  uint4* dh;
+  int64_t dh_ld;
+  float* dw;
+  int64_t tokens, slots;
+  int32_t top_k, vecs, bf16;   // vecs: 16-byte vectors per row
+};
+
+__global__ void __launch_bounds__(kThreads) expert_combine_kernel(const CombineParams p) {
+  const int64_t t = blockIdx.x;
+  const int v = blockIdx.y * kThreads + threadIdx.x;
+  if (v >= p.vecs) return;
+  float acc[8] = {};
+  if (p.add != nullptr) tile_accumulate_16x8(p.bf16 != 0, acc, p.add[t * p.add_ld + v]);
+  for (int j = 0; j < p.top_k; ++j) {
+    const int32_t s = p.slot_of[t * p.top_k + j];
+    if (s < 0 || s >= p.slots) continue;
+    const float w = p.weights != nullptr ? p.weights[t * p.top_k + j] : 1.f;
+    float x[8] = {};
+    tile_accumulate_16x8(p.bf16 != 0, x, p.h[s * p.h_ld + v]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, x[i], acc[i]);
+  }
+  p.out[t * p.out_ld + v] = tile_cast_f32x8(p.bf16 != 0, acc);
+}
+
+__global__ void __launch_bounds__(kThreads) expert_combine_backward_kernel(const CombineParams p) {
+  __shared__ float part[kThreads / 32];
+  const int64_t t = blockIdx.x;
+  for (int j = 0; j < p.top_k; ++j) {
+    const int32_t s = p.slot_of[t * p.top_k + j];
+    float dot = 0.f;
+    if (s >= 0 && s < p.slots) {
+      const float w = p.weights[t * p.top_k + j];
+      for (int v = threadIdx.x; v < p.vecs; v += kThreads) {
+        float g[8] = {}, x[8] = {};
+        tile_accumulate_16x8(p.bf16 != 0, g, p.dy[t * p.dy_ld + v]);
+        tile_accumulate_16x8(p.bf16 != 0, x, p.h[s * p.h_ld + v]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dot = fmaf(g[i], x[i], dot);
+          g[i] *= w;
+        }
+        p.dh[s * p.dh_ld + v] = tile_cast_f32x8(p.bf16 != 0, g);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float sum = 0.f;
+      for (int w = 0; w < kThreads / 32; ++w) sum += part[w];
+      p.dw[t * p.top_k + j] = sum;
+    }
+    __syncthreads();
+  }
+}
+
+int check(const CombineParams& p) {
+  TCCL_CHECK_ARG(p.tokens >= 0 && p.tokens < (int64_t(1) << 31), "tokens out of range");
+  TCCL_CHECK_ARG(p.top_k >= 1 && p.vecs >= 1, "empty rows");
+  TCCL_CHECK_ARG(p.vecs <= 65535 * kThreads, "rows are too long");
+  return kOk;
+}
+
+}  // namespace
+
+cudaError_t preload_expert_combine_kernels() {
+  cudaFuncAttributes a;
+  cudaError_t e = cudaFuncGetAttributes(&a, expert_combine_kernel);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_combine_backward_kernel);
+  return e;
+}
+
+}  // namespace tileccl
+
+using namespace tileccl;
+
+extern "C" int tccl_expert_combine(uint64_t h, int64_t h_ld, uint64_t slot_of, uint64_t weights,
+                                   uint64_t add, int64_t add_ld, uint64_t out, int64_t out_ld,
+                                   int64_t tokens, int64_t slots, int32_t top_k, int32_t n,
+                                   int32_t dtype, uint64_t stream) {
+  TCCL_CHECK_ARG(dtype == 0 || dtype == 1, "dtype must be 0 (fp16) or 1 (bf16)");
+  TCCL_CHECK_ARG(n % 8 == 0 && h_ld % 8 == 0 && add_ld % 8 == 0 && out_ld % 8 == 0,
+                 "row lengths and pitches must be multiples of 8 elements");
+  TCCL_CHECK_ARG(h % 16 == 0 && add % 16 == 0 && out % 16 == 0, "rows must be 16-byte aligned");
+  CombineParams p = {};
+  p.h = reinterpret_cast<const uint4*>(h);
+  p.h_ld = h_ld / 8;
+  p.slot_of = reinterpret_cast<const int32_t*>(slot_of);
+  p.weights = reinterpret_cast<const float*>(weights);
+  p.add = reinterpret_cast<const uint4*>(add);
+  p.add_ld = add_ld / 8;
+  p.out = reinterpret_cast<uint4*>(out);
+  p.out_ld = out_ld / 8;
+  p.tokens = tokens;
+  p.slots = slots;
+  p.top_k = top_k;
+  p.vecs = n / 8;
+  p.bf16 = dtype;
+  const int rc = check(p);
+  if (rc) return rc;
+  if (tokens == 0) return kOk;
+  TCCL_CHECK_ARG(h != 0 && slot_of != 0 && out != 0, "null argument");
+  const dim3 grid(static_cast<unsigned>(tokens), (p.vecs + kThreads - 1) / kThreads);
+  expert_combine_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  TCCL_CHECK_CUDA(cudaGetLastError());
+  return kOk;
+}
+
+extern "C" int tccl_expert_combine_backward(uint64_t dy, int64_t dy_ld, uint64_t h, int64_t h_ld,
+                                            uint64_t slot_of, uint64_t weights, uint64_t dh,
+                                            int64_t dh_ld, uint64_t dw, int64_t tokens,
+                                            int64_t slots, int32_t top_k, int32_t n, int32_t dtype,
+                                            uint64_t stream) {
+  TCCL_CHECK_ARG(dtype == 0 || dtype == 1, "dtype must be 0 (fp16) or 1 (bf16)");
+  TCCL_CHECK_ARG(n % 8 == 0 && h_ld % 8 == 0 && dy_ld % 8 == 0 && dh_ld % 8 == 0,
+                 "row lengths and pitches must be multiples of 8 elements");
+  TCCL_CHECK_ARG(h % 16 == 0 && dy % 16 == 0 && dh % 16 == 0, "rows must be 16-byte aligned");
+  CombineParams p = {};
+  p.h = reinterpret_cast<const uint4*>(h);
+  p.h_ld = h_ld / 8;
+  p.slot_of = reinterpret_cast<const int32_t*>(slot_of);
+  p.weights = reinterpret_cast<const float*>(weights);
+  p.dy = reinterpret_cast<const uint4*>(dy);
+  p.dy_ld = dy_ld / 8;
+  p.dh = reinterpret_cast<uint4*>(dh);
+  p.dh_ld = dh_ld / 8;
+  p.dw = reinterpret_cast<float*>(dw);
+  p.tokens = tokens;
+  p.slots = slots;
+  p.top_k = top_k;
+  p.vecs = n / 8;
+  p.bf16 = dtype;
+  const int rc = check(p);
+  if (rc) return rc;
+  if (tokens == 0) return kOk;
+  TCCL_CHECK_ARG(h != 0 && slot_of != 0 && weights != 0 && dy != 0 && dh != 0 && dw != 0,
+                 "null argument");
+  expert_combine_backward_kernel<<<static_cast<unsigned>(tokens), kThreads, 0,
+                                   reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  TCCL_CHECK_CUDA(cudaGetLastError());
+  return kOk;
+}

@@ -21,6 +21,10 @@ cudaError_t preload_gemm_kernels();
 cudaError_t preload_collective_kernels();
 cudaError_t preload_push_kernels();
 cudaError_t preload_prim_kernels();
+cudaError_t preload_expert_route_kernels();
+cudaError_t preload_expert_slot_kernels();
+cudaError_t preload_expert_gemm_kernels();
+cudaError_t preload_expert_combine_kernels();
 cudaError_t launch_wait_groups(const uint32_t* sig, int sig_stride, int n_src, int n_groups,
                                const uint32_t* per_epoch, uint32_t epoch, int skip_src,
                                uint32_t* status, uint64_t budget_ns, int rank,
@@ -423,5 +427,9 @@ extern "C" int tccl_preload_kernels(void) {
   TCCL_CHECK_CUDA(preload_collective_kernels());
   TCCL_CHECK_CUDA(preload_push_kernels());
   TCCL_CHECK_CUDA(preload_prim_kernels());
+  TCCL_CHECK_CUDA(preload_expert_route_kernels());
+  TCCL_CHECK_CUDA(preload_expert_slot_kernels());
+  TCCL_CHECK_CUDA(preload_expert_gemm_kernels());
+  TCCL_CHECK_CUDA(preload_expert_combine_kernels());
   return kOk;
 }

@@ -1,0 +1,449 @@
+"""Mixture-of-experts operators: routing, slot map, grouped products, combine, and their
+backward passes (``csrc/kernels/expert_*.cu``).
+
+A layer runs them in this order::
+
+    weights, ids = route_experts(logits, top_k)            # [tokens, top_k]
+    slots = expert_slots(ids, num_experts)                 # (token, choice) pairs by expert
+    h = expert_gemm(x, w_gate_up, slots, epilogue="silu_gate")
+    y = expert_gemm(h, w_down, slots, rows="slots")
+    out = expert_combine(y, slots, weights)                # [tokens, hidden]
+
+Nothing here synchronises with the host: how many rows an expert has stays on the GPU, and
+every shape depends on ``tokens * top_k`` alone, so a layer can be captured into a CUDA graph.
+All results repeat bit for bit from call to call.
+
+``stream``: the stream to run on (default: the current stream of the tensors' device).  Results
+are allocated on that stream; the caller orders it behind the work that produced the inputs.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from contextlib import contextmanager
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .. import _native
+from . import fused_gemm as _fg
+
+MAX_ROUTED_EXPERTS = 512
+MAX_EXPERTS = 1024
+MAX_TOP_K = 32
+
+_LOGIT_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_EPILOGUES = {"none": 0, "silu_gate": 1}
+_EPI_SILU_GATE_GRAD = 2
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORES = {"top2": 0, "max": 1}
+_ROWS = ("tokens", "slots")
+
+
+# --------------------------------------------------------------------------- checks
+def _choice(name: str, value, table):
+    if value not in table:
+        raise ValueError(f"{name} must be one of {tuple(table)}, got {value!r}")
+    return table[value] if isinstance(table, dict) else value
+
+
+def _check_tensor(name: str, t, dim: int, dtypes, device=None, *, contiguous: bool = False):
+    if not isinstance(t, torch.Tensor) or t.dim() != dim:
+        raise ValueError(f"{name} must be a {dim}-D tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must have dtype {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t
+
+
+def _pitch(name: str, t) -> int:
+    """Elements between rows of a row-major matrix (the last two dimensions of ``t``)."""
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{name} must be row-major with unit column stride")
+    if t.shape[-2] <= 1:
+        return t.shape[-1]
+    if t.stride(-2) < t.shape[-1]:
+        raise ValueError(f"{name} has rows that overlap (row stride {t.stride(-2)}, "
+                         f"{t.shape[-1]} columns)")
+    return t.stride(-2)
+
+
+_HALF = (torch.float16, torch.bfloat16)
+
+
+@contextmanager
+def _on(stream, inputs):
+    """Current device and stream of a launch; yields the raw stream.  Inputs that are used on
+    another stream than the current one are reported to the caching allocator."""
+    dev = inputs[0].device
+    if dev.type != "cuda":
+        raise ValueError(f"the expert operators take CUDA tensors, got tensors on {dev}")
+    with torch.cuda.device(dev):
+        if stream is None:
+            yield torch.cuda.current_stream(dev).cuda_stream
+        else:
+            if stream.device != dev:
+                raise ValueError(f"stream is on {stream.device}, the tensors are on {dev}")
+            for t in inputs:
+                if t is not None:
+                    t.record_stream(stream)
+            with torch.cuda.stream(stream):
+                yield stream.cuda_stream
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _launch(fn: str, *args) -> None:
+    _native.call(fn, *args)
+    _fg.count_launches(1)
+
+
+# -------------------------------------------------------------------------- routing
+def _check_routing(logits, top_k, score, scale):
+    _check_tensor("logits", logits, 2, tuple(_LOGIT_DTYPES))
+    tokens, experts = logits.shape
+    if not 1 <= experts <= MAX_ROUTED_EXPERTS:
+        raise ValueError(f"logits have {experts} experts, supported are 1..{MAX_ROUTED_EXPERTS}")
+    if not 1 <= top_k <= min(MAX_TOP_K, experts):
+        raise ValueError(f"top_k={top_k} must be in 1..{min(MAX_TOP_K, experts)}")
+    return tokens, experts, _choice("score", score, _SCORES), float(scale)
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
+                  bias: Optional[torch.Tensor] = None, groups: int = 1,
+                  top_groups: Optional[int] = None, group_score: str = "top2",
+                  renormalize: bool = True, scale: float = 1.0,
+                  mask: Optional[torch.Tensor] = None,
+                  stream: Optional[torch.cuda.Stream] = None):
+    """The ``top_k`` experts of every token and their weights.
+
+    ``logits [tokens, experts]`` (fp32, bf16 or fp16; rows may be strided) become scores
+    ``p = softmax(logits)`` or ``sigmoid(logits)``.  An expert competes with ``p + bias``
+    (``bias``: fp32 ``[experts]``, a balance term that does not enter the weights).  With
+    ``groups > 1`` the experts form that many equal runs; a group counts by the sum of its two
+    largest competing values (``group_score="max"``: by its largest) and only the
+    ``top_groups`` best groups' experts stay.  Weights are ``scale * p`` of the chosen
+    experts, divided by their sum if ``renormalize``.
+
+    Returns ``(weights, ids)``: fp32 and int32 ``[tokens, top_k]``, best first, ties to the
+    lower index.  The choice is exact (made in 64 bits where 32 cannot tell).  A logit or bias
+    of ``-inf`` takes an expert out; a token whose ``mask`` (bool ``[tokens]``) is false, or
+    that has fewer than ``top_k`` experts left, gets id -1 and weight 0 in the places that
+    stay empty.  A NaN among an unmasked row's logits makes the row's weights NaN (its ids
+    stay distinct and in range).
+    """
+    tokens, experts, sig, scale = _check_routing(logits, top_k, score, scale)
+    if groups < 1 or groups > 32 or experts % groups:
+        raise ValueError(f"groups={groups} must be in 1..32 and divide the {experts} experts")
+    top_groups = groups if top_groups is None else top_groups
+    if not 1 <= top_groups <= groups:
+        raise ValueError(f"top_groups={top_groups} must be in 1..{groups}")
+    by_max = _choice("group_score", group_score, _GROUP_SCORES)
+    if bias is not None:
+        _check_tensor("bias", bias, 1, (torch.float32,), logits.device, contiguous=True)
+        if bias.shape[0] != experts:
+            raise ValueError(f"bias has {bias.shape[0]} entries for {experts} experts")
+    if mask is not None:
+        _check_tensor("mask", mask, 1, (torch.bool,), logits.device, contiguous=True)
+        if mask.shape[0] != tokens:
+            raise ValueError(f"mask has {mask.shape[0]} entries for {tokens} tokens")
+    ld = _pitch("logits", logits)
+    with _on(stream, (logits, bias, mask)) as raw:
+        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=logits.device)
+        ids = torch.empty((tokens, top_k), dtype=torch.int32, device=logits.device)
+        _launch("tccl_expert_route", logits.data_ptr(), ld, _ptr(bias), _ptr(mask),
+                weights.data_ptr(), ids.data_ptr(), tokens, experts, top_k,
+                _LOGIT_DTYPES[logits.dtype], sig, groups, top_groups, by_max,
+                1 if renormalize else 0, scale, raw)
+    return weights, ids
+
+
+def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, *,
+                           score: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+                           stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Gradient of the logits from ``grad_weights`` (fp32 ``[tokens, top_k]``) and the ``ids``
+    that :func:`route_experts` chose.  The choice itself has no gradient (so neither has
+    ``bias``); places with id -1 contribute nothing, tokens without any id get zeros."""
+    if not isinstance(ids, torch.Tensor) or ids.dim() != 2:
+        raise ValueError("ids must be a 2-D tensor")
+    top_k = ids.shape[1]
+    tokens, experts, sig, scale = _check_routing(logits, top_k, score, scale)
+    _check_tensor("ids", ids, 2, (torch.int32,), logits.device, contiguous=True)
+    _check_tensor("grad_weights", grad_weights, 2, (torch.float32,), logits.device, contiguous=True)
+    if tuple(ids.shape) != (tokens, top_k) or tuple(grad_weights.shape) != (tokens, top_k):
+        raise ValueError(f"ids {tuple(ids.shape)} and grad_weights {tuple(grad_weights.shape)} "
+                         f"must both be {(tokens, top_k)}")
+    ld = _pitch("logits", logits)
+    with _on(stream, (logits, ids, grad_weights)) as raw:
+        grad = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
+        _launch("tccl_expert_route_backward", grad_weights.data_ptr(), logits.data_ptr(), ld,
+                ids.data_ptr(), grad.data_ptr(), tokens, experts, top_k,
+                _LOGIT_DTYPES[logits.dtype], sig, 1 if renormalize else 0, scale, raw)
+    return grad
+
+
+# ------------------------------------------------------------------------- slot map
+@dataclass(frozen=True)
+class ExpertSlots:
+    """The (token, choice) pairs of a batch in the order of their experts.
+
+    ``offsets`` int32 ``[experts + 1]``: expert ``e`` has slots ``offsets[e]:offsets[e + 1]``;
+    ``token_of_slot`` int32 ``[tokens * top_k]``, -1 behind the last slot;
+    ``slot_of`` int32 ``[tokens, top_k]``, -1 for a choice without a slot.
+    """
+
+    offsets: torch.Tensor
+    token_of_slot: torch.Tensor
+    slot_of: torch.Tensor
+
+    def __post_init__(self) -> None:
+        _check_tensor("offsets", self.offsets, 1, (torch.int32,), contiguous=True)
+        dev = self.offsets.device
+        _check_tensor("token_of_slot", self.token_of_slot, 1, (torch.int32,), dev, contiguous=True)
+        _check_tensor("slot_of", self.slot_of, 2, (torch.int32,), dev, contiguous=True)
+        if not 1 <= self.num_experts <= MAX_EXPERTS:
+            raise ValueError(f"offsets must have 2..{MAX_EXPERTS + 1} entries")
+        if self.token_of_slot.shape[0] != self.slot_of.numel():
+            raise ValueError(f"token_of_slot has {self.token_of_slot.shape[0]} entries, "
+                             f"slot_of {self.slot_of.numel()}")
+
+    @property
+    def num_experts(self) -> int:
+        return self.offsets.shape[0] - 1
+
+    @property
+    def tokens(self) -> int:
+        return self.slot_of.shape[0]
+
+    @property
+    def top_k(self) -> int:
+        return self.slot_of.shape[1]
+
+    @property
+    def capacity(self) -> int:
+        """Rows of a slot-ordered matrix: ``tokens * top_k``."""
+        return self.token_of_slot.shape[0]
+
+
+def expert_slots(ids: torch.Tensor, num_experts: int, *, first_expert: int = 0,
+                 stream: Optional[torch.cuda.Stream] = None) -> ExpertSlots:
+    """Slot map of ``ids`` (int32 ``[tokens, top_k]``) for the experts
+    ``first_expert .. first_expert + num_experts`` that live here.  Ids outside that range
+    (another rank's experts, -1) get no slot.  Pairs of one expert keep the order of their
+    tokens."""
+    _check_tensor("ids", ids, 2, (torch.int32,), contiguous=True)
+    tokens, top_k = ids.shape
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ValueError(f"num_experts={num_experts} must be in 1..{MAX_EXPERTS}")
+    if not 0 <= first_expert < 1 << 31:
+        raise ValueError(f"first_expert={first_expert} must not be negative")
+    if top_k < 1 or tokens * top_k >= 1 << 31:
+        raise ValueError(f"ids have an unsupported shape {tuple(ids.shape)}")
+    dev = ids.device
+    with _on(stream, (ids,)) as raw:
+        offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+        token_of_slot = torch.empty(tokens * top_k, dtype=torch.int32, device=dev)
+        slot_of = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
+        need = C.c_int64()
+        _native.call("tccl_expert_slots_workspace", tokens * top_k, num_experts, C.byref(need))
+        scratch = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+        _launch("tccl_expert_slots", ids.data_ptr(), tokens, top_k, num_experts, first_expert,
+                offsets.data_ptr(), token_of_slot.data_ptr(), slot_of.data_ptr(), _ptr(scratch), raw)
+    return ExpertSlots(offsets, token_of_slot, slot_of)
+
+
+# ----------------------------------------------------------------- grouped products
+def _check_product(X, W, slots, rows, b_is_nk, epilogue):
+    _choice("rows", rows, _ROWS)
+    epi = _choice("epilogue", epilogue, _EPILOGUES)
+    if not isinstance(slots, ExpertSlots):
+        raise ValueError("slots must be an ExpertSlots")
+    _check_tensor("X", X, 2, _HALF)
+    _check_tensor("W", W, 3, (X.dtype,), X.device)
+    if slots.offsets.device != X.device:
+        raise ValueError(f"slots are on {slots.offsets.device}, X is on {X.device}")
+    E = W.shape[0]
+    N, K = (W.shape[1], W.shape[2]) if b_is_nk else (W.shape[2], W.shape[1])
+    if E != slots.num_experts:
+        raise ValueError(f"W has {E} experts, slots {slots.num_experts}")
+    if X.shape[1] != K:
+        raise ValueError(f"inner dimensions differ: X is {tuple(X.shape)}, W is {tuple(W.shape)}")
+    want = slots.tokens if rows == "tokens" else slots.capacity
+    if X.shape[0] != want:
+        raise ValueError(f"X has {X.shape[0]} rows, expected {want} for rows={rows!r}")
+    if K < 8 or N < 8 or K % 8 or N % 8:
+        raise ValueError(f"K={K} and N={N} must be multiples of 8 (16-byte rows)")
+    if epi and N % _fg.BLOCK_N:
+        raise ValueError(f"epilogue 'silu_gate' needs N={N} to be a multiple of {_fg.BLOCK_N} "
+                         "(128 gate columns followed by 128 up columns)")
+    return E, K, N, epi
+
+
+def _check_rows(name, t, shape, like):
+    _check_tensor(name, t, 2, (like.dtype,), like.device)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} is {tuple(t.shape)}, expected {shape}")
+    return _aligned(name, t)
+
+
+def _aligned(name, t) -> int:
+    ld = _pitch(name, t)
+    if ld % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name} must have 16-byte aligned rows")
+    return ld
+
+
+def _product(X, W, slots, out, rows, b_is_nk, epi, dh, raw):
+    """One launch of the grouped product; every argument is checked already."""
+    E = W.shape[0]
+    N, K = (W.shape[1], W.shape[2]) if b_is_nk else (W.shape[2], W.shape[1])
+    d = _native.ExpertGemm()
+    d.dtype, d.epilogue, d.experts, d.w_nk = _fg.dtype_code(X.dtype), epi, E, 1 if b_is_nk else 0
+    d.k, d.n, d.slots, d.x_rows = K, N, slots.capacity, X.shape[0]
+    d.offsets = slots.offsets.data_ptr()
+    d.token_of_slot = slots.token_of_slot.data_ptr() if rows == "tokens" else 0
+    d.x, d.w, d.out, d.dh = X.data_ptr(), W.data_ptr(), out.data_ptr(), _ptr(dh)
+    d.ldx, d.ldw, d.ldo = _aligned("X", X), _aligned("W", W), _aligned("out", out)
+    d.w_expert = W.stride(0) if E > 1 else W.shape[1] * d.ldw
+    if d.w_expert < (W.shape[1] - 1) * d.ldw + W.shape[2] or d.w_expert % 8:
+        raise ValueError("W's experts overlap or are not 16-byte aligned")
+    d.ld_dh = 0 if dh is None else _aligned("grad_out", dh)
+    _launch("tccl_expert_gemm", C.byref(d), raw)
+
+
+def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
+                out: Optional[torch.Tensor] = None, *, rows: str = "tokens",
+                b_is_nk: bool = False, epilogue: str = "none",
+                stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """``out[s] = X[row of slot s] @ W[expert of slot s]`` (fp16 / bf16, fp32 accumulation).
+
+    ``rows="tokens"``: ``X [tokens, K]``, gathered through the slot map; ``rows="slots"``: ``X
+    [tokens * top_k, K]``, one row per slot.  ``W`` is ``[experts, K, N]``, or ``[experts, N,
+    K]`` with ``b_is_nk``.  ``epilogue="silu_gate"`` takes every 256 columns of the product as
+    128 gate columns followed by 128 up columns (``models.pack_gate_up`` of every expert) and
+    writes ``silu(gate) * up``, half as wide.  Rows of ``out [tokens * top_k, N]`` behind the
+    last slot keep what they held.  ``out`` must not overlap an input.
+    """
+    E, K, N, epi = _check_product(X, W, slots, rows, b_is_nk, epilogue)
+    shape = (slots.capacity, N // 2 if epi else N)
+    if out is not None:
+        _check_rows("out", out, shape, X)
+    with _on(stream, (X, W, slots.offsets, slots.token_of_slot, out)) as raw:
+        if out is None:
+            out = torch.empty(shape, dtype=X.dtype, device=X.device)
+        _product(X, W, slots, out, rows, b_is_nk, epi, None, raw)
+    return out
+
+
+def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tensor,
+                         slots: ExpertSlots, *, rows: str = "tokens", b_is_nk: bool = False,
+                         epilogue: str = "none", stream: Optional[torch.cuda.Stream] = None):
+    """``(grad_X, grad_W)`` of :func:`expert_gemm` for ``grad_out`` (shaped like its result).
+
+    With ``epilogue="silu_gate"`` gate and up are computed again from ``X`` and ``W``, so the
+    forward pass keeps nothing.  ``grad_X`` has ``X``'s shape: with ``rows="tokens"`` the sum
+    over a token's slots (zero for a token without one), with ``rows="slots"`` one row per
+    slot, undefined behind the last slot.  ``grad_W`` has ``W``'s shape and is contiguous;
+    experts without a slot get zeros.
+    """
+    E, K, N, epi = _check_product(X, W, slots, rows, b_is_nk, epilogue)
+    _check_rows("grad_out", grad_out, (slots.capacity, N // 2 if epi else N), X)
+    S = slots.capacity
+    with _on(stream, (X, W, grad_out, slots.offsets, slots.token_of_slot, slots.slot_of)) as raw:
+        dy = grad_out
+        if epi:
+            # gate and up again, their gradients straight from the accumulators (one rounding
+            # to 16 bits: the operand type of the two products that follow)
+            dy = torch.empty((S, N), dtype=X.dtype, device=X.device)
+            _product(X, W, slots, dy, rows, b_is_nk, _EPI_SILU_GATE_GRAD, grad_out, raw)
+        grad_rows = torch.empty((S, K), dtype=X.dtype, device=X.device)
+        _product(dy, W, slots, grad_rows, "slots", not b_is_nk, 0, None, raw)
+        grad_X = grad_rows
+        if rows == "tokens":
+            grad_X = torch.empty((slots.tokens, K), dtype=X.dtype, device=X.device)
+            _combine(grad_rows, slots, None, None, grad_X, raw)
+        grad_W = torch.empty(W.shape, dtype=X.dtype, device=X.device)
+        d = _native.ExpertWeightGrad()
+        d.dtype, d.experts, d.slots = _fg.dtype_code(X.dtype), E, S
+        d.offsets, d.token_of_slot = slots.offsets.data_ptr(), slots.token_of_slot.data_ptr()
+        a, b = (dy, X) if b_is_nk else (X, dy)
+        d.gather_a = 1 if rows == "tokens" and a is X else 0
+        d.gather_b = 1 if rows == "tokens" and b is X else 0
+        d.m, d.n, d.a_rows, d.b_rows = a.shape[1], b.shape[1], a.shape[0], b.shape[0]
+        d.a, d.b, d.out = a.data_ptr(), b.data_ptr(), grad_W.data_ptr()
+        d.lda, d.ldb = _aligned("X", a), _aligned("X", b)
+        _launch("tccl_expert_weight_grad", C.byref(d), raw)
+    return grad_X, grad_W
+
+
+# -------------------------------------------------------------------------- combine
+def _combine(H, slots, weights, add, out, raw):
+    _launch("tccl_expert_combine", H.data_ptr(), _aligned("H", H), slots.slot_of.data_ptr(),
+            _ptr(weights), _ptr(add), 0 if add is None else _aligned("add", add), out.data_ptr(),
+            _aligned("out", out), slots.tokens, slots.capacity, slots.top_k, H.shape[1],
+            _fg.dtype_code(H.dtype), raw)
+
+
+def _check_combine(H, slots, weights):
+    if not isinstance(slots, ExpertSlots):
+        raise ValueError("slots must be an ExpertSlots")
+    _check_tensor("H", H, 2, _HALF, slots.offsets.device)
+    if H.shape[0] != slots.capacity:
+        raise ValueError(f"H has {H.shape[0]} rows, expected {slots.capacity}")
+    if H.shape[1] < 8 or H.shape[1] % 8:
+        raise ValueError(f"H has {H.shape[1]} columns, which must be a multiple of 8")
+    _aligned("H", H)
+    if weights is not None:
+        _check_tensor("weights", weights, 2, (torch.float32,), H.device, contiguous=True)
+        if tuple(weights.shape) != (slots.tokens, slots.top_k):
+            raise ValueError(f"weights are {tuple(weights.shape)}, expected "
+                             f"{(slots.tokens, slots.top_k)}")
+
+
+def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None, *, add: Optional[torch.Tensor] = None,
+                   stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """``out[t] = add[t] + sum_j weights[t, j] * H[slot_of[t, j]]`` in fp32, rounded once.
+
+    ``H [tokens * top_k, N]`` is slot-ordered (fp16 / bf16), ``weights`` fp32 ``[tokens,
+    top_k]`` (None: all ones), ``add [tokens, N]`` a residual or a shared expert's output.
+    Choices without a slot add nothing.  ``out`` may be ``add`` (in place) but must not overlap
+    ``H``.
+    """
+    _check_combine(H, slots, weights)
+    shape = (slots.tokens, H.shape[1])
+    if add is not None:
+        _check_rows("add", add, shape, H)
+    if out is not None:
+        _check_rows("out", out, shape, H)
+    with _on(stream, (H, weights, add, slots.slot_of, out)) as raw:
+        if out is None:
+            out = torch.empty(shape, dtype=H.dtype, device=H.device)
+        _combine(H, slots, weights, add, out, raw)
+    return out
+
+
+def expert_combine_backward(grad_out: torch.Tensor, H: torch.Tensor, slots: ExpertSlots,
+                            weights: torch.Tensor, *,
+                            stream: Optional[torch.cuda.Stream] = None):
+    """``(grad_H, grad_weights)`` of :func:`expert_combine`.  Rows of ``grad_H`` behind the last
+    slot are undefined; choices without a slot have weight gradient 0.  (The gradient of
+    ``add`` is ``grad_out`` itself.)"""
+    if weights is None:
+        raise ValueError("weights must be a 2-D tensor")
+    _check_combine(H, slots, weights)
+    _check_rows("grad_out", grad_out, (slots.tokens, H.shape[1]), H)
+    with _on(stream, (H, weights, grad_out, slots.slot_of)) as raw:
+        grad_H = torch.empty(H.shape, dtype=H.dtype, device=H.device)
+        grad_weights = torch.empty(weights.shape, dtype=torch.float32, device=H.device)
+        _launch("tccl_expert_combine_backward", grad_out.data_ptr(), _aligned("grad_out", grad_out),
+                H.data_ptr(), _aligned("H", H), slots.slot_of.data_ptr(), weights.data_ptr(),
+                grad_H.data_ptr(), _aligned("grad_H", grad_H), grad_weights.data_ptr(),
+                slots.tokens, slots.capacity, slots.top_k, H.shape[1], _fg.dtype_code(H.dtype), raw)
+    return grad_H, grad_weights

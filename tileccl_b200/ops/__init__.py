@@ -16,6 +16,10 @@ Two layout families exist for the GEMM + collective ops:
 
 Both run on the same fused tcgen05 kernel (``csrc/kernels/gemm_sm100.cu``); no
 library GEMM or NCCL call is involved.
+
+The mixture-of-experts operators (``route_experts``, ``expert_slots``,
+``expert_gemm``, ``expert_combine`` and their backward passes) work on one GPU's
+tensors and need no context.
 """
 
 from __future__ import annotations
@@ -27,6 +31,9 @@ import torch
 
 from . import _fused
 from ._fused import call_stats, check_status, recover
+from ..kernels.experts import (ExpertSlots, expert_combine, expert_combine_backward, expert_gemm,
+                               expert_gemm_backward, expert_slots, route_experts,
+                               route_experts_backward)
 from ..kernels.fused_gemm import TileCCLTimeoutError
 from ..primitives import collectives as _coll
 
@@ -42,6 +49,8 @@ __all__ = [
     "ReduceScatterPlan",
     "GemmAllScatterContract", "GemmAllGatherContract", "GemmReduceScatterContract",
     "AllGatherGemmReduceScatterContract",
+    "route_experts", "route_experts_backward", "expert_slots", "ExpertSlots", "expert_gemm",
+    "expert_gemm_backward", "expert_combine", "expert_combine_backward",
     "check_status", "recover", "call_stats", "TileCCLTimeoutError",
 ]
 
