@@ -175,6 +175,7 @@ class ExpertGemm(C.Structure):
         ("w_expert", C.c_int64),
         ("ldo", C.c_int64),
         ("ld_dh", C.c_int64),
+        ("status", C.c_uint64),
     ]
 
 
@@ -196,6 +197,7 @@ class ExpertWeightGrad(C.Structure):
         ("out", C.c_uint64),
         ("lda", C.c_int64),
         ("ldb", C.c_int64),
+        ("status", C.c_uint64),
     ]
 
 

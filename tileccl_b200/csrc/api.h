@@ -333,6 +333,7 @@ typedef struct TcclExpertGemm {
   uint64_t token_of_slot;     // int32[slots]; 0 = row s of x belongs to slot s
   uint64_t x, w, out, dh;     // dh: epilogue 2 only
   int64_t ldx, ldw, w_expert, ldo, ld_dh;   // pitches in elements
+  uint64_t status;            // uint32[8] status words (0 = a wait that gave up is not reported)
 } TcclExpertGemm;
 int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream);
 
@@ -342,6 +343,7 @@ typedef struct TcclExpertWeightGrad {
   int64_t m, n, slots, a_rows, b_rows;
   uint64_t offsets, token_of_slot, a, b, out;
   int64_t lda, ldb;
+  uint64_t status;
 } TcclExpertWeightGrad;
 int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_t stream);
 

@@ -1,5 +1,5 @@
 // Products of the experts over a slot map (expert_slots.cu): every slot's row times the weight
-// matrix of its expert, and the gradient of those weights.
+// matrix of its expert, and the gradient of those weights, on the sm_100a tensor cores.
 //
 //   out[s] = x[row(s)] @ W[e(s)]                                row(s) = token of slot s, or s
 //   SiLU gate: W's columns come as 128 gate columns followed by 128 up columns;
@@ -7,12 +7,16 @@
 //   gradient of the gate: gate and up are computed again and with dh[s] = dL/dout[s]
 //              dgate = dh * up * sg * (1 + gate * (1 - sg)),  dup = dh * gate * sg,
 //              sg = 1 / (1 + e^-gate), packed like W's columns
-//   dW[e] = sum over the slots of e of x[row(s)]^T dy[s]
+//   dW[e] = sum over the slots of e of a[row(s)]^T b[row(s)]
 //
-// 64 x 64 tiles, fp32 accumulation on the CUDA cores.
+// Both kernels are persistent: a cluster of two CTAs per tile, tcgen05.mma.cta_group::2, a TMA
+// ring of operand stages, two accumulators in TMEM so that the epilogue of one tile runs under
+// the next tile's products.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "../api.h"
+#include "../device/ptx.cuh"
 #include "../device/tile_compute.cuh"
 #include "../runtime/errors.h"
 
@@ -21,145 +25,711 @@ namespace {
 
 enum Epilogue : int { kNone = 0, kSiluGate = 1, kSiluGateGrad = 2 };
 
-__device__ __forceinline__ float load16(const void* base, int64_t i, bool bf16) {
-  return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i])
-              : __half2float(static_cast<const __half*>(base)[i]);
+constexpr int kMaxExperts = 1024;
+constexpr int kThreads = 256;            // warp 0 TMA, 1 MMA, 2 TMEM, 3 idle, 4-7 epilogue
+constexpr int kEpiThreads = 128;
+constexpr int kStages = 6;
+constexpr int kBK = 64;                  // contraction elements per stage (one 128-byte row)
+constexpr int kUmmaK = 16;
+constexpr int kHalfBytes = 64 * 128;     // 64 rows of 128 bytes: one TMA box, 8 KB
+constexpr int kOperandBytes = 2 * kHalfBytes;
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kTile = 256;               // features (M) and, at most, tokens (N) of a pair's tile
+constexpr int kAccCols = 256;            // TMEM columns of one accumulator
+constexpr int kBand = 16;                // token tiles that share a sweep over the features
+constexpr int kChunk = 16;               // tokens per epilogue step
+constexpr int kStageLd = 132;            // floats between tokens of the staging buffer
+constexpr int kStagingBytes = 2 * kChunk * kStageLd * 4;
+constexpr int kCtlBytes = 512;
+constexpr int kListBytes = 2 * 4 * (kMaxExperts + 2);
+constexpr int kGemmSmem = kStages * kStageBytes + kStagingBytes + kCtlBytes + kListBytes + 1024;
+constexpr int kGradStagingBytes = 4 * 2 * 4096;   // per epilogue warp two buffers of 32 x 64
+constexpr int kGradSmem = kStages * kStageBytes + kGradStagingBytes + kCtlBytes + 1024;
+static_assert(kGemmSmem <= 232448 && kGradSmem <= 232448, "shared memory of one SM");
+
+struct GemmParams {
+  CUtensorMap tma_w;          // {columns, rows, experts}, box {64, 64, 1}, 128-byte swizzle
+  CUtensorMap tma_x;          // {K, rows}, box {64, 16}, gathered: {64, 1}
+  const int32_t* offsets;
+  const int32_t* token_of_slot;
+  void* out;
+  const void* dh;
+  int64_t ldo, ld_dh;
+  int32_t slots, x_rows, experts, k_blocks, n, f_tiles, bf16, w_nk;
+  uint32_t* status;
+  uint64_t budget_ns;
+};
+
+struct GradParams {
+  CUtensorMap tma_a, tma_b;           // {columns, rows}, box {64, 64}
+  CUtensorMap tma_a_rows, tma_b_rows; // the same, box {64, 1}, for single rows
+  CUtensorMap tma_out;                // {n, m, experts}, box {64, 32, 1}
+  const int32_t* offsets;
+  const int32_t* token_of_slot;
+  int32_t slots, a_rows, b_rows, experts, m, n, m_tiles, n_tiles, bf16, gather_a, gather_b;
+  uint32_t* status;
+  uint64_t budget_ns;
+};
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* m, int x, int y,
+                                                 int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile"
+      ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
 }
-__device__ __forceinline__ void store16(void* base, int64_t i, bool bf16, float v) {
-  if (bf16) static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16(v);
-  else static_cast<__half*>(base)[i] = __float2half(v);
+// Four rows of a matrix, 64 columns each, into 512 consecutive bytes (swizzled by address).
+__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap* m, int x,
+                                                 const int (&r)[4], uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4"
+      ".mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+      "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, int x, int y, int z,
+                                             uint32_t src) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+          reinterpret_cast<uint64_t>(m)),
+      "r"(x), "r"(y), "r"(z), "r"(src)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Barrier of the epilogue warps that also agrees on a condition.
+__device__ __forceinline__ bool epilogue_all(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(ok ? 1u : 0u)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void epilogue_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
+// Shared memory of a CTA pair.  Every CTA has all barriers; in use are the leader's "full" and
+// "accumulator empty" (both CTAs report to them) and both CTAs' "empty" and "accumulator full"
+// (signalled by multicast commits).
+struct Pipe {
+  uint32_t base, staging, ctl;
+  uint32_t full, empty, acc_full, acc_empty, drain, tmem_slot;
+  volatile uint32_t* words;        // generic view of tmem_slot: [0] TMEM base, [1] abort flag
+  int32_t* start;                  // [experts + 1] first slot of every expert
+  int32_t* tiles;                  // [experts + 1] tiles of all lower experts
+};
+
+__device__ __forceinline__ Pipe make_pipe(uint8_t* raw, int staging_bytes) {
+  Pipe s;
+  s.base = (smem_u32(raw) + 1023u) & ~1023u;
+  s.staging = s.base + kStages * kStageBytes;
+  s.ctl = s.staging + staging_bytes;
+  s.full = s.ctl;
+  s.empty = s.full + 8 * kStages;
+  s.acc_full = s.empty + 8 * kStages;
+  s.acc_empty = s.acc_full + 16;
+  s.drain = s.acc_empty + 16;
+  s.tmem_slot = s.drain + 8;
+  uint8_t* const g = raw + (s.ctl - smem_u32(raw));
+  s.words = reinterpret_cast<volatile uint32_t*>(g + (s.tmem_slot - s.ctl));
+  s.start = reinterpret_cast<int32_t*>(g + kCtlBytes);
+  s.tiles = s.start + kMaxExperts + 2;
+  return s;
 }
 
-__device__ __forceinline__ int slot_bound(const TcclExpertGemm& d, int e) {
-  const int v = reinterpret_cast<const int32_t*>(d.offsets)[e];
-  return v < 0 ? 0 : v > d.slots ? static_cast<int>(d.slots) : v;
-}
-__device__ __forceinline__ int64_t source_row(const TcclExpertGemm& d, int s) {
-  if (d.token_of_slot == 0) return s;
-  const int t = reinterpret_cast<const int32_t*>(d.token_of_slot)[s];
-  return t >= 0 && t < d.x_rows ? t : 0;
-}
-
-__global__ void __launch_bounds__(256) expert_gemm_kernel(const TcclExpertGemm d) {
-  __shared__ float xs[16][65], ws[16][65], us[16][65];
-  __shared__ int tile_e, tile_row, tile_end;
-  const bool bf16 = d.dtype == 1;
+// Barriers and TMEM of a CTA pair; returns the TMEM base.  Ends in a barrier of the pair, so
+// what a thread wrote to shared memory before is visible to its CTA afterwards.
+__device__ __forceinline__ uint32_t pipe_start(const Pipe& s) {
   if (threadIdx.x == 0) {
-    int left = blockIdx.y;
-    tile_e = -1;
-    for (int e = 0; e < d.experts; ++e) {
-      const int a = slot_bound(d, e), b = slot_bound(d, e + 1);
-      const int tiles = b > a ? (b - a + 63) / 64 : 0;
-      if (left < tiles) { tile_e = e; tile_row = a + left * 64; tile_end = b; break; }
-      left -= tiles;
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(s.full + 8 * i, 1);
+      mbar_init(s.empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s.acc_full + 8 * i, 1);
+      mbar_init(s.acc_empty + 8 * i, 8);     // four epilogue warps of both CTAs
+    }
+    mbar_init(s.drain, 1);
+    s.words[1] = 0;
+    mbar_fence_init();
+  }
+  if ((threadIdx.x >> 5) == 2) {
+    tmem_alloc_pair(s.tmem_slot, 2 * kAccCols);
+    tmem_relinquish_pair();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tcgen05_fence_after();
+  return s.words[0];
+}
+
+__device__ __forceinline__ int slot_bound(const int32_t* offsets, int e, int slots) {
+  return min(max(offsets[e], 0), slots);
+}
+
+// The list of tiles: expert e has tiles_of(rows of e) of them.  The counts per expert live on
+// the GPU only, so every CTA derives the whole schedule from the offsets.
+template <typename F>
+__device__ __forceinline__ void list_tiles(const Pipe& s, const int32_t* offsets, int slots,
+                                           int experts, F tiles_of) {
+  __shared__ int32_t warp_sum[kThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kPer = kMaxExperts / kThreads;
+  int32_t count[kPer];
+  int32_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = threadIdx.x * kPer + i;
+    count[i] = 0;
+    if (e < experts) {
+      const int a = slot_bound(offsets, e, slots), b = slot_bound(offsets, e + 1, slots);
+      s.start[e] = a;
+      if (e == experts - 1) s.start[experts] = b;
+      count[i] = tiles_of(max(b - a, 0));
+    }
+    sum += count[i];
+  }
+  int32_t scan = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) warp_sum[warp] = scan;
+  __syncthreads();
+  int32_t at = scan - sum;
+  for (int w = 0; w < warp; ++w) at += warp_sum[w];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = threadIdx.x * kPer + i;
+    if (e < experts) {
+      s.tiles[e] = at;
+      at += count[i];
+      if (e == experts - 1) s.tiles[experts] = at;
     }
   }
+}
+
+// Neither CTA of a pair may retire while its partner can still read its operands or touch its
+// barriers; TMEM goes back after every MMA and TMEM read is done.
+__device__ __forceinline__ void pipe_end(uint32_t tmem_base) {
+  tcgen05_fence_before();
   __syncthreads();
-  if (tile_e < 0) return;
-  const bool gate = d.epilogue != kNone;
-  const int n_cols = static_cast<int>(gate ? d.n / 2 : d.n);
-  const int f0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {}, up[4][4] = {};
-  const void* x = reinterpret_cast<const void*>(d.x);
-  const void* w = reinterpret_cast<const void*>(d.w);
-  for (int64_t k0 = 0; k0 < d.k; k0 += 16) {
-    for (int i = threadIdx.x; i < 16 * 64; i += 256) {
-      const int kk = i & 15, r = i >> 4;
-      const int s = tile_row + r;
-      xs[kk][r] = s < tile_end && k0 + kk < d.k ? load16(x, source_row(d, s) * d.ldx + k0 + kk, bf16) : 0.f;
-      const int f = f0 + r;
-      const int64_t c = gate ? (f / 128) * 256 + f % 128 : f;
-      const bool ok = f < n_cols && k0 + kk < d.k;
-      auto at = [&](int64_t col) {
-        return tile_e * d.w_expert + (d.w_nk ? col * d.ldw + k0 + kk : (k0 + kk) * d.ldw + col);
-      };
-      ws[kk][r] = ok ? load16(w, at(c), bf16) : 0.f;
-      us[kk][r] = ok && gate ? load16(w, at(c + 128), bf16) : 0.f;
-    }
-    __syncthreads();
-    for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
+  cluster_sync_all();
+  if ((threadIdx.x >> 5) == 2) {
+    tcgen05_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * kAccCols);
+  }
+}
+
+// After a wait that gave up: copies still in flight get two milliseconds to land.
+__device__ __forceinline__ void drain_copies() {
+  const uint64_t until = globaltimer_ns() + 2000000ull;
+  for (int i = 0; i < 1000000 && globaltimer_ns() < until; ++i) __nanosleep(1000);
+}
+
+__device__ __forceinline__ int expert_of(const Pipe& s, int experts, int t) {
+  int lo = 0, hi = experts;                    // tiles[lo] <= t < tiles[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s.tiles[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void store_row8(void* base, int64_t i, bool bf16, const float* v) {
+  *reinterpret_cast<uint4*>(static_cast<char*>(base) + 2 * i) = tile_cast_f32x8(bf16, v);
+}
+
+// ---------------------------------------------------------------------------------------
+// out[s] = epilogue(x[row(s)] @ W[e(s)])
+//
+// The weights are the M operand (256 features per pair, 128 per CTA) and the tokens the N
+// operand: M is fixed to 256 by the pair form of the instruction while N may be any multiple
+// of 32, so an expert's tile is as wide as its rows need.  With the gate a CTA's 128 features
+// are 64 gate columns and the 64 up columns that belong to them.
+// ---------------------------------------------------------------------------------------
+struct Item {
+  int e, row0, rows, n, f0;
+};
+
+template <int kEpi, bool kGather>
+__global__ void __launch_bounds__(kThreads, 1)
+expert_gemm_kernel(const __grid_constant__ GemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const Pipe s = make_pipe(smem_raw, kStagingBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = static_cast<int>(cluster_ctarank());
+  const bool leader = cta == 0;
+  list_tiles(s, p.offsets, p.slots, p.experts,
+             [&](int rows) { return (rows + kTile - 1) / kTile * p.f_tiles; });
+  const uint32_t tmem_base = pipe_start(s);
+  WaitBudget wb;
+  wb.start(p.budget_ns, s.words + 1);
+
+  const int total = s.tiles[p.experts];
+  const int step = static_cast<int>(gridDim.x >> 1);
+  // Tile t: token tiles run fastest, in bands of kBand, so that the tiles in flight share both
+  // their weights and a band of tokens in L2.
+  auto item_of = [&](int t) {
+    Item it;
+    it.e = expert_of(s, p.experts, t);
+    const int rows = s.start[it.e + 1] - s.start[it.e];
+    const int tiles = (rows + kTile - 1) / kTile;
+    int local = t - s.tiles[it.e];
+    const int band = local / (kBand * p.f_tiles);
+    local -= band * kBand * p.f_tiles;
+    const int wide = min(kBand, tiles - band * kBand);
+    const int ti = band * kBand + local % wide;
+    it.f0 = local / wide * kTile;
+    const int per = ((rows + tiles - 1) / tiles + 31) & ~31;   // even shares, a multiple of 32
+    it.row0 = s.start[it.e] + ti * per;
+    it.rows = min(per, rows - ti * per);
+    it.n = (max(it.rows, 1) + 31) & ~31;
+    return it;
+  };
+
+  if (warp == 0) {
+    // ------------------------------- TMA producer -------------------------------
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
+      const Item it = item_of(t);
+      const int mine = it.n >> 1;                          // token rows this CTA stages
+      const int first = it.row0 + cta * mine;
+      int r[4] = {};
+      if (kGather) {
+        // Rows behind the tile's last slot (and tokens that do not exist) are read out of
+        // range: the copy fills them with zeros.
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          acc[i][j] = fmaf(xs[kk][ty * 4 + i], ws[kk][tx * 4 + j], acc[i][j]);
-          if (gate) up[i][j] = fmaf(xs[kk][ty * 4 + i], us[kk][tx * 4 + j], up[i][j]);
+          const int slot = first + 4 * lane + j;
+          int tok = -1;
+          if (4 * lane < mine && slot < it.row0 + it.rows) tok = p.token_of_slot[slot];
+          r[j] = tok >= 0 && tok < p.x_rows ? tok : p.x_rows;
         }
-    __syncthreads();
-  }
-  void* out = reinterpret_cast<void*>(d.out);
-  for (int i = 0; i < 4; ++i) {
-    const int64_t s = tile_row + ty * 4 + i;
-    if (s >= tile_end) continue;
-    for (int j = 0; j < 4; ++j) {
-      const int f = f0 + tx * 4 + j;
-      if (f >= n_cols) continue;
-      const float g = acc[i][j], u = up[i][j];
-      const float sg = 1.f / (1.f + __expf(-g));
-      if (d.epilogue == kNone) {
-        store16(out, s * d.ldo + f, bf16, g);
-      } else if (d.epilogue == kSiluGate) {
-        store16(out, s * d.ldo + f, bf16, g * sg * u);
-      } else {
-        const int64_t c = (f / 128) * 256 + f % 128;
-        const float dh = load16(reinterpret_cast<const void*>(d.dh), s * d.ld_dh + f, bf16);
-        store16(out, s * d.ldo + c, bf16, dh * u * sg * (1.f + g * (1.f - sg)));
-        store16(out, s * d.ldo + c + 128, bf16, dh * g * sg);
+      }
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb));
+        if (!ok) {
+          if (lane == 0) report_status(p.status, kStatusTimeoutMbarrier, 101, 0, kb, 0, t);
+          break;
+        }
+        const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+        const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
+        if (lane == 0) {
+          // the bytes of both CTAs are counted on the leader's barrier
+          if (leader) mbar_expect_tx(s.full + 8 * stage, 2 * (kOperandBytes + mine * 128));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int f = kEpi == kNone ? it.f0 + cta * 128 + h * 64 : it.f0 + h * 128 + cta * 64;
+            if (p.w_nk) tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, kb * kBK, f, it.e, bar);
+            else tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, f, kb * kBK, it.e, bar);
+          }
+          if (!kGather)
+            for (int i = 0; i < mine; i += 16)
+              tma_load_2d_pair(sb + i * 128, &p.tma_x, kb * kBK, first + i, bar);
+        }
+        if (kGather && 4 * lane < mine) tma_gather4_pair(sb + lane * 512, &p.tma_x, kb * kBK, r, bar);
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
     }
+    if (!ok) drain_copies();
+  } else if (warp == 1 && leader) {
+    // ----------------------- MMA issuer (leader CTA only) -----------------------
+    if (elect_one_sync()) {
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
+        const Item it = item_of(t);
+        const uint32_t idesc = umma_idesc_f16(p.bf16, p.w_nk ? 0 : 1, 0, kTile, it.n);
+        if (!mbar_wait(s.acc_empty + 8 * acc, acc_phase ^ 1u, wb)) {
+          report_status(p.status, kStatusTimeoutMbarrier, 102, 0, 0, 0, t);
+          ok = false;
+          break;
+        }
+        tcgen05_fence_after();
+        const uint32_t d = tmem_base + acc * kAccCols;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(s.full + 8 * stage, phase, wb)) {
+            report_status(p.status, kStatusTimeoutMbarrier, 103, p.k_blocks, kb, 0, t);
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after();
+          const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+#pragma unroll
+          for (int k = 0; k < kBK / kUmmaK; ++k) {
+            const uint64_t da = p.w_nk ? umma_smem_desc_sw128(sa + k * kUmmaK * 2, 16, 1024)
+                                       : umma_smem_desc_sw128(sa + k * kUmmaK * 128, kHalfBytes, 1024);
+            const uint64_t db = umma_smem_desc_sw128(sb + k * kUmmaK * 2, 16, 1024);
+            umma_f16_pair(d, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+          }
+          umma_commit_pair(s.empty + 8 * stage, 3);
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit_pair(s.acc_full + 8 * acc, 3);
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      if (!ok) {
+        umma_commit_pair(s.drain, 1);       // outstanding MMAs end before TMEM is released
+        for (int i = 0; i < 1000000 && !mbar_try_wait(s.drain, 0); ++i) {}
+      }
+    }
+  } else if (warp >= 4) {
+    // --------------------------------- epilogue ---------------------------------
+    // A TMEM lane is a feature and a column a token; results are rows of features.  Sixteen
+    // tokens at a time cross over through shared memory in fp32: written by feature, read back
+    // by token, eight features per thread.
+    const int q = warp - 4, me = threadIdx.x - (kThreads - kEpiThreads);
+    float* const staging = reinterpret_cast<float*>(smem_raw + (s.staging - smem_u32(smem_raw)));
+    const bool bf16 = p.bf16 != 0;
+    constexpr int kVecs = kEpi == kNone ? 16 : 8;          // 8-feature vectors per token
+    uint32_t acc = 0, acc_phase = 0, buf = 0;
+    for (int t = blockIdx.x >> 1; t < total; t += step) {
+      const Item it = item_of(t);
+      if (!epilogue_all(mbar_wait(s.acc_full + 8 * acc, acc_phase, wb))) {
+        if (me == 0) report_status(p.status, kStatusTimeoutMbarrier, 104, 0, 0, 0, t);
+        break;
+      }
+      tcgen05_fence_after();
+      const uint32_t t_acc = tmem_base + acc * kAccCols + (static_cast<uint32_t>(q * 32) << 16);
+      for (int c0 = 0; c0 < it.n; c0 += kChunk) {
+        float v[kChunk];
+        tmem_ld_x16(t_acc + c0, v);
+        if (c0 + kChunk >= it.n) {
+          // every TMEM read of this accumulator is done: hand it back to the MMA warp
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(s.acc_empty + 8 * acc, 0));
+        }
+        float* const sbuf = staging + buf * (kChunk * kStageLd);
+        buf ^= 1u;
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) sbuf[i * kStageLd + q * 32 + lane] = v[i];
+        epilogue_sync();       // (two buffers: one barrier per step suffices)
+#pragma unroll
+        for (int i = me; i < kChunk * kVecs; i += kEpiThreads) {
+          const int tok = i / kVecs, vec = i % kVecs;
+          if (c0 + tok >= it.rows) continue;
+          const int64_t slot = it.row0 + c0 + tok;
+          float a[8];
+          const float4* src = reinterpret_cast<const float4*>(sbuf + tok * kStageLd + vec * 8);
+          *reinterpret_cast<float4*>(a) = src[0];
+          *reinterpret_cast<float4*>(a + 4) = src[1];
+          if (kEpi == kNone) {
+            const int f = it.f0 + cta * 128 + vec * 8;
+            if (f < p.n) store_row8(p.out, slot * p.ldo + f, bf16, a);
+            continue;
+          }
+          float u[8];
+          *reinterpret_cast<float4*>(u) = src[16];
+          *reinterpret_cast<float4*>(u + 4) = src[17];
+          const int f = it.f0 / 2 + cta * 64 + vec * 8;
+          if (kEpi == kSiluGate) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] = apply_elementwise(kOpSilu, a[j]) * u[j];
+            store_row8(p.out, slot * p.ldo + f, bf16, a);
+          } else {
+            float g[8] = {};
+            tile_accumulate_16x8(bf16, g, *reinterpret_cast<const uint4*>(
+                static_cast<const char*>(p.dh) + 2 * (slot * p.ld_dh + f)));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float sg = apply_elementwise(kOpSigmoid, a[j]);
+              const float da = g[j] * u[j] * sg * (1.f + a[j] * (1.f - sg));
+              u[j] = g[j] * a[j] * sg;
+              a[j] = da;
+            }
+            const int64_t at = slot * p.ldo + it.f0 + cta * 64 + vec * 8;
+            store_row8(p.out, at, bf16, a);
+            store_row8(p.out, at + 128, bf16, u);
+          }
+        }
+      }
+      acc ^= 1u;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  }
+  pipe_end(tmem_base);
+}
+
+// ---------------------------------------------------------------------------------------
+// out[e] = sum over the slots of e of a[row(s)]^T b[row(s)]
+//
+// 256 x 256 tiles of out[e]; the contraction runs over the expert's rows, 64 per stage, so both
+// operands are MN-major (a row of 64 columns is 128 bytes of a stage).  The rows of the last,
+// partial block that belong to the next expert are read out of range instead, single row by
+// single row, and come as zeros.
+// ---------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(kThreads, 1)
+expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const Pipe s = make_pipe(smem_raw, kGradStagingBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = static_cast<int>(cluster_ctarank());
+  const bool leader = cta == 0;
+  const int per_expert = p.m_tiles * p.n_tiles;
+  const uint32_t tmem_base = pipe_start(s);
+  WaitBudget wb;
+  wb.start(p.budget_ns, s.words + 1);
+  const int total = p.experts * per_expert;
+  const int step = static_cast<int>(gridDim.x >> 1);
+
+  if (warp == 0) {
+    // ------------------------------- TMA producer -------------------------------
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
+      const int e = t / per_expert, local = t % per_expert;
+      const int x_a = local / p.n_tiles * kTile + cta * 128;
+      const int x_b = local % p.n_tiles * kTile + cta * 128;
+      const int row0 = slot_bound(p.offsets, e, p.slots), row1 = slot_bound(p.offsets, e + 1, p.slots);
+      for (int r0 = row0; r0 < row1; r0 += kBK) {
+        ok = __all_sync(0xffffffffu, mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb));
+        if (!ok) {
+          if (lane == 0) report_status(p.status, kStatusTimeoutMbarrier, 111, 0, r0, 0, t);
+          break;
+        }
+        const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+        const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
+        const bool whole = r0 + kBK <= row1;
+        if (lane == 0 && leader) mbar_expect_tx(s.full + 8 * stage, 2 * kStageBytes);
+        auto load = [&](uint32_t dst, const CUtensorMap* boxes, const CUtensorMap* rows, int x,
+                        bool gather, int n_rows) {
+          if (whole && !gather) {
+            if (lane < 2)
+              tma_load_2d_pair(dst + lane * kHalfBytes, boxes, x + lane * 64, r0, bar);
+            return;
+          }
+          // lane: column half, and four of the block's 64 rows
+          int r[4];
+          const int h = lane >> 4, at = r0 + 4 * (lane & 15);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            r[j] = at + j < row1 ? at + j : -1;
+            if (gather && r[j] >= 0) r[j] = p.token_of_slot[r[j]];
+            if (r[j] < 0 || r[j] >= n_rows) r[j] = n_rows;
+          }
+          tma_gather4_pair(dst + h * kHalfBytes + (lane & 15) * 512, rows, x + h * 64, r, bar);
+        };
+        load(sa, &p.tma_a, &p.tma_a_rows, x_a, p.gather_a != 0, p.a_rows);
+        load(sb, &p.tma_b, &p.tma_b_rows, x_b, p.gather_b != 0, p.b_rows);
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (!ok) drain_copies();
+  } else if (warp == 1 && leader) {
+    // ----------------------- MMA issuer (leader CTA only) -----------------------
+    if (elect_one_sync()) {
+      const uint32_t idesc = umma_idesc_f16(p.bf16, 1, 1, kTile, kTile);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
+        const int e = t / per_expert;
+        const int rows = slot_bound(p.offsets, e + 1, p.slots) - slot_bound(p.offsets, e, p.slots);
+        const int blocks = (max(rows, 0) + kBK - 1) / kBK;
+        if (blocks == 0) continue;                       // the epilogue writes zeros
+        if (!mbar_wait(s.acc_empty + 8 * acc, acc_phase ^ 1u, wb)) {
+          report_status(p.status, kStatusTimeoutMbarrier, 112, 0, 0, 0, t);
+          ok = false;
+          break;
+        }
+        tcgen05_fence_after();
+        const uint32_t d = tmem_base + acc * kAccCols;
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(s.full + 8 * stage, phase, wb)) {
+            report_status(p.status, kStatusTimeoutMbarrier, 113, blocks, kb, 0, t);
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after();
+          const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+#pragma unroll
+          for (int k = 0; k < kBK / kUmmaK; ++k)
+            umma_f16_pair(d, umma_smem_desc_sw128(sa + k * kUmmaK * 128, kHalfBytes, 1024),
+                          umma_smem_desc_sw128(sb + k * kUmmaK * 128, kHalfBytes, 1024), idesc,
+                          (kb | k) != 0 ? 1u : 0u);
+          umma_commit_pair(s.empty + 8 * stage, 3);
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit_pair(s.acc_full + 8 * acc, 3);
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      if (!ok) {
+        umma_commit_pair(s.drain, 1);
+        for (int i = 0; i < 1000000 && !mbar_try_wait(s.drain, 0); ++i) {}
+      }
+    }
+  } else if (warp >= 4) {
+    // --------------------------------- epilogue ---------------------------------
+    // A lane is a row of out[e]: 32 rows x 64 columns at a time go through a swizzled buffer
+    // into a TMA store, which clips them to the matrix.
+    const int q = warp - 4;
+    const uint32_t mine = s.staging + q * 2 * 4096;
+    const bool bf16 = p.bf16 != 0;
+    uint32_t acc = 0, acc_phase = 0, buf = 0;
+    bool ok = true;
+    for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
+      const int e = t / per_expert, local = t % per_expert;
+      const int y = local / p.n_tiles * kTile + cta * 128 + q * 32, x = local % p.n_tiles * kTile;
+      const bool empty = slot_bound(p.offsets, e + 1, p.slots) <= slot_bound(p.offsets, e, p.slots);
+      if (!empty) {
+        if (!mbar_wait(s.acc_full + 8 * acc, acc_phase, wb)) {
+          if (lane == 0) report_status(p.status, kStatusTimeoutMbarrier, 114, 0, 0, 0, t);
+          ok = false;
+          break;
+        }
+        tcgen05_fence_after();
+      }
+      const uint32_t t_acc = tmem_base + acc * kAccCols + (static_cast<uint32_t>(q * 32) << 16);
+      for (int ch = 0; ch < kTile / 64; ++ch) {
+        float v[64];
+        if (!empty) {
+          uint32_t r0[32], r1[32];
+          tmem_ld_32x32b_x32(t_acc + ch * 64, r0);
+          tmem_ld_32x32b_x32(t_acc + ch * 64 + 32, r1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v[i] = __uint_as_float(r0[i]);
+            v[32 + i] = __uint_as_float(r1[i]);
+          }
+          if (ch == kTile / 64 - 1) {
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(s.acc_empty + 8 * acc, 0));
+          }
+        } else {
+          tile_zeros(v);
+        }
+        if (lane == 0) tma_store_wait_read<1>();    // the store that last read this buffer
+        __syncwarp();
+        const uint32_t sbuf = mine + buf * 4096;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint4 w = tile_cast_f32x8(bf16, &v[j * 8]);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                           sbuf + lane * 128 + ((j ^ (lane & 7)) << 4)),
+                       "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                       : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (x + ch * 64 < p.n && y < p.m) tma_store_3d(&p.tma_out, x + ch * 64, y, e, sbuf);
+          tma_store_commit();
+        }
+        buf ^= 1u;
+      }
+      if (!empty) {
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+    if (lane == 0) tma_store_wait_all<0>();
+  }
+  pipe_end(tmem_base);
+}
+
+// ------------------------------------------------------------------------------- host side
+int encode(CUtensorMap* map, bool bf16, uint64_t base, uint64_t cols, uint64_t rows,
+           uint64_t depth, uint64_t ld_bytes, uint64_t slab_bytes, uint32_t box_rows,
+           const char* what) {
+  const DriverApi& d = driver();
+  cuuint64_t dims[3] = {cols, rows, depth};
+  cuuint64_t strides[2] = {ld_bytes, slab_bytes};
+  cuuint32_t box[3] = {64, box_rows, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = d.cuTensorMapEncodeTiled(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+      depth > 0 ? 3 : 2, reinterpret_cast<void*>(base), dims, strides, box, es,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(kErrCuda, std::string("cuTensorMapEncodeTiled(") + what + "): " + driver_error_string(r));
+  return kOk;
+}
+
+using GemmKernel = void (*)(const GemmParams);
+GemmKernel gemm_kernel(int epilogue, bool gather) {
+  switch (epilogue) {
+    case kNone: return gather ? expert_gemm_kernel<kNone, true> : expert_gemm_kernel<kNone, false>;
+    case kSiluGate:
+      return gather ? expert_gemm_kernel<kSiluGate, true> : expert_gemm_kernel<kSiluGate, false>;
+    default:
+      return gather ? expert_gemm_kernel<kSiluGateGrad, true> : expert_gemm_kernel<kSiluGateGrad, false>;
   }
 }
 
-// out[e][i][j] = sum over the slots of e of a[row(s)][i] * b[row'(s)][j]; one of the operands
-// is gathered by token (gather_a / gather_b).
-__global__ void __launch_bounds__(256) expert_weight_grad_kernel(const TcclExpertWeightGrad d) {
-  __shared__ float as[16][65], bs[16][65];
-  const bool bf16 = d.dtype == 1;
-  const int e = blockIdx.z;
-  const int32_t* offsets = reinterpret_cast<const int32_t*>(d.offsets);
-  auto bound = [&](int i) { const int v = offsets[i]; return v < 0 ? 0 : v > d.slots ? static_cast<int>(d.slots) : v; };
-  const int s0 = bound(e), s1 = bound(e + 1);
-  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int32_t* tok = reinterpret_cast<const int32_t*>(d.token_of_slot);
-  auto row = [&](int s, bool gather, int64_t rows) -> int64_t {
-    if (!gather) return s;
-    const int t = tok[s];
-    return t >= 0 && t < rows ? t : 0;
-  };
-  float acc[4][4] = {};
-  for (int s = s0; s < s1; s += 16) {
-    for (int i = threadIdx.x; i < 16 * 64; i += 256) {
-      const int c = i & 63, r = i >> 6;
-      const bool ok = s + r < s1;
-      as[r][c] = ok && i0 + c < d.m ? load16(reinterpret_cast<const void*>(d.a),
-                                             row(s + r, d.gather_a, d.a_rows) * d.lda + i0 + c, bf16) : 0.f;
-      bs[r][c] = ok && j0 + c < d.n ? load16(reinterpret_cast<const void*>(d.b),
-                                             row(s + r, d.gather_b, d.b_rows) * d.ldb + j0 + c, bf16) : 0.f;
-    }
-    __syncthreads();
-    for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[kk][ty * 4 + i], bs[kk][tx * 4 + j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = i0 + ty * 4 + i, c = j0 + tx * 4 + j;
-      if (r < d.m && c < d.n)
-        store16(reinterpret_cast<void*>(d.out), (e * d.m + r) * d.n + c, bf16, acc[i][j]);
-    }
+cudaError_t attrs_once(int* sms) {
+  static int count[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && count[dev] != 0) { *sms = count[dev]; return cudaSuccess; }
+  e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  for (int i = 0; i < 6 && e == cudaSuccess; ++i)
+    e = cudaFuncSetAttribute(gemm_kernel(i / 2, i % 2 != 0),
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(expert_weight_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kGradSmem);
+  if (e == cudaSuccess && dev < 64) count[dev] = *sms;
+  return e;
 }
+
+template <typename P>
+cudaError_t launch_pairs(void (*kernel)(const P), const P& p, int pairs, int smem, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+constexpr uint64_t kWaitBudgetNs = 2000000000ull;
 
 }  // namespace
 
 cudaError_t preload_expert_gemm_kernels() {
   cudaFuncAttributes a;
-  cudaError_t e = cudaFuncGetAttributes(&a, expert_gemm_kernel);
-  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_weight_grad_kernel);
+  int sms = 0;
+  cudaError_t e = cudaFuncGetAttributes(&a, expert_weight_grad_kernel);
+  for (int i = 0; i < 6 && e == cudaSuccess; ++i)
+    e = cudaFuncGetAttributes(&a, gemm_kernel(i / 2, i % 2 != 0));
+  if (e == cudaSuccess) e = attrs_once(&sms);
   return e;
 }
 
@@ -172,8 +742,9 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   const TcclExpertGemm& d = *desc;
   TCCL_CHECK_ARG(d.dtype == 0 || d.dtype == 1, "dtype must be 0 (fp16) or 1 (bf16)");
   TCCL_CHECK_ARG(d.epilogue >= kNone && d.epilogue <= kSiluGateGrad, "epilogue must be 0..2");
-  TCCL_CHECK_ARG(d.experts >= 1 && d.experts <= 1024, "experts must be 1..1024");
-  TCCL_CHECK_ARG(d.k >= 1 && d.n >= 1, "empty problem");
+  TCCL_CHECK_ARG(d.experts >= 1 && d.experts <= kMaxExperts, "experts must be 1..1024");
+  TCCL_CHECK_ARG(d.k >= 1 && d.n >= 1 && d.k < (int64_t(1) << 31) && d.n < (int64_t(1) << 31) - kTile,
+                 "K and N must be 1..2^31");
   TCCL_CHECK_ARG(d.k % 8 == 0, "K must be a multiple of 8 (16-byte TMA rows)");
   TCCL_CHECK_ARG(d.n % 8 == 0, "N must be a multiple of 8 (16-byte TMA rows)");
   TCCL_CHECK_ARG(d.ldx % 8 == 0 && d.ldw % 8 == 0 && d.w_expert % 8 == 0 && d.ldo % 8 == 0 &&
@@ -183,16 +754,43 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
                  "operands must be 16-byte aligned");
   TCCL_CHECK_ARG(d.epilogue == kNone || d.n % 256 == 0,
                  "SiLU-gate epilogue needs N to be a multiple of 256");
-  TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) && d.x_rows < (int64_t(1) << 31),
+  TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) - kTile && d.x_rows < (int64_t(1) << 31),
                  "too many rows");
   if (d.slots == 0) return kOk;
   TCCL_CHECK_ARG(d.x != 0 && d.w != 0 && d.out != 0 && d.offsets != 0 && d.x_rows >= 1, "null argument");
   TCCL_CHECK_ARG(d.epilogue != kSiluGateGrad || d.dh != 0, "null argument");
-  const int64_t cols = d.epilogue == kNone ? d.n : d.n / 2;
-  const int64_t tiles = d.slots / 64 + (d.slots < d.experts ? d.slots : d.experts);
-  const dim3 grid(static_cast<unsigned>((cols + 63) / 64), static_cast<unsigned>(tiles));
-  expert_gemm_kernel<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(d);
-  TCCL_CHECK_CUDA(cudaGetLastError());
+  const int64_t f_tiles = (d.n + kTile - 1) / kTile;
+  const int64_t tiles = (d.slots / kTile + (d.slots < d.experts ? d.slots : d.experts)) * f_tiles;
+  TCCL_CHECK_ARG(tiles < (int64_t(1) << 31), "too many tiles");
+  TCCL_REQUIRE_DRIVER();
+  const bool bf16 = d.dtype == 1, gather = d.token_of_slot != 0;
+  GemmParams p;
+  int rc = encode(&p.tma_w, bf16, d.w, d.w_nk ? d.k : d.n, d.w_nk ? d.n : d.k, d.experts, d.ldw * 2,
+                  d.w_expert * 2, 64, "W");
+  if (rc) return rc;
+  rc = encode(&p.tma_x, bf16, d.x, d.k, d.x_rows, 0, d.ldx * 2, 0, gather ? 1 : 16, "X");
+  if (rc) return rc;
+  p.offsets = reinterpret_cast<const int32_t*>(d.offsets);
+  p.token_of_slot = reinterpret_cast<const int32_t*>(d.token_of_slot);
+  p.out = reinterpret_cast<void*>(d.out);
+  p.dh = reinterpret_cast<const void*>(d.dh);
+  p.ldo = d.ldo;
+  p.ld_dh = d.ld_dh;
+  p.slots = static_cast<int32_t>(d.slots);
+  p.x_rows = static_cast<int32_t>(d.x_rows);
+  p.experts = d.experts;
+  p.k_blocks = static_cast<int32_t>((d.k + kBK - 1) / kBK);
+  p.n = static_cast<int32_t>(d.n);
+  p.f_tiles = static_cast<int32_t>(f_tiles);
+  p.bf16 = bf16 ? 1 : 0;
+  p.w_nk = d.w_nk ? 1 : 0;
+  p.status = reinterpret_cast<uint32_t*>(d.status);
+  p.budget_ns = kWaitBudgetNs;
+  int sms = 0;
+  TCCL_CHECK_CUDA(attrs_once(&sms));
+  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+  TCCL_CHECK_CUDA(launch_pairs(gemm_kernel(d.epilogue, gather), p, pairs, kGemmSmem,
+                               reinterpret_cast<cudaStream_t>(stream)));
   return kOk;
 }
 
@@ -200,19 +798,53 @@ extern "C" int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_
   TCCL_CHECK_ARG(desc != nullptr, "null argument");
   const TcclExpertWeightGrad& d = *desc;
   TCCL_CHECK_ARG(d.dtype == 0 || d.dtype == 1, "dtype must be 0 (fp16) or 1 (bf16)");
-  TCCL_CHECK_ARG(d.experts >= 1 && d.experts <= 1024, "experts must be 1..1024");
-  TCCL_CHECK_ARG(d.m >= 1 && d.n >= 1, "empty problem");
+  TCCL_CHECK_ARG(d.experts >= 1 && d.experts <= kMaxExperts, "experts must be 1..1024");
+  TCCL_CHECK_ARG(d.m >= 1 && d.n >= 1 && d.m < (int64_t(1) << 31) - kTile &&
+                     d.n < (int64_t(1) << 31) - kTile, "rows and columns must be 1..2^31");
   TCCL_CHECK_ARG(d.m % 8 == 0 && d.n % 8 == 0, "rows and columns must be multiples of 8");
   TCCL_CHECK_ARG(d.lda % 8 == 0 && d.ldb % 8 == 0, "leading dimensions must be multiples of 8 elements");
   TCCL_CHECK_ARG(d.a % 16 == 0 && d.b % 16 == 0 && d.out % 16 == 0, "operands must be 16-byte aligned");
-  TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) && d.a_rows < (int64_t(1) << 31) &&
-                     d.b_rows < (int64_t(1) << 31), "too many rows");
+  TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) - kTile &&
+                     d.a_rows < (int64_t(1) << 31) && d.b_rows < (int64_t(1) << 31), "too many rows");
   TCCL_CHECK_ARG(d.out != 0 && d.offsets != 0, "null argument");
-  TCCL_CHECK_ARG(d.slots == 0 || (d.a != 0 && d.b != 0 && d.a_rows >= 1 && d.b_rows >= 1), "null argument");
-  TCCL_CHECK_ARG(!(d.gather_a || d.gather_b) || d.slots == 0 || d.token_of_slot != 0, "null argument");
-  const dim3 grid(static_cast<unsigned>((d.n + 63) / 64), static_cast<unsigned>((d.m + 63) / 64),
-                  static_cast<unsigned>(d.experts));
-  expert_weight_grad_kernel<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(d);
-  TCCL_CHECK_CUDA(cudaGetLastError());
+  if (d.slots == 0) {
+    TCCL_CHECK_CUDA(cudaMemsetAsync(reinterpret_cast<void*>(d.out), 0, d.experts * d.m * d.n * 2,
+                                    reinterpret_cast<cudaStream_t>(stream)));
+    return kOk;
+  }
+  TCCL_CHECK_ARG(d.a != 0 && d.b != 0 && d.a_rows >= 1 && d.b_rows >= 1, "null argument");
+  TCCL_CHECK_ARG(!(d.gather_a || d.gather_b) || d.token_of_slot != 0, "null argument");
+  const int64_t m_tiles = (d.m + kTile - 1) / kTile, n_tiles = (d.n + kTile - 1) / kTile;
+  const int64_t tiles = d.experts * m_tiles * n_tiles;
+  TCCL_CHECK_ARG(tiles < (int64_t(1) << 31), "too many tiles");
+  TCCL_REQUIRE_DRIVER();
+  const bool bf16 = d.dtype == 1;
+  GradParams p;
+  int rc = encode(&p.tma_a, bf16, d.a, d.m, d.a_rows, 0, d.lda * 2, 0, 64, "A");
+  if (!rc) rc = encode(&p.tma_b, bf16, d.b, d.n, d.b_rows, 0, d.ldb * 2, 0, 64, "B");
+  if (!rc) rc = encode(&p.tma_a_rows, bf16, d.a, d.m, d.a_rows, 0, d.lda * 2, 0, 1, "A");
+  if (!rc) rc = encode(&p.tma_b_rows, bf16, d.b, d.n, d.b_rows, 0, d.ldb * 2, 0, 1, "B");
+  if (!rc) rc = encode(&p.tma_out, bf16, d.out, d.n, d.m, d.experts, d.n * 2, d.m * d.n * 2, 32, "out");
+  if (rc) return rc;
+  p.offsets = reinterpret_cast<const int32_t*>(d.offsets);
+  p.token_of_slot = reinterpret_cast<const int32_t*>(d.token_of_slot);
+  p.slots = static_cast<int32_t>(d.slots);
+  p.a_rows = static_cast<int32_t>(d.a_rows);
+  p.b_rows = static_cast<int32_t>(d.b_rows);
+  p.experts = d.experts;
+  p.m = static_cast<int32_t>(d.m);
+  p.n = static_cast<int32_t>(d.n);
+  p.m_tiles = static_cast<int32_t>(m_tiles);
+  p.n_tiles = static_cast<int32_t>(n_tiles);
+  p.bf16 = bf16 ? 1 : 0;
+  p.gather_a = d.gather_a;
+  p.gather_b = d.gather_b;
+  p.status = reinterpret_cast<uint32_t*>(d.status);
+  p.budget_ns = kWaitBudgetNs;
+  int sms = 0;
+  TCCL_CHECK_CUDA(attrs_once(&sms));
+  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+  TCCL_CHECK_CUDA(launch_pairs(&expert_weight_grad_kernel, p, pairs, kGradSmem,
+                               reinterpret_cast<cudaStream_t>(stream)));
   return kOk;
 }

@@ -104,6 +104,30 @@ def _launch(fn: str, *args) -> None:
     _fg.count_launches(1)
 
 
+_STATUS: dict = {}
+
+
+def _status_ptr(dev: torch.device) -> int:
+    """Status words of a device's products (see :func:`check_expert_status`)."""
+    t = _STATUS.get(dev.index)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0                      # (cannot be cleared inside a capture: not reported)
+        t = _STATUS[dev.index] = torch.zeros(_fg.STATUS_WORDS, dtype=torch.int32, device=dev)
+    return t.data_ptr()
+
+
+def check_expert_status(device=None) -> None:
+    """Synchronise and raise :class:`TileCCLTimeoutError` if a wait inside a grouped product on
+    ``device`` (default: the current one) ran out of its two-second budget since the last check;
+    the results of that call are then undefined."""
+    dev = torch.device("cuda" if device is None else device)
+    t = _STATUS.get(torch.cuda.current_device() if dev.index is None else dev.index)
+    if t is not None:
+        torch.cuda.synchronize(t.device)
+        _fg.raise_on_status(t)
+
+
 # -------------------------------------------------------------------------- routing
 def _check_routing(logits, top_k, score, scale):
     _check_tensor("logits", logits, 2, tuple(_LOGIT_DTYPES))
@@ -314,6 +338,7 @@ def _product(X, W, slots, out, rows, b_is_nk, epi, dh, raw):
     if d.w_expert < (W.shape[1] - 1) * d.ldw + W.shape[2] or d.w_expert % 8:
         raise ValueError("W's experts overlap or are not 16-byte aligned")
     d.ld_dh = 0 if dh is None else _aligned("grad_out", dh)
+    d.status = _status_ptr(X.device)
     _launch("tccl_expert_gemm", C.byref(d), raw)
 
 
@@ -378,6 +403,7 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
         d.m, d.n, d.a_rows, d.b_rows = a.shape[1], b.shape[1], a.shape[0], b.shape[0]
         d.a, d.b, d.out = a.data_ptr(), b.data_ptr(), grad_W.data_ptr()
         d.lda, d.ldb = _aligned("X", a), _aligned("X", b)
+        d.status = _status_ptr(X.device)
         _launch("tccl_expert_weight_grad", C.byref(d), raw)
     return grad_X, grad_W
 

@@ -31,9 +31,9 @@ import torch
 
 from . import _fused
 from ._fused import call_stats, check_status, recover
-from ..kernels.experts import (ExpertSlots, expert_combine, expert_combine_backward, expert_gemm,
-                               expert_gemm_backward, expert_slots, route_experts,
-                               route_experts_backward)
+from ..kernels.experts import (ExpertSlots, check_expert_status, expert_combine,
+                               expert_combine_backward, expert_gemm, expert_gemm_backward,
+                               expert_slots, route_experts, route_experts_backward)
 from ..kernels.fused_gemm import TileCCLTimeoutError
 from ..primitives import collectives as _coll
 
@@ -51,6 +51,7 @@ __all__ = [
     "AllGatherGemmReduceScatterContract",
     "route_experts", "route_experts_backward", "expert_slots", "ExpertSlots", "expert_gemm",
     "expert_gemm_backward", "expert_combine", "expert_combine_backward",
+    "check_expert_status",
     "check_status", "recover", "call_stats", "TileCCLTimeoutError",
 ]
 
