@@ -183,15 +183,10 @@ class ExpertWeightGrad(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32),
         ("experts", C.c_int32),
-        ("gather_a", C.c_int32),
-        ("gather_b", C.c_int32),
         ("m", C.c_int64),
         ("n", C.c_int64),
         ("slots", C.c_int64),
-        ("a_rows", C.c_int64),
-        ("b_rows", C.c_int64),
         ("offsets", C.c_uint64),
-        ("token_of_slot", C.c_uint64),
         ("a", C.c_uint64),
         ("b", C.c_uint64),
         ("out", C.c_uint64),
@@ -271,6 +266,7 @@ def _declare(lib: C.CDLL) -> None:
         "tccl_expert_slots": [u64, i64, i32, i32, i32, u64, u64, u64, u64, u64],
         "tccl_expert_gemm": [C.POINTER(ExpertGemm), u64],
         "tccl_expert_weight_grad": [C.POINTER(ExpertWeightGrad), u64],
+        "tccl_expert_gather": [u64, i64, i64, u64, u64, i64, i64, i32, u64],
         "tccl_expert_combine": [u64, i64, u64, u64, u64, i64, u64, i64, i64, i64, i32, i32, i32, u64],
         "tccl_expert_combine_backward": [u64, i64, u64, i64, u64, u64, u64, i64, u64, i64, i64, i32,
                                          i32, i32, u64],

@@ -337,16 +337,19 @@ typedef struct TcclExpertGemm {
 } TcclExpertGemm;
 int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream);
 
-// out[e] = sum over the slots of expert e of a[row(s)]^T b[row(s)]: [experts, m, n] contiguous.
+// out[e] = sum over the slots s of expert e of a[s]^T b[s]: [experts, m, n] contiguous.
 typedef struct TcclExpertWeightGrad {
-  int32_t dtype, experts, gather_a, gather_b;   // a gathered operand has one row per token
-  int64_t m, n, slots, a_rows, b_rows;
-  uint64_t offsets, token_of_slot, a, b, out;
+  int32_t dtype, experts;
+  int64_t m, n, slots;
+  uint64_t offsets, a, b, out;
   int64_t lda, ldb;
   uint64_t status;
 } TcclExpertWeightGrad;
 int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_t stream);
 
+// out[s] = x[token of slot s]; rows behind the last slot are left as they are.
+int tccl_expert_gather(uint64_t x, int64_t x_ld, int64_t x_rows, uint64_t token_of_slot,
+                       uint64_t out, int64_t out_ld, int64_t slots, int32_t n, uint64_t stream);
 int tccl_expert_combine(uint64_t h, int64_t h_ld, uint64_t slot_of, uint64_t weights, uint64_t add,
                         int64_t add_ld, uint64_t out, int64_t out_ld, int64_t tokens,
                         int64_t slots, int32_t top_k, int32_t n, int32_t dtype, uint64_t stream);

@@ -1,4 +1,4 @@
-// Weighted sum of a token's expert outputs and its gradient.
+// Weighted sum of a token's expert outputs and its gradient, and tokens' rows in slot order.
 //
 //   y[t] = add[t] + sum_j w[t][j] * h[slot_of[t][j]]        (choices without a slot add nothing)
 //   dh[slot_of[t][j]] = w[t][j] * dy[t]      dw[t][j] = <dy[t], h[slot_of[t][j]]>
@@ -84,6 +84,18 @@ __global__ void __launch_bounds__(kThreads) expert_combine_backward_kernel(const
   }
 }
 
+// out[s] = x[token of slot s]; zeros for a token that does not exist, nothing behind the last
+// slot (token -1).
+__global__ void __launch_bounds__(kThreads) expert_gather_kernel(
+    const uint4* x, int64_t x_ld, int64_t x_rows, const int32_t* token_of_slot, uint4* out,
+    int64_t out_ld, int32_t vecs) {
+  const int64_t s = blockIdx.x;
+  const int32_t t = token_of_slot[s];
+  if (t < 0) return;
+  const int v = blockIdx.y * kThreads + threadIdx.x;
+  if (v < vecs) out[s * out_ld + v] = t < x_rows ? x[t * x_ld + v] : make_uint4(0, 0, 0, 0);
+}
+
 int check(const CombineParams& p) {
   TCCL_CHECK_ARG(p.tokens >= 0 && p.tokens < (int64_t(1) << 31), "tokens out of range");
   TCCL_CHECK_ARG(p.top_k >= 1 && p.vecs >= 1, "empty rows");
@@ -97,6 +109,7 @@ cudaError_t preload_expert_combine_kernels() {
   cudaFuncAttributes a;
   cudaError_t e = cudaFuncGetAttributes(&a, expert_combine_kernel);
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_combine_backward_kernel);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_gather_kernel);
   return e;
 }
 
@@ -167,6 +180,25 @@ extern "C" int tccl_expert_combine_backward(uint64_t dy, int64_t dy_ld, uint64_t
                  "null argument");
   expert_combine_backward_kernel<<<static_cast<unsigned>(tokens), kThreads, 0,
                                    reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  TCCL_CHECK_CUDA(cudaGetLastError());
+  return kOk;
+}
+
+extern "C" int tccl_expert_gather(uint64_t x, int64_t x_ld, int64_t x_rows, uint64_t token_of_slot,
+                                  uint64_t out, int64_t out_ld, int64_t slots, int32_t n,
+                                  uint64_t stream) {
+  TCCL_CHECK_ARG(n >= 8 && n % 8 == 0 && x_ld % 8 == 0 && out_ld % 8 == 0,
+                 "row lengths and pitches must be multiples of 8 elements");
+  TCCL_CHECK_ARG(x % 16 == 0 && out % 16 == 0, "rows must be 16-byte aligned");
+  TCCL_CHECK_ARG(slots >= 0 && slots < (int64_t(1) << 31), "too many rows");
+  const int vecs = n / 8;
+  TCCL_CHECK_ARG(vecs <= 65535 * kThreads, "rows are too long");
+  if (slots == 0) return kOk;
+  TCCL_CHECK_ARG(x != 0 && token_of_slot != 0 && out != 0, "null argument");
+  const dim3 grid(static_cast<unsigned>(slots), (vecs + kThreads - 1) / kThreads);
+  expert_gather_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      reinterpret_cast<const uint4*>(x), x_ld / 8, x_rows,
+      reinterpret_cast<const int32_t*>(token_of_slot), reinterpret_cast<uint4*>(out), out_ld / 8, vecs);
   TCCL_CHECK_CUDA(cudaGetLastError());
   return kOk;
 }

@@ -7,7 +7,7 @@
 //   gradient of the gate: gate and up are computed again and with dh[s] = dL/dout[s]
 //              dgate = dh * up * sg * (1 + gate * (1 - sg)),  dup = dh * gate * sg,
 //              sg = 1 / (1 + e^-gate), packed like W's columns
-//   dW[e] = sum over the slots of e of a[row(s)]^T b[row(s)]
+//   dW[e] = sum over the slots s of e of a[s]^T b[s]
 //
 // Both kernels are persistent: a cluster of two CTAs per tile, tcgen05.mma.cta_group::2, a TMA
 // ring of operand stages, two accumulators in TMEM so that the epilogue of one tile runs under
@@ -27,7 +27,8 @@ enum Epilogue : int { kNone = 0, kSiluGate = 1, kSiluGateGrad = 2 };
 
 constexpr int kMaxExperts = 1024;
 constexpr int kThreads = 256;            // warp 0 TMA, 1 MMA, 2 TMEM, 3 idle, 4-7 epilogue
-constexpr int kEpiThreads = 128;
+constexpr int kCopyThreads = 128;        // warps 8-11 of the weight gradient
+constexpr int kEpiThreads = 128;         // warps 4-7
 constexpr int kStages = 6;
 constexpr int kBK = 64;                  // contraction elements per stage (one 128-byte row)
 constexpr int kUmmaK = 16;
@@ -40,7 +41,7 @@ constexpr int kBand = 16;                // token tiles that share a sweep over 
 constexpr int kChunk = 16;               // tokens per epilogue step
 constexpr int kStageLd = 132;            // floats between tokens of the staging buffer
 constexpr int kStagingBytes = 2 * kChunk * kStageLd * 4;
-constexpr int kCtlBytes = 512;
+constexpr int kCtlBytes = 1024;         // barriers; from 512 on the rows a gathering CTA stages
 constexpr int kListBytes = 2 * 4 * (kMaxExperts + 2);
 constexpr int kGemmSmem = kStages * kStageBytes + kStagingBytes + kCtlBytes + kListBytes + 1024;
 constexpr int kGradStagingBytes = 4 * 2 * 4096;   // per epilogue warp two buffers of 32 x 64
@@ -49,7 +50,8 @@ static_assert(kGemmSmem <= 232448 && kGradSmem <= 232448, "shared memory of one 
 
 struct GemmParams {
   CUtensorMap tma_w;          // {columns, rows, experts}, box {64, 64, 1}, 128-byte swizzle
-  CUtensorMap tma_x;          // {K, rows}, box {64, 16}, gathered: {64, 1}
+  CUtensorMap tma_x[4];       // {K, rows}, boxes {64, 128}, {64, 64}, {64, 32}, {64, 16};
+                              // gathered: [0] only, box {64, 1}
   const int32_t* offsets;
   const int32_t* token_of_slot;
   void* out;
@@ -61,12 +63,13 @@ struct GemmParams {
 };
 
 struct GradParams {
-  CUtensorMap tma_a, tma_b;           // {columns, rows}, box {64, 64}
-  CUtensorMap tma_a_rows, tma_b_rows; // the same, box {64, 1}, for single rows
-  CUtensorMap tma_out;                // {n, m, experts}, box {64, 32, 1}
+  CUtensorMap tma_a, tma_b;   // {columns, rows}, box {64, 64}
+  CUtensorMap tma_out;        // {n, m, experts}, box {64, 32, 1}
   const int32_t* offsets;
-  const int32_t* token_of_slot;
-  int32_t slots, a_rows, b_rows, experts, m, n, m_tiles, n_tiles, bf16, gather_a, gather_b;
+  const void* a;
+  const void* b;
+  int64_t lda, ldb;
+  int32_t slots, experts, m, n, m_tiles, n_tiles, bf16;
   uint32_t* status;
   uint64_t budget_ns;
 };
@@ -79,6 +82,13 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
+// 16 bytes of a row, zeros instead when `take` is false (the source must be a valid address).
+__device__ __forceinline__ void copy_16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(take ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Four rows of a matrix, 64 columns each, into 512 consecutive bytes (swizzled by address).
 __device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap* m, int x,
                                                  const int (&r)[4], uint32_t bar) {
@@ -111,19 +121,21 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
-// Barrier of the epilogue warps that also agrees on a condition.
-__device__ __forceinline__ bool epilogue_all(bool ok) {
+// Barrier `id` of 128 threads that also agrees on a condition.
+__device__ __forceinline__ bool barrier_all(int id, bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "setp.ne.b32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 128, p;\n\t"
       "selp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(ok ? 1u : 0u)
+      : "r"(id), "r"(ok ? 1u : 0u)
       : "memory");
   return r != 0;
 }
+__device__ __forceinline__ bool epilogue_all(bool ok) { return barrier_all(1, ok); }
+__device__ __forceinline__ bool copiers_all(bool ok) { return barrier_all(2, ok); }
 __device__ __forceinline__ void epilogue_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
 // Shared memory of a CTA pair.  Every CTA has all barriers; in use are the leader's "full" and
@@ -131,7 +143,7 @@ __device__ __forceinline__ void epilogue_sync() { asm volatile("barrier.cta.sync
 // (signalled by multicast commits).
 struct Pipe {
   uint32_t base, staging, ctl;
-  uint32_t full, empty, acc_full, acc_empty, drain, tmem_slot;
+  uint32_t full, empty, tail, acc_full, acc_empty, drain, tmem_slot;
   volatile uint32_t* words;        // generic view of tmem_slot: [0] TMEM base, [1] abort flag
   int32_t* start;                  // [experts + 1] first slot of every expert
   int32_t* tiles;                  // [experts + 1] tiles of all lower experts
@@ -144,7 +156,8 @@ __device__ __forceinline__ Pipe make_pipe(uint8_t* raw, int staging_bytes) {
   s.ctl = s.staging + staging_bytes;
   s.full = s.ctl;
   s.empty = s.full + 8 * kStages;
-  s.acc_full = s.empty + 8 * kStages;
+  s.tail = s.empty + 8 * kStages;
+  s.acc_full = s.tail + 8;
   s.acc_empty = s.acc_full + 16;
   s.drain = s.acc_empty + 16;
   s.tmem_slot = s.drain + 8;
@@ -167,6 +180,7 @@ __device__ __forceinline__ uint32_t pipe_start(const Pipe& s) {
       mbar_init(s.acc_full + 8 * i, 1);
       mbar_init(s.acc_empty + 8 * i, 8);     // four epilogue warps of both CTAs
     }
+    mbar_init(s.tail, 2);                    // the copying warps of both CTAs
     mbar_init(s.drain, 1);
     s.words[1] = 0;
     mbar_fence_init();
@@ -238,6 +252,17 @@ __device__ __forceinline__ void pipe_end(uint32_t tmem_base) {
   if ((threadIdx.x >> 5) == 2) {
     tcgen05_fence_after();
     tmem_dealloc_pair(tmem_base, 2 * kAccCols);
+  }
+}
+
+// Bounded wait for arrivals of the other CTA of the pair.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, const WaitBudget& wb) {
+  for (uint32_t it = 0;; ++it) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if (wb.expired(it)) {
+      *wb.abort_flag = 1;
+      return false;
+    }
   }
 }
 
@@ -316,27 +341,33 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
       const Item it = item_of(t);
       const int mine = it.n >> 1;                          // token rows this CTA stages
       const int first = it.row0 + cta * mine;
-      int r[4] = {};
       if (kGather) {
         // Rows behind the tile's last slot (and tokens that do not exist) are read out of
         // range: the copy fills them with zeros.
+        int4 r;
+        int* const rj = &r.x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int slot = first + 4 * lane + j;
           int tok = -1;
           if (4 * lane < mine && slot < it.row0 + it.rows) tok = p.token_of_slot[slot];
-          r[j] = tok >= 0 && tok < p.x_rows ? tok : p.x_rows;
+          rj[j] = tok >= 0 && tok < p.x_rows ? tok : p.x_rows;
         }
+        __syncwarp();
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s.ctl + 512 + 16 * lane), "r"(r.x),
+                     "r"(r.y), "r"(r.z), "r"(r.w)
+                     : "memory");
+        __syncwarp();
       }
-      for (int kb = 0; kb < p.k_blocks; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb));
-        if (!ok) {
-          if (lane == 0) report_status(p.status, kStatusTimeoutMbarrier, 101, 0, kb, 0, t);
-          break;
-        }
-        const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
-        const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
-        if (lane == 0) {
+      if (elect_one_sync()) {
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb)) {
+            report_status(p.status, kStatusTimeoutMbarrier, 101, 0, kb, 0, t);
+            ok = false;
+            break;
+          }
+          const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+          const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
           // the bytes of both CTAs are counted on the leader's barrier
           if (leader) mbar_expect_tx(s.full + 8 * stage, 2 * (kOperandBytes + mine * 128));
 #pragma unroll
@@ -345,13 +376,32 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
             if (p.w_nk) tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, kb * kBK, f, it.e, bar);
             else tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, f, kb * kBK, it.e, bar);
           }
-          if (!kGather)
-            for (int i = 0; i < mine; i += 16)
-              tma_load_2d_pair(sb + i * 128, &p.tma_x, kb * kBK, first + i, bar);
+          if (kGather) {
+            for (int i = 0; i < mine; i += 4) {
+              int r[4];
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                           : "r"(s.ctl + 512 + 4 * i));
+              tma_gather4_pair(sb + i * 128, &p.tma_x[0], kb * kBK, r, bar);
+            }
+          } else {
+            // as few boxes as the row count has binary digits: a copy keeps the TMA unit busy
+            // however small it is (boxes of 16 rows throughout: 999 instead of 1549 TFLOP/s)
+            int at = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (mine & (128 >> i)) {
+                tma_load_2d_pair(sb + at * 128, &p.tma_x[i], kb * kBK, first + at, bar);
+                at += 128 >> i;
+              }
+            }
+          }
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
-        if (kGather && 4 * lane < mine) tma_gather4_pair(sb + lane * 512, &p.tma_x, kb * kBK, r, bar);
-        if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
+      // (the elected thread's state is the only one that counts; the warp leaves together)
+      __syncwarp();
+      ok = !wb.aborted();
     }
     if (!ok) drain_copies();
   } else if (warp == 1 && leader) {
@@ -402,7 +452,7 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
     // A TMEM lane is a feature and a column a token; results are rows of features.  Sixteen
     // tokens at a time cross over through shared memory in fp32: written by feature, read back
     // by token, eight features per thread.
-    const int q = warp - 4, me = threadIdx.x - (kThreads - kEpiThreads);
+    const int q = warp - 4, me = threadIdx.x - 128;
     float* const staging = reinterpret_cast<float*>(smem_raw + (s.staging - smem_u32(smem_raw)));
     const bool bf16 = p.bf16 != 0;
     constexpr int kVecs = kEpi == kNone ? 16 : 8;          // 8-feature vectors per token
@@ -476,14 +526,13 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
 }
 
 // ---------------------------------------------------------------------------------------
-// out[e] = sum over the slots of e of a[row(s)]^T b[row(s)]
+// out[e] = sum over the slots s of e of a[s]^T b[s]
 //
 // 256 x 256 tiles of out[e]; the contraction runs over the expert's rows, 64 per stage, so both
-// operands are MN-major (a row of 64 columns is 128 bytes of a stage).  The rows of the last,
-// partial block that belong to the next expert are read out of range instead, single row by
-// single row, and come as zeros.
+// operands are MN-major (a row of 64 columns is 128 bytes of a stage).  The last block of an
+// expert is copied row by row, with zeros in place of the next expert's rows.
 // ---------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads + kCopyThreads, 1)
 expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
   extern __shared__ uint8_t smem_raw[];
   const Pipe s = make_pipe(smem_raw, kGradStagingBytes);
@@ -499,52 +548,41 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
 
   if (warp == 0) {
     // ------------------------------- TMA producer -------------------------------
-    uint32_t stage = 0, phase = 0;
-    bool ok = true;
-    for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
-      const int e = t / per_expert, local = t % per_expert;
-      const int x_a = local / p.n_tiles * kTile + cta * 128;
-      const int x_b = local % p.n_tiles * kTile + cta * 128;
-      const int row0 = slot_bound(p.offsets, e, p.slots), row1 = slot_bound(p.offsets, e + 1, p.slots);
-      for (int r0 = row0; r0 < row1; r0 += kBK) {
-        ok = __all_sync(0xffffffffu, mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb));
-        if (!ok) {
-          if (lane == 0) report_status(p.status, kStatusTimeoutMbarrier, 111, 0, r0, 0, t);
-          break;
-        }
-        const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
-        const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
-        const bool whole = r0 + kBK <= row1;
-        if (lane == 0 && leader) mbar_expect_tx(s.full + 8 * stage, 2 * kStageBytes);
-        auto load = [&](uint32_t dst, const CUtensorMap* boxes, const CUtensorMap* rows, int x,
-                        bool gather, int n_rows) {
-          if (whole && !gather) {
-            if (lane < 2)
-              tma_load_2d_pair(dst + lane * kHalfBytes, boxes, x + lane * 64, r0, bar);
-            return;
+    if (elect_one_sync()) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
+        const int e = t / per_expert, local = t % per_expert;
+        const int x_a = local / p.n_tiles * kTile + cta * 128;
+        const int x_b = local % p.n_tiles * kTile + cta * 128;
+        const int row0 = slot_bound(p.offsets, e, p.slots), row1 = slot_bound(p.offsets, e + 1, p.slots);
+        for (int r0 = row0; r0 < row1; r0 += kBK) {
+          if (!mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb)) {
+            report_status(p.status, kStatusTimeoutMbarrier, 111, 0, r0, 0, t);
+            ok = false;
+            break;
           }
-          // lane: column half, and four of the block's 64 rows
-          int r[4];
-          const int h = lane >> 4, at = r0 + 4 * (lane & 15);
+          const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+          const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
+          const bool whole = r0 + kBK <= row1;
+          if (leader) mbar_expect_tx(s.full + 8 * stage, whole ? 2 * kStageBytes : 0);
+          if (whole) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            r[j] = at + j < row1 ? at + j : -1;
-            if (gather && r[j] >= 0) r[j] = p.token_of_slot[r[j]];
-            if (r[j] < 0 || r[j] >= n_rows) r[j] = n_rows;
+            for (int h = 0; h < 2; ++h) {
+              tma_load_2d_pair(sa + h * kHalfBytes, &p.tma_a, x_a + h * 64, r0, bar);
+              tma_load_2d_pair(sb + h * kHalfBytes, &p.tma_b, x_b + h * 64, r0, bar);
+            }
           }
-          tma_gather4_pair(dst + h * kHalfBytes + (lane & 15) * 512, rows, x + h * 64, r, bar);
-        };
-        load(sa, &p.tma_a, &p.tma_a_rows, x_a, p.gather_a != 0, p.a_rows);
-        load(sb, &p.tma_b, &p.tma_b_rows, x_b, p.gather_b != 0, p.b_rows);
-        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
       }
+      if (!ok) drain_copies();
     }
-    if (!ok) drain_copies();
   } else if (warp == 1 && leader) {
     // ----------------------- MMA issuer (leader CTA only) -----------------------
     if (elect_one_sync()) {
       const uint32_t idesc = umma_idesc_f16(p.bf16, 1, 1, kTile, kTile);
-      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, tail_phase = 0;
       bool ok = true;
       for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
         const int e = t / per_expert;
@@ -559,7 +597,12 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
         tcgen05_fence_after();
         const uint32_t d = tmem_base + acc * kAccCols;
         for (int kb = 0; kb < blocks; ++kb) {
-          if (!mbar_wait(s.full + 8 * stage, phase, wb)) {
+          bool full = mbar_wait(s.full + 8 * stage, phase, wb);
+          if (full && kb * kBK + kBK > rows) {           // the copied block
+            full = wait_cluster(s.tail, tail_phase, wb);
+            tail_phase ^= 1u;
+          }
+          if (!full) {
             report_status(p.status, kStatusTimeoutMbarrier, 113, blocks, kb, 0, t);
             ok = false;
             break;
@@ -582,6 +625,45 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
       if (!ok) {
         umma_commit_pair(s.drain, 1);
         for (int i = 0; i < 1000000 && !mbar_try_wait(s.drain, 0); ++i) {}
+      }
+    }
+  } else if (warp >= kThreads / 32) {
+    // ------------- copying warps: the partial block at the end of an expert -------------
+    // Thread c copies 16-byte chunk c % 8 of one half of the columns (c / 8 % 2) of the rows
+    // c / 16, c / 16 + 8, ... of both operands.  The arrival at the other CTA is a release at
+    // cluster scope, about a microsecond; it comes once per tile and runs ahead of the MMAs.
+    const int c = threadIdx.x - kThreads, chunk = c & 7, h = (c >> 3) & 1, row = c >> 4;
+    const uint32_t dst = h * kHalfBytes + row * 128 + ((chunk ^ row) << 4);
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
+      const int e = t / per_expert, local = t % per_expert;
+      const int x_a = local / p.n_tiles * kTile + cta * 128 + h * 64 + chunk * 8;
+      const int x_b = local % p.n_tiles * kTile + cta * 128 + h * 64 + chunk * 8;
+      const int row0 = slot_bound(p.offsets, e, p.slots), row1 = slot_bound(p.offsets, e + 1, p.slots);
+      for (int r0 = row0; r0 < row1; r0 += kBK) {
+        ok = copiers_all(mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb));
+        if (!ok) {
+          if (c == 0) report_status(p.status, kStatusTimeoutMbarrier, 115, 0, r0, 0, t);
+          break;
+        }
+        if (r0 + kBK > row1) {
+          const uint32_t sa = s.base + stage * kStageBytes + dst;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int64_t r = r0 + row + 8 * i;
+            const bool in_a = r < row1 && x_a < p.m, in_b = r < row1 && x_b < p.n;
+            copy_16(sa + i * 1024,
+                    static_cast<const char*>(p.a) + (in_a ? 2 * (r * p.lda + x_a) : 0), in_a);
+            copy_16(sa + kOperandBytes + i * 1024,
+                    static_cast<const char*>(p.b) + (in_b ? 2 * (r * p.ldb + x_b) : 0), in_b);
+          }
+          copy_wait_all();
+          fence_proxy_async_smem();
+          copiers_all(true);
+          if (c == 0) mbar_arrive_cluster(mapa_shared(s.tail, 0));
+        }
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
     }
   } else if (warp >= 4) {
@@ -680,8 +762,7 @@ GemmKernel gemm_kernel(int epilogue, bool gather) {
     case kNone: return gather ? expert_gemm_kernel<kNone, true> : expert_gemm_kernel<kNone, false>;
     case kSiluGate:
       return gather ? expert_gemm_kernel<kSiluGate, true> : expert_gemm_kernel<kSiluGate, false>;
-    default:
-      return gather ? expert_gemm_kernel<kSiluGateGrad, true> : expert_gemm_kernel<kSiluGateGrad, false>;
+    default: return expert_gemm_kernel<kSiluGateGrad, false>;
   }
 }
 
@@ -703,10 +784,11 @@ cudaError_t attrs_once(int* sms) {
 }
 
 template <typename P>
-cudaError_t launch_pairs(void (*kernel)(const P), const P& p, int pairs, int smem, cudaStream_t stream) {
+cudaError_t launch_pairs(void (*kernel)(const P), const P& p, int pairs, int threads, int smem,
+                         cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -758,7 +840,8 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
                  "too many rows");
   if (d.slots == 0) return kOk;
   TCCL_CHECK_ARG(d.x != 0 && d.w != 0 && d.out != 0 && d.offsets != 0 && d.x_rows >= 1, "null argument");
-  TCCL_CHECK_ARG(d.epilogue != kSiluGateGrad || d.dh != 0, "null argument");
+  TCCL_CHECK_ARG(d.epilogue != kSiluGateGrad || (d.dh != 0 && d.token_of_slot == 0),
+                 "the gate's gradient takes slot-ordered rows and dh");
   const int64_t f_tiles = (d.n + kTile - 1) / kTile;
   const int64_t tiles = (d.slots / kTile + (d.slots < d.experts ? d.slots : d.experts)) * f_tiles;
   TCCL_CHECK_ARG(tiles < (int64_t(1) << 31), "too many tiles");
@@ -768,8 +851,10 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   int rc = encode(&p.tma_w, bf16, d.w, d.w_nk ? d.k : d.n, d.w_nk ? d.n : d.k, d.experts, d.ldw * 2,
                   d.w_expert * 2, 64, "W");
   if (rc) return rc;
-  rc = encode(&p.tma_x, bf16, d.x, d.k, d.x_rows, 0, d.ldx * 2, 0, gather ? 1 : 16, "X");
-  if (rc) return rc;
+  for (int i = 0; i < (gather ? 1 : 4); ++i) {
+    rc = encode(&p.tma_x[i], bf16, d.x, d.k, d.x_rows, 0, d.ldx * 2, 0, gather ? 1 : 128 >> i, "X");
+    if (rc) return rc;
+  }
   p.offsets = reinterpret_cast<const int32_t*>(d.offsets);
   p.token_of_slot = reinterpret_cast<const int32_t*>(d.token_of_slot);
   p.out = reinterpret_cast<void*>(d.out);
@@ -789,7 +874,8 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   int sms = 0;
   TCCL_CHECK_CUDA(attrs_once(&sms));
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
-  TCCL_CHECK_CUDA(launch_pairs(gemm_kernel(d.epilogue, gather), p, pairs, kGemmSmem,
+  TCCL_CHECK_CUDA(launch_pairs(gemm_kernel(d.epilogue, gather), p, pairs,
+                               kThreads, kGemmSmem,
                                reinterpret_cast<cudaStream_t>(stream)));
   return kOk;
 }
@@ -804,47 +890,42 @@ extern "C" int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_
   TCCL_CHECK_ARG(d.m % 8 == 0 && d.n % 8 == 0, "rows and columns must be multiples of 8");
   TCCL_CHECK_ARG(d.lda % 8 == 0 && d.ldb % 8 == 0, "leading dimensions must be multiples of 8 elements");
   TCCL_CHECK_ARG(d.a % 16 == 0 && d.b % 16 == 0 && d.out % 16 == 0, "operands must be 16-byte aligned");
-  TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) - kTile &&
-                     d.a_rows < (int64_t(1) << 31) && d.b_rows < (int64_t(1) << 31), "too many rows");
+  TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) - kTile, "too many rows");
   TCCL_CHECK_ARG(d.out != 0 && d.offsets != 0, "null argument");
   if (d.slots == 0) {
     TCCL_CHECK_CUDA(cudaMemsetAsync(reinterpret_cast<void*>(d.out), 0, d.experts * d.m * d.n * 2,
                                     reinterpret_cast<cudaStream_t>(stream)));
     return kOk;
   }
-  TCCL_CHECK_ARG(d.a != 0 && d.b != 0 && d.a_rows >= 1 && d.b_rows >= 1, "null argument");
-  TCCL_CHECK_ARG(!(d.gather_a || d.gather_b) || d.token_of_slot != 0, "null argument");
+  TCCL_CHECK_ARG(d.a != 0 && d.b != 0, "null argument");
   const int64_t m_tiles = (d.m + kTile - 1) / kTile, n_tiles = (d.n + kTile - 1) / kTile;
   const int64_t tiles = d.experts * m_tiles * n_tiles;
   TCCL_CHECK_ARG(tiles < (int64_t(1) << 31), "too many tiles");
   TCCL_REQUIRE_DRIVER();
   const bool bf16 = d.dtype == 1;
   GradParams p;
-  int rc = encode(&p.tma_a, bf16, d.a, d.m, d.a_rows, 0, d.lda * 2, 0, 64, "A");
-  if (!rc) rc = encode(&p.tma_b, bf16, d.b, d.n, d.b_rows, 0, d.ldb * 2, 0, 64, "B");
-  if (!rc) rc = encode(&p.tma_a_rows, bf16, d.a, d.m, d.a_rows, 0, d.lda * 2, 0, 1, "A");
-  if (!rc) rc = encode(&p.tma_b_rows, bf16, d.b, d.n, d.b_rows, 0, d.ldb * 2, 0, 1, "B");
+  int rc = encode(&p.tma_a, bf16, d.a, d.m, d.slots, 0, d.lda * 2, 0, 64, "A");
+  if (!rc) rc = encode(&p.tma_b, bf16, d.b, d.n, d.slots, 0, d.ldb * 2, 0, 64, "B");
   if (!rc) rc = encode(&p.tma_out, bf16, d.out, d.n, d.m, d.experts, d.n * 2, d.m * d.n * 2, 32, "out");
   if (rc) return rc;
   p.offsets = reinterpret_cast<const int32_t*>(d.offsets);
-  p.token_of_slot = reinterpret_cast<const int32_t*>(d.token_of_slot);
+  p.a = reinterpret_cast<const void*>(d.a);
+  p.b = reinterpret_cast<const void*>(d.b);
+  p.lda = d.lda;
+  p.ldb = d.ldb;
   p.slots = static_cast<int32_t>(d.slots);
-  p.a_rows = static_cast<int32_t>(d.a_rows);
-  p.b_rows = static_cast<int32_t>(d.b_rows);
   p.experts = d.experts;
   p.m = static_cast<int32_t>(d.m);
   p.n = static_cast<int32_t>(d.n);
   p.m_tiles = static_cast<int32_t>(m_tiles);
   p.n_tiles = static_cast<int32_t>(n_tiles);
   p.bf16 = bf16 ? 1 : 0;
-  p.gather_a = d.gather_a;
-  p.gather_b = d.gather_b;
   p.status = reinterpret_cast<uint32_t*>(d.status);
   p.budget_ns = kWaitBudgetNs;
   int sms = 0;
   TCCL_CHECK_CUDA(attrs_once(&sms));
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
-  TCCL_CHECK_CUDA(launch_pairs(&expert_weight_grad_kernel, p, pairs, kGradSmem,
+  TCCL_CHECK_CUDA(launch_pairs(&expert_weight_grad_kernel, p, pairs, kThreads + kCopyThreads, kGradSmem,
                                reinterpret_cast<cudaStream_t>(stream)));
   return kOk;
 }

@@ -33,6 +33,13 @@ MAX_ROUTED_EXPERTS = 512
 MAX_EXPERTS = 1024
 MAX_TOP_K = 32
 
+# Up to this many slots the product gathers the tokens' rows itself (TMA, four rows per copy);
+# above, a copy kernel puts them in slot order first.  The TMA unit needs some 70 cycles for four
+# rows, which a tile of 64 tokens hides behind its weights and one of 256 does not: gated product
+# of 8192 tokens x top 2, 4096 x 28672: 8.4 ms gathered in the kernel, 2.5 ms behind the copy
+# (35 us).  With few slots the extra launch would cost more than it saves.
+GATHER_IN_KERNEL_SLOTS = 64
+
 _LOGIT_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _EPILOGUES = {"none": 0, "silu_gate": 1}
 _EPI_SILU_GATE_GRAD = 2
@@ -323,6 +330,15 @@ def _aligned(name, t) -> int:
     return ld
 
 
+def _gather(X, slots, raw):
+    """``X``'s rows in slot order."""
+    S, K = slots.capacity, X.shape[1]
+    xs = torch.empty((S, K), dtype=X.dtype, device=X.device)
+    _launch("tccl_expert_gather", X.data_ptr(), _aligned("X", X), X.shape[0],
+            slots.token_of_slot.data_ptr(), xs.data_ptr(), K, S, K, raw)
+    return xs
+
+
 def _product(X, W, slots, out, rows, b_is_nk, epi, dh, raw):
     """One launch of the grouped product; every argument is checked already."""
     E = W.shape[0]
@@ -362,6 +378,8 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
     with _on(stream, (X, W, slots.offsets, slots.token_of_slot, out)) as raw:
         if out is None:
             out = torch.empty(shape, dtype=X.dtype, device=X.device)
+        if rows == "tokens" and slots.capacity > GATHER_IN_KERNEL_SLOTS:
+            X, rows = _gather(X, slots, raw), "slots"
         _product(X, W, slots, out, rows, b_is_nk, epi, None, raw)
     return out
 
@@ -381,12 +399,14 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
     _check_rows("grad_out", grad_out, (slots.capacity, N // 2 if epi else N), X)
     S = slots.capacity
     with _on(stream, (X, W, grad_out, slots.offsets, slots.token_of_slot, slots.slot_of)) as raw:
+        # (once in slot order for both products that read X)
+        xs = _gather(X, slots, raw) if rows == "tokens" else X
         dy = grad_out
         if epi:
             # gate and up again, their gradients straight from the accumulators (one rounding
             # to 16 bits: the operand type of the two products that follow)
             dy = torch.empty((S, N), dtype=X.dtype, device=X.device)
-            _product(X, W, slots, dy, rows, b_is_nk, _EPI_SILU_GATE_GRAD, grad_out, raw)
+            _product(xs, W, slots, dy, "slots", b_is_nk, _EPI_SILU_GATE_GRAD, grad_out, raw)
         grad_rows = torch.empty((S, K), dtype=X.dtype, device=X.device)
         _product(dy, W, slots, grad_rows, "slots", not b_is_nk, 0, None, raw)
         grad_X = grad_rows
@@ -394,13 +414,11 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
             grad_X = torch.empty((slots.tokens, K), dtype=X.dtype, device=X.device)
             _combine(grad_rows, slots, None, None, grad_X, raw)
         grad_W = torch.empty(W.shape, dtype=X.dtype, device=X.device)
+        a, b = (dy, xs) if b_is_nk else (xs, dy)
         d = _native.ExpertWeightGrad()
         d.dtype, d.experts, d.slots = _fg.dtype_code(X.dtype), E, S
-        d.offsets, d.token_of_slot = slots.offsets.data_ptr(), slots.token_of_slot.data_ptr()
-        a, b = (dy, X) if b_is_nk else (X, dy)
-        d.gather_a = 1 if rows == "tokens" and a is X else 0
-        d.gather_b = 1 if rows == "tokens" and b is X else 0
-        d.m, d.n, d.a_rows, d.b_rows = a.shape[1], b.shape[1], a.shape[0], b.shape[0]
+        d.offsets = slots.offsets.data_ptr()
+        d.m, d.n = a.shape[1], b.shape[1]
         d.a, d.b, d.out = a.data_ptr(), b.data_ptr(), grad_W.data_ptr()
         d.lda, d.ldb = _aligned("X", a), _aligned("X", b)
         d.status = _status_ptr(X.device)
