@@ -163,9 +163,7 @@ class ExpertGemm(C.Structure):
         ("k", C.c_int64),
         ("n", C.c_int64),
         ("slots", C.c_int64),
-        ("x_rows", C.c_int64),
         ("offsets", C.c_uint64),
-        ("token_of_slot", C.c_uint64),
         ("x", C.c_uint64),
         ("w", C.c_uint64),
         ("out", C.c_uint64),
@@ -176,6 +174,8 @@ class ExpertGemm(C.Structure):
         ("ldo", C.c_int64),
         ("ld_dh", C.c_int64),
         ("status", C.c_uint64),
+        ("partial", C.c_uint64),
+        ("counters", C.c_uint64),
     ]
 
 
@@ -265,6 +265,7 @@ def _declare(lib: C.CDLL) -> None:
         "tccl_expert_slots_workspace": [i64, i32, C.POINTER(i64)],
         "tccl_expert_slots": [u64, i64, i32, i32, i32, u64, u64, u64, u64, u64],
         "tccl_expert_gemm": [C.POINTER(ExpertGemm), u64],
+        "tccl_expert_gemm_scratch": [i64, i64, C.POINTER(i64), C.POINTER(i64)],
         "tccl_expert_weight_grad": [C.POINTER(ExpertWeightGrad), u64],
         "tccl_expert_gather": [u64, i64, i64, u64, u64, i64, i64, i32, u64],
         "tccl_expert_combine": [u64, i64, u64, u64, u64, i64, u64, i64, i64, i64, i32, i32, i32, u64],

@@ -328,14 +328,19 @@ int tccl_expert_slots(uint64_t ids, int64_t tokens, int32_t top_k, int32_t exper
 typedef struct TcclExpertGemm {
   int32_t dtype, epilogue;    // epilogue: 0 none, 1 SiLU gate, 2 gradient of the SiLU gate
   int32_t experts, w_nk;      // w_nk: W is [experts, N, K], else [experts, K, N]
-  int64_t k, n, slots, x_rows;
+  int64_t k, n, slots;
   uint64_t offsets;           // int32[experts + 1]
-  uint64_t token_of_slot;     // int32[slots]; 0 = row s of x belongs to slot s
-  uint64_t x, w, out, dh;     // dh: epilogue 2 only
+  uint64_t x, w, out, dh;     // x: row s belongs to slot s; dh: epilogue 2 only
   int64_t ldx, ldw, w_expert, ldo, ld_dh;   // pitches in elements
   uint64_t status;            // uint32[8] status words (0 = a wait that gave up is not reported)
+  uint64_t partial, counters; // scratch of tccl_expert_gemm_scratch's sizes, 0 = none
 } TcclExpertGemm;
 int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream);
+// Scratch with which a product shares its tiles evenly among the SMs (0 bytes: it would not
+// help).  `counters` must be zero before the first call, every call leaves them at zero; two
+// calls that may run at the same time need scratch of their own.
+int tccl_expert_gemm_scratch(int64_t slots, int64_t k, int64_t* partial_bytes,
+                             int64_t* counter_bytes);
 
 // out[e] = sum over the slots s of expert e of a[s]^T b[s]: [experts, m, n] contiguous.
 typedef struct TcclExpertWeightGrad {

@@ -1,7 +1,7 @@
 // Products of the experts over a slot map (expert_slots.cu): every slot's row times the weight
 // matrix of its expert, and the gradient of those weights, on the sm_100a tensor cores.
 //
-//   out[s] = x[row(s)] @ W[e(s)]                                row(s) = token of slot s, or s
+//   out[s] = x[s] @ W[e(s)]
 //   SiLU gate: W's columns come as 128 gate columns followed by 128 up columns;
 //              out[s] = silu(gate) * up, half as wide
 //   gradient of the gate: gate and up are computed again and with dh[s] = dL/dout[s]
@@ -38,10 +38,11 @@ constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kTile = 256;               // features (M) and, at most, tokens (N) of a pair's tile
 constexpr int kAccCols = 256;            // TMEM columns of one accumulator
 constexpr int kBand = 16;                // token tiles that share a sweep over the features
+constexpr int kMinBlocks = 4;            // K blocks a pair takes at least of a shared tile
 constexpr int kChunk = 16;               // tokens per epilogue step
 constexpr int kStageLd = 132;            // floats between tokens of the staging buffer
 constexpr int kStagingBytes = 2 * kChunk * kStageLd * 4;
-constexpr int kCtlBytes = 1024;         // barriers; from 512 on the rows a gathering CTA stages
+constexpr int kCtlBytes = 512;
 constexpr int kListBytes = 2 * 4 * (kMaxExperts + 2);
 constexpr int kGemmSmem = kStages * kStageBytes + kStagingBytes + kCtlBytes + kListBytes + 1024;
 constexpr int kGradStagingBytes = 4 * 2 * 4096;   // per epilogue warp two buffers of 32 x 64
@@ -50,14 +51,15 @@ static_assert(kGemmSmem <= 232448 && kGradSmem <= 232448, "shared memory of one 
 
 struct GemmParams {
   CUtensorMap tma_w;          // {columns, rows, experts}, box {64, 64, 1}, 128-byte swizzle
-  CUtensorMap tma_x[4];       // {K, rows}, boxes {64, 128}, {64, 64}, {64, 32}, {64, 16};
-                              // gathered: [0] only, box {64, 1}
+  CUtensorMap tma_x[4];       // {K, rows}, boxes {64, 128}, {64, 64}, {64, 32}, {64, 16}
   const int32_t* offsets;
-  const int32_t* token_of_slot;
   void* out;
   const void* dh;
+  float* partial;             // [pairs][2][2 CTAs][128 * partial_tokens], null = tiles stay whole
+  uint32_t* counters;         // [2 * pairs][2], zero between calls
   int64_t ldo, ld_dh;
-  int32_t slots, x_rows, experts, k_blocks, n, f_tiles, bf16, w_nk;
+  int32_t partial_tokens;
+  int32_t slots, experts, k_blocks, n, f_tiles, bf16, w_nk;
   uint32_t* status;
   uint64_t budget_ns;
 };
@@ -89,16 +91,6 @@ __device__ __forceinline__ void copy_16(uint32_t dst, const void* src, bool take
                : "memory");
 }
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// Four rows of a matrix, 64 columns each, into 512 consecutive bytes (swizzled by address).
-__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap* m, int x,
-                                                 const int (&r)[4], uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4"
-      ".mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-      "r"(bar)
-      : "memory");
-}
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, int x, int y, int z,
                                              uint32_t src) {
   asm volatile(
@@ -286,18 +278,41 @@ __device__ __forceinline__ void store_row8(void* base, int64_t i, bool bf16, con
 }
 
 // ---------------------------------------------------------------------------------------
-// out[s] = epilogue(x[row(s)] @ W[e(s)])
+// out[s] = epilogue(x[s] @ W[e(s)])
 //
 // The weights are the M operand (256 features per pair, 128 per CTA) and the tokens the N
 // operand: M is fixed to 256 by the pair form of the instruction while N may be any multiple
 // of 32, so an expert's tile is as wide as its rows need.  With the gate a CTA's 128 features
 // are 64 gate columns and the 64 up columns that belong to them.
 // ---------------------------------------------------------------------------------------
+//
+// Schedule: tile t goes to pair t mod P.  With few tokens the time is that of streaming the
+// weights, and half of the SMs suffice to draw the full memory bandwidth: only a last round with
+// fewer tiles than that is worth spreading.  The first R = P + T mod P tiles (all of them when
+// T < P) are then cut into P equal runs of K blocks: a pair's run covers the end of one tile,
+// whole tiles, the start of another.  Parts of a tile are left in `partial` as fp32 sums;
+// whichever pair comes last (a counter per tile and CTA) adds them up in the order of K, so the
+// result does not depend on who that was.  Measured with one token (us, shared / whole): 2
+// experts of 14336 x 4096 47 / 56, 1 expert 28 / 55, 4 tokens of 2 104 / 129; against that 8
+// experts of 2048 x 1024 16 / 14 (short K), 8 of 4096 x 3584 50 / 45 (T = 1.5 P), and 512 tokens
+// of 2 204 / 158 (wide partial tiles), all of which stay whole.
+// ---------------------------------------------------------------------------------------
 struct Item {
   int e, row0, rows, n, f0;
+  int kb0, kb1;              // K blocks of this item
+  int part, parts, slot;     // parts > 1: the tile is shared; slot = the tile's counter
+  int first_pair;            // pair that computes part 0
 };
 
-template <int kEpi, bool kGather>
+// The items of one pair, in order; every role walks the same list.
+struct Walker {
+  int pos, end;              // K blocks of the shared tiles (tile * k_blocks + block)
+  int unit;                  // K blocks per pair there
+  int shared;                // tiles that are cut up
+  int next;                  // next whole tile
+};
+
+template <int kEpi>
 __global__ void __launch_bounds__(kThreads, 1)
 expert_gemm_kernel(const __grid_constant__ GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -312,11 +327,40 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
   wb.start(p.budget_ns, s.words + 1);
 
   const int total = s.tiles[p.experts];
-  const int step = static_cast<int>(gridDim.x >> 1);
+  const int pairs = static_cast<int>(gridDim.x >> 1), pair = static_cast<int>(blockIdx.x >> 1);
+  auto walk = [&]() {
+    Walker w;
+    const int over = total % pairs;
+    w.shared = p.partial == nullptr || 2 * over >= pairs ? 0 : total < pairs ? total : over > 0 ? pairs + over : 0;
+    const int blocks = w.shared * p.k_blocks;      // (at most 2 * pairs tiles)
+    w.unit = max((blocks + pairs - 1) / pairs, min(kMinBlocks, p.k_blocks));
+    w.pos = min(pair * w.unit, blocks);
+    w.end = min(w.pos + w.unit, blocks);
+    w.next = w.shared + pair;
+    return w;
+  };
   // Tile t: token tiles run fastest, in bands of kBand, so that the tiles in flight share both
   // their weights and a band of tokens in L2.
-  auto item_of = [&](int t) {
-    Item it;
+  auto advance = [&](Walker& w, Item& it) {
+    int t;
+    if (w.pos < w.end) {
+      t = w.pos / p.k_blocks;
+      it.kb0 = w.pos - t * p.k_blocks;
+      it.kb1 = min(p.k_blocks, it.kb0 + w.end - w.pos);
+      w.pos += it.kb1 - it.kb0;
+      it.first_pair = t * p.k_blocks / w.unit;
+      it.part = pair - it.first_pair;
+      it.parts = ((t + 1) * p.k_blocks - 1) / w.unit - it.first_pair + 1;
+      it.slot = t;
+    } else {
+      t = w.next;
+      if (t >= total) return false;
+      w.next += pairs;
+      it.kb0 = 0;
+      it.kb1 = p.k_blocks;
+      it.part = it.slot = it.first_pair = 0;
+      it.parts = 1;
+    }
     it.e = expert_of(s, p.experts, t);
     const int rows = s.start[it.e + 1] - s.start[it.e];
     const int tiles = (rows + kTile - 1) / kTile;
@@ -330,39 +374,22 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
     it.row0 = s.start[it.e] + ti * per;
     it.rows = min(per, rows - ti * per);
     it.n = (max(it.rows, 1) + 31) & ~31;
-    return it;
+    return true;
   };
+  Walker w = walk();
+  Item it;
 
   if (warp == 0) {
     // ------------------------------- TMA producer -------------------------------
-    uint32_t stage = 0, phase = 0;
-    bool ok = true;
-    for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
-      const Item it = item_of(t);
-      const int mine = it.n >> 1;                          // token rows this CTA stages
-      const int first = it.row0 + cta * mine;
-      if (kGather) {
-        // Rows behind the tile's last slot (and tokens that do not exist) are read out of
-        // range: the copy fills them with zeros.
-        int4 r;
-        int* const rj = &r.x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int slot = first + 4 * lane + j;
-          int tok = -1;
-          if (4 * lane < mine && slot < it.row0 + it.rows) tok = p.token_of_slot[slot];
-          rj[j] = tok >= 0 && tok < p.x_rows ? tok : p.x_rows;
-        }
-        __syncwarp();
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s.ctl + 512 + 16 * lane), "r"(r.x),
-                     "r"(r.y), "r"(r.z), "r"(r.w)
-                     : "memory");
-        __syncwarp();
-      }
-      if (elect_one_sync()) {
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+    if (elect_one_sync()) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      while (ok && advance(w, it)) {
+        const int mine = it.n >> 1;                          // token rows this CTA stages
+        const int first = it.row0 + cta * mine;
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (!mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb)) {
-            report_status(p.status, kStatusTimeoutMbarrier, 101, 0, kb, 0, t);
+            report_status(p.status, kStatusTimeoutMbarrier, 101, 0, kb, 0, it.row0);
             ok = false;
             break;
           }
@@ -376,52 +403,39 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
             if (p.w_nk) tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, kb * kBK, f, it.e, bar);
             else tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, f, kb * kBK, it.e, bar);
           }
-          if (kGather) {
-            for (int i = 0; i < mine; i += 4) {
-              int r[4];
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                           : "r"(s.ctl + 512 + 4 * i));
-              tma_gather4_pair(sb + i * 128, &p.tma_x[0], kb * kBK, r, bar);
-            }
-          } else {
-            // as few boxes as the row count has binary digits: a copy keeps the TMA unit busy
-            // however small it is (boxes of 16 rows throughout: 999 instead of 1549 TFLOP/s)
-            int at = 0;
+          // as few boxes as the row count has binary digits: a copy keeps the TMA unit busy for
+          // some 70 cycles however small it is (boxes of 16 rows throughout: 999 instead of 1549
+          // TFLOP/s; the unit's own gather, four rows per copy: 460)
+          int at = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (mine & (128 >> i)) {
-                tma_load_2d_pair(sb + at * 128, &p.tma_x[i], kb * kBK, first + at, bar);
-                at += 128 >> i;
-              }
+          for (int i = 0; i < 4; ++i) {
+            if (mine & (128 >> i)) {
+              tma_load_2d_pair(sb + at * 128, &p.tma_x[i], kb * kBK, first + at, bar);
+              at += 128 >> i;
             }
           }
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
-      // (the elected thread's state is the only one that counts; the warp leaves together)
-      __syncwarp();
-      ok = !wb.aborted();
+      if (!ok) drain_copies();
     }
-    if (!ok) drain_copies();
   } else if (warp == 1 && leader) {
     // ----------------------- MMA issuer (leader CTA only) -----------------------
     if (elect_one_sync()) {
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
-        const Item it = item_of(t);
+      while (ok && advance(w, it)) {
         const uint32_t idesc = umma_idesc_f16(p.bf16, p.w_nk ? 0 : 1, 0, kTile, it.n);
         if (!mbar_wait(s.acc_empty + 8 * acc, acc_phase ^ 1u, wb)) {
-          report_status(p.status, kStatusTimeoutMbarrier, 102, 0, 0, 0, t);
+          report_status(p.status, kStatusTimeoutMbarrier, 102, 0, 0, 0, it.row0);
           ok = false;
           break;
         }
         tcgen05_fence_after();
         const uint32_t d = tmem_base + acc * kAccCols;
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (!mbar_wait(s.full + 8 * stage, phase, wb)) {
-            report_status(p.status, kStatusTimeoutMbarrier, 103, p.k_blocks, kb, 0, t);
+            report_status(p.status, kStatusTimeoutMbarrier, 103, it.kb1, kb, 0, it.row0);
             ok = false;
             break;
           }
@@ -432,7 +446,7 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
             const uint64_t da = p.w_nk ? umma_smem_desc_sw128(sa + k * kUmmaK * 2, 16, 1024)
                                        : umma_smem_desc_sw128(sa + k * kUmmaK * 128, kHalfBytes, 1024);
             const uint64_t db = umma_smem_desc_sw128(sb + k * kUmmaK * 2, 16, 1024);
-            umma_f16_pair(d, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+            umma_f16_pair(d, da, db, idesc, kb > it.kb0 || k > 0 ? 1u : 0u);
           }
           umma_commit_pair(s.empty + 8 * stage, 3);
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
@@ -457,22 +471,74 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
     const bool bf16 = p.bf16 != 0;
     constexpr int kVecs = kEpi == kNone ? 16 : 8;          // 8-feature vectors per token
     uint32_t acc = 0, acc_phase = 0, buf = 0;
-    for (int t = blockIdx.x >> 1; t < total; t += step) {
-      const Item it = item_of(t);
+    while (advance(w, it)) {
       if (!epilogue_all(mbar_wait(s.acc_full + 8 * acc, acc_phase, wb))) {
-        if (me == 0) report_status(p.status, kStatusTimeoutMbarrier, 104, 0, 0, 0, t);
+        if (me == 0) report_status(p.status, kStatusTimeoutMbarrier, 104, 0, 0, 0, it.row0);
         break;
       }
       tcgen05_fence_after();
       const uint32_t t_acc = tmem_base + acc * kAccCols + (static_cast<uint32_t>(q * 32) << 16);
-      for (int c0 = 0; c0 < it.n; c0 += kChunk) {
-        float v[kChunk];
+      const int last_c0 = (max(it.rows, 1) - 1) / kChunk * kChunk;
+      auto read_acc = [&](int c0, float (&v)[kChunk]) {
         tmem_ld_x16(t_acc + c0, v);
-        if (c0 + kChunk >= it.n) {
-          // every TMEM read of this accumulator is done: hand it back to the MMA warp
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(mapa_shared(s.acc_empty + 8 * acc, 0));
+        if (c0 != last_c0) return;
+        // every TMEM read of this accumulator is done: hand it back to the MMA warp
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(s.acc_empty + 8 * acc, 0));
+      };
+      // Parts of a shared tile: part q lies at pair first_pair + q, in its second place if the
+      // tile starts there.  Layout: [step of 16 tokens][4][feature][4 tokens].
+      auto partial_of = [&](int part) {
+        const int64_t at = ((it.first_pair + part) * 2 + (part == 0 ? 1 : 0)) * 2 + cta;
+        return p.partial + at * p.partial_tokens * 128 + me * 4;
+      };
+      if (it.parts > 1) {
+        float* const mine = partial_of(it.part);
+        for (int c0 = 0; c0 <= last_c0; c0 += kChunk) {
+          float v[kChunk];
+          read_acc(c0, v);
+#pragma unroll
+          for (int j = 0; j < kChunk / 4; ++j)
+            __stcg(reinterpret_cast<float4*>(mine + (c0 / 4 + j) * 512),
+                   make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+        }
+        __threadfence();
+        epilogue_sync();
+        if (me == 0) {
+          uint32_t* const ctr = p.counters + it.slot * 2 + cta;
+          const bool last = atomicAdd(ctr, 1u) == static_cast<uint32_t>(it.parts - 1);
+          if (last) *ctr = 0;                      // as the next call finds it
+          s.words[2] = last ? 1u : 0u;
+        }
+        epilogue_sync();
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+        if (s.words[2] == 0) continue;
+        __threadfence();
+      }
+      for (int c0 = 0; c0 <= last_c0; c0 += kChunk) {
+        uint4 dh = make_uint4(0, 0, 0, 0);
+        if (kEpi == kSiluGateGrad && c0 + me / kVecs < it.rows)      // (one vector per thread)
+          dh = __ldg(reinterpret_cast<const uint4*>(
+              static_cast<const char*>(p.dh) +
+              2 * (static_cast<int64_t>(it.row0 + c0 + me / kVecs) * p.ld_dh + it.f0 / 2 + cta * 64 +
+                   me % kVecs * 8)));
+        float v[kChunk];
+        if (it.parts > 1) {
+          for (int i = 0; i < it.parts; ++i) {
+            const float* const src = partial_of(i);
+#pragma unroll
+            for (int j = 0; j < kChunk / 4; ++j) {
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (c0 / 4 + j) * 512));
+              v[4 * j] = i == 0 ? x.x : v[4 * j] + x.x;
+              v[4 * j + 1] = i == 0 ? x.y : v[4 * j + 1] + x.y;
+              v[4 * j + 2] = i == 0 ? x.z : v[4 * j + 2] + x.z;
+              v[4 * j + 3] = i == 0 ? x.w : v[4 * j + 3] + x.w;
+            }
+          }
+        } else {
+          read_acc(c0, v);
         }
         float* const sbuf = staging + buf * (kChunk * kStageLd);
         buf ^= 1u;
@@ -503,8 +569,7 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
             store_row8(p.out, slot * p.ldo + f, bf16, a);
           } else {
             float g[8] = {};
-            tile_accumulate_16x8(bf16, g, *reinterpret_cast<const uint4*>(
-                static_cast<const char*>(p.dh) + 2 * (slot * p.ld_dh + f)));
+            tile_accumulate_16x8(bf16, g, dh);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float sg = apply_elementwise(kOpSigmoid, a[j]);
@@ -518,8 +583,10 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
           }
         }
       }
-      acc ^= 1u;
-      if (acc == 0) acc_phase ^= 1u;
+      if (it.parts == 1) {
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+      }
     }
   }
   pipe_end(tmem_base);
@@ -757,13 +824,10 @@ int encode(CUtensorMap* map, bool bf16, uint64_t base, uint64_t cols, uint64_t r
 }
 
 using GemmKernel = void (*)(const GemmParams);
-GemmKernel gemm_kernel(int epilogue, bool gather) {
-  switch (epilogue) {
-    case kNone: return gather ? expert_gemm_kernel<kNone, true> : expert_gemm_kernel<kNone, false>;
-    case kSiluGate:
-      return gather ? expert_gemm_kernel<kSiluGate, true> : expert_gemm_kernel<kSiluGate, false>;
-    default: return expert_gemm_kernel<kSiluGateGrad, false>;
-  }
+GemmKernel gemm_kernel(int epilogue) {
+  return epilogue == kNone       ? expert_gemm_kernel<kNone>
+         : epilogue == kSiluGate ? expert_gemm_kernel<kSiluGate>
+                                 : expert_gemm_kernel<kSiluGateGrad>;
 }
 
 cudaError_t attrs_once(int* sms) {
@@ -773,8 +837,8 @@ cudaError_t attrs_once(int* sms) {
   if (e != cudaSuccess) return e;
   if (dev < 64 && count[dev] != 0) { *sms = count[dev]; return cudaSuccess; }
   e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
-  for (int i = 0; i < 6 && e == cudaSuccess; ++i)
-    e = cudaFuncSetAttribute(gemm_kernel(i / 2, i % 2 != 0),
+  for (int i = 0; i < 3 && e == cudaSuccess; ++i)
+    e = cudaFuncSetAttribute(gemm_kernel(i),
                              cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(expert_weight_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -801,6 +865,14 @@ cudaError_t launch_pairs(void (*kernel)(const P), const P& p, int pairs, int thr
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+// Tiles of a product at most: a partial tile more per expert that has rows.
+int64_t most_tiles(int64_t slots, int64_t experts, int64_t n) {
+  return (slots / kTile + (slots < experts ? slots : experts)) * ((n + kTile - 1) / kTile);
+}
+int32_t partial_tokens(int64_t slots) {
+  return static_cast<int32_t>(slots < kTile ? (slots + 31) / 32 * 32 : kTile);
+}
+
 constexpr uint64_t kWaitBudgetNs = 2000000000ull;
 
 }  // namespace
@@ -809,8 +881,7 @@ cudaError_t preload_expert_gemm_kernels() {
   cudaFuncAttributes a;
   int sms = 0;
   cudaError_t e = cudaFuncGetAttributes(&a, expert_weight_grad_kernel);
-  for (int i = 0; i < 6 && e == cudaSuccess; ++i)
-    e = cudaFuncGetAttributes(&a, gemm_kernel(i / 2, i % 2 != 0));
+  for (int i = 0; i < 3 && e == cudaSuccess; ++i) e = cudaFuncGetAttributes(&a, gemm_kernel(i));
   if (e == cudaSuccess) e = attrs_once(&sms);
   return e;
 }
@@ -818,6 +889,23 @@ cudaError_t preload_expert_gemm_kernels() {
 }  // namespace tileccl
 
 using namespace tileccl;
+
+// Tiles are shared for at most this many slots, and at least this long a contraction (see the
+// schedule of expert_gemm_kernel).
+constexpr int64_t kSharedSlots = 128, kSharedK = 4096;
+
+extern "C" int tccl_expert_gemm_scratch(int64_t slots, int64_t k, int64_t* partial_bytes,
+                                        int64_t* counter_bytes) {
+  TCCL_CHECK_ARG(partial_bytes != nullptr && counter_bytes != nullptr, "null argument");
+  *partial_bytes = *counter_bytes = 0;
+  int sms = 0;
+  TCCL_CHECK_CUDA(attrs_once(&sms));
+  const int64_t pairs = sms / 2;
+  if (slots <= 0 || slots > kSharedSlots || k < kSharedK) return kOk;
+  *partial_bytes = pairs * 4 * 128 * partial_tokens(slots) * static_cast<int64_t>(sizeof(float));
+  *counter_bytes = pairs * 4 * static_cast<int64_t>(sizeof(uint32_t));
+  return kOk;
+}
 
 extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   TCCL_CHECK_ARG(desc != nullptr, "null argument");
@@ -836,35 +924,35 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
                  "operands must be 16-byte aligned");
   TCCL_CHECK_ARG(d.epilogue == kNone || d.n % 256 == 0,
                  "SiLU-gate epilogue needs N to be a multiple of 256");
-  TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) - kTile && d.x_rows < (int64_t(1) << 31),
-                 "too many rows");
+  TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) - kTile, "too many rows");
   if (d.slots == 0) return kOk;
-  TCCL_CHECK_ARG(d.x != 0 && d.w != 0 && d.out != 0 && d.offsets != 0 && d.x_rows >= 1, "null argument");
-  TCCL_CHECK_ARG(d.epilogue != kSiluGateGrad || (d.dh != 0 && d.token_of_slot == 0),
-                 "the gate's gradient takes slot-ordered rows and dh");
-  const int64_t f_tiles = (d.n + kTile - 1) / kTile;
-  const int64_t tiles = (d.slots / kTile + (d.slots < d.experts ? d.slots : d.experts)) * f_tiles;
+  TCCL_CHECK_ARG(d.x != 0 && d.w != 0 && d.out != 0 && d.offsets != 0, "null argument");
+  TCCL_CHECK_ARG(d.epilogue != kSiluGateGrad || d.dh != 0, "null argument");
+  TCCL_CHECK_ARG(d.partial == 0 || (d.counters != 0 && d.partial % 16 == 0), "bad scratch");
+  const int64_t f_tiles = (d.n + kTile - 1) / kTile, tiles = most_tiles(d.slots, d.experts, d.n);
   TCCL_CHECK_ARG(tiles < (int64_t(1) << 31), "too many tiles");
   TCCL_REQUIRE_DRIVER();
-  const bool bf16 = d.dtype == 1, gather = d.token_of_slot != 0;
+  const bool bf16 = d.dtype == 1;
   GemmParams p;
   int rc = encode(&p.tma_w, bf16, d.w, d.w_nk ? d.k : d.n, d.w_nk ? d.n : d.k, d.experts, d.ldw * 2,
                   d.w_expert * 2, 64, "W");
   if (rc) return rc;
-  for (int i = 0; i < (gather ? 1 : 4); ++i) {
-    rc = encode(&p.tma_x[i], bf16, d.x, d.k, d.x_rows, 0, d.ldx * 2, 0, gather ? 1 : 128 >> i, "X");
+  for (int i = 0; i < 4; ++i) {
+    rc = encode(&p.tma_x[i], bf16, d.x, d.k, d.slots, 0, d.ldx * 2, 0, 128 >> i, "X");
     if (rc) return rc;
   }
   p.offsets = reinterpret_cast<const int32_t*>(d.offsets);
-  p.token_of_slot = reinterpret_cast<const int32_t*>(d.token_of_slot);
   p.out = reinterpret_cast<void*>(d.out);
   p.dh = reinterpret_cast<const void*>(d.dh);
   p.ldo = d.ldo;
   p.ld_dh = d.ld_dh;
   p.slots = static_cast<int32_t>(d.slots);
-  p.x_rows = static_cast<int32_t>(d.x_rows);
-  p.experts = d.experts;
   p.k_blocks = static_cast<int32_t>((d.k + kBK - 1) / kBK);
+  // (K blocks of all shared tiles are counted in 32 bits)
+  p.partial = p.k_blocks < (1 << 20) ? reinterpret_cast<float*>(d.partial) : nullptr;
+  p.counters = reinterpret_cast<uint32_t*>(d.counters);
+  p.partial_tokens = partial_tokens(d.slots);
+  p.experts = d.experts;
   p.n = static_cast<int32_t>(d.n);
   p.f_tiles = static_cast<int32_t>(f_tiles);
   p.bf16 = bf16 ? 1 : 0;
@@ -873,8 +961,10 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   p.budget_ns = kWaitBudgetNs;
   int sms = 0;
   TCCL_CHECK_CUDA(attrs_once(&sms));
-  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
-  TCCL_CHECK_CUDA(launch_pairs(gemm_kernel(d.epilogue, gather), p, pairs,
+  // (a shared tile is cut into runs of kMinBlocks K blocks at least)
+  const int64_t runs = p.partial == nullptr ? tiles : tiles * ((p.k_blocks + kMinBlocks - 1) / kMinBlocks);
+  const int pairs = static_cast<int>(runs < sms / 2 ? runs : sms / 2);
+  TCCL_CHECK_CUDA(launch_pairs(gemm_kernel(d.epilogue), p, pairs,
                                kThreads, kGemmSmem,
                                reinterpret_cast<cudaStream_t>(stream)));
   return kOk;

@@ -20,8 +20,8 @@ are allocated on that stream; the caller orders it behind the work that produced
 from __future__ import annotations
 
 import ctypes as C
-from contextlib import contextmanager
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -32,13 +32,6 @@ from . import fused_gemm as _fg
 MAX_ROUTED_EXPERTS = 512
 MAX_EXPERTS = 1024
 MAX_TOP_K = 32
-
-# Up to this many slots the product gathers the tokens' rows itself (TMA, four rows per copy);
-# above, a copy kernel puts them in slot order first.  The TMA unit needs some 70 cycles for four
-# rows, which a tile of 64 tokens hides behind its weights and one of 256 does not: gated product
-# of 8192 tokens x top 2, 4096 x 28672: 8.4 ms gathered in the kernel, 2.5 ms behind the copy
-# (35 us).  With few slots the extra launch would cost more than it saves.
-GATHER_IN_KERNEL_SLOTS = 64
 
 _LOGIT_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _EPILOGUES = {"none": 0, "silu_gate": 1}
@@ -82,24 +75,46 @@ def _pitch(name: str, t) -> int:
 _HALF = (torch.float16, torch.bfloat16)
 
 
-@contextmanager
-def _on(stream, inputs):
+# The raw handle of a device's current stream, without the Python object around it (1.2 us).
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
+    else lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+class _On:
     """Current device and stream of a launch; yields the raw stream.  Inputs that are used on
-    another stream than the current one are reported to the caching allocator."""
-    dev = inputs[0].device
-    if dev.type != "cuda":
-        raise ValueError(f"the expert operators take CUDA tensors, got tensors on {dev}")
-    with torch.cuda.device(dev):
-        if stream is None:
-            yield torch.cuda.current_stream(dev).cuda_stream
-        else:
-            if stream.device != dev:
-                raise ValueError(f"stream is on {stream.device}, the tensors are on {dev}")
-            for t in inputs:
-                if t is not None:
-                    t.record_stream(stream)
-            with torch.cuda.stream(stream):
-                yield stream.cuda_stream
+    another stream than the current one are reported to the caching allocator.  (A class: as a
+    generator it took 4 us of a call's 20.)"""
+
+    __slots__ = ("stream", "inputs", "dev", "device_guard", "stream_guard")
+
+    def __init__(self, stream, inputs):
+        self.stream, self.inputs, self.dev = stream, inputs, inputs[0].device
+        if self.dev.type != "cuda":
+            raise ValueError(f"the expert operators take CUDA tensors, got tensors on {self.dev}")
+        if stream is not None and stream.device != self.dev:
+            raise ValueError(f"stream is on {stream.device}, the tensors are on {self.dev}")
+        self.device_guard = self.stream_guard = None
+
+    def __enter__(self) -> int:
+        index = self.dev.index
+        if torch.cuda.current_device() != index:
+            self.device_guard = torch.cuda.device(index)
+            self.device_guard.__enter__()
+        if self.stream is None:
+            return _raw_stream(index)
+        for t in self.inputs:
+            if t is not None:
+                t.record_stream(self.stream)
+        self.stream_guard = torch.cuda.stream(self.stream)
+        self.stream_guard.__enter__()
+        return self.stream.cuda_stream
+
+    def __exit__(self, *exc):
+        if self.stream_guard is not None:
+            self.stream_guard.__exit__(*exc)
+        if self.device_guard is not None:
+            self.device_guard.__exit__(*exc)
+        return False
 
 
 def _ptr(t) -> int:
@@ -132,6 +147,8 @@ def check_expert_status(device=None) -> None:
     t = _STATUS.get(torch.cuda.current_device() if dev.index is None else dev.index)
     if t is not None:
         torch.cuda.synchronize(t.device)
+        if int(t[0]) != 0:
+            _COUNTERS.clear()             # (an abandoned call may have left some above zero)
         _fg.raise_on_status(t)
 
 
@@ -185,7 +202,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
         if mask.shape[0] != tokens:
             raise ValueError(f"mask has {mask.shape[0]} entries for {tokens} tokens")
     ld = _pitch("logits", logits)
-    with _on(stream, (logits, bias, mask)) as raw:
+    with _On(stream, (logits, bias, mask)) as raw:
         weights = torch.empty((tokens, top_k), dtype=torch.float32, device=logits.device)
         ids = torch.empty((tokens, top_k), dtype=torch.int32, device=logits.device)
         _launch("tccl_expert_route", logits.data_ptr(), ld, _ptr(bias), _ptr(mask),
@@ -211,7 +228,7 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids
         raise ValueError(f"ids {tuple(ids.shape)} and grad_weights {tuple(grad_weights.shape)} "
                          f"must both be {(tokens, top_k)}")
     ld = _pitch("logits", logits)
-    with _on(stream, (logits, ids, grad_weights)) as raw:
+    with _On(stream, (logits, ids, grad_weights)) as raw:
         grad = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
         _launch("tccl_expert_route_backward", grad_weights.data_ptr(), logits.data_ptr(), ld,
                 ids.data_ptr(), grad.data_ptr(), tokens, experts, top_k,
@@ -262,6 +279,13 @@ class ExpertSlots:
         return self.token_of_slot.shape[0]
 
 
+@lru_cache(maxsize=4096)
+def _slots_scratch(entries: int, experts: int) -> int:
+    need = C.c_int64()
+    _native.call("tccl_expert_slots_workspace", entries, experts, C.byref(need))
+    return need.value
+
+
 def expert_slots(ids: torch.Tensor, num_experts: int, *, first_expert: int = 0,
                  stream: Optional[torch.cuda.Stream] = None) -> ExpertSlots:
     """Slot map of ``ids`` (int32 ``[tokens, top_k]``) for the experts
@@ -277,16 +301,19 @@ def expert_slots(ids: torch.Tensor, num_experts: int, *, first_expert: int = 0,
     if top_k < 1 or tokens * top_k >= 1 << 31:
         raise ValueError(f"ids have an unsupported shape {tuple(ids.shape)}")
     dev = ids.device
-    with _on(stream, (ids,)) as raw:
-        offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-        token_of_slot = torch.empty(tokens * top_k, dtype=torch.int32, device=dev)
-        slot_of = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
-        need = C.c_int64()
-        _native.call("tccl_expert_slots_workspace", tokens * top_k, num_experts, C.byref(need))
-        scratch = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+    with _On(stream, (ids,)) as raw:
+        n = tokens * top_k
+        need = _slots_scratch(n, num_experts)
+        # one allocation for the three parts
+        slot_of, token_of_slot, offsets = torch.empty(
+            2 * n + num_experts + 1, dtype=torch.int32, device=dev).split((n, n, num_experts + 1))
+        slot_of = slot_of.view(tokens, top_k)
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _launch("tccl_expert_slots", ids.data_ptr(), tokens, top_k, num_experts, first_expert,
                 offsets.data_ptr(), token_of_slot.data_ptr(), slot_of.data_ptr(), _ptr(scratch), raw)
-    return ExpertSlots(offsets, token_of_slot, slot_of)
+    slots = object.__new__(ExpertSlots)           # (its parts need no second check)
+    slots.__dict__.update(offsets=offsets, token_of_slot=token_of_slot, slot_of=slot_of)
+    return slots
 
 
 # ----------------------------------------------------------------- grouped products
@@ -339,15 +366,37 @@ def _gather(X, slots, raw):
     return xs
 
 
-def _product(X, W, slots, out, rows, b_is_nk, epi, dh, raw):
+@lru_cache(maxsize=4096)
+def _scratch_sizes(device: int, slots: int, k: int) -> tuple:
+    a, b = C.c_int64(), C.c_int64()
+    _native.call("tccl_expert_gemm_scratch", slots, k, C.byref(a), C.byref(b))
+    return a.value, b.value
+
+
+_COUNTERS: dict = {}
+
+
+def _counters(dev, raw, nbytes):
+    """Zeroed arrival counters of a product.  Calls on one stream follow one another and leave
+    the counters at zero, so a stream's are kept; a captured call gets its own, because its graph
+    may be replayed beside anything else."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+    key = (dev.index, raw)
+    t = _COUNTERS.get(key)
+    if t is None:
+        t = _COUNTERS[key] = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+    return t
+
+
+def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
     """One launch of the grouped product; every argument is checked already."""
     E = W.shape[0]
     N, K = (W.shape[1], W.shape[2]) if b_is_nk else (W.shape[2], W.shape[1])
     d = _native.ExpertGemm()
     d.dtype, d.epilogue, d.experts, d.w_nk = _fg.dtype_code(X.dtype), epi, E, 1 if b_is_nk else 0
-    d.k, d.n, d.slots, d.x_rows = K, N, slots.capacity, X.shape[0]
+    d.k, d.n, d.slots = K, N, slots.capacity
     d.offsets = slots.offsets.data_ptr()
-    d.token_of_slot = slots.token_of_slot.data_ptr() if rows == "tokens" else 0
     d.x, d.w, d.out, d.dh = X.data_ptr(), W.data_ptr(), out.data_ptr(), _ptr(dh)
     d.ldx, d.ldw, d.ldo = _aligned("X", X), _aligned("W", W), _aligned("out", out)
     d.w_expert = W.stride(0) if E > 1 else W.shape[1] * d.ldw
@@ -355,6 +404,12 @@ def _product(X, W, slots, out, rows, b_is_nk, epi, dh, raw):
         raise ValueError("W's experts overlap or are not 16-byte aligned")
     d.ld_dh = 0 if dh is None else _aligned("grad_out", dh)
     d.status = _status_ptr(X.device)
+    partial_bytes, counter_bytes = _scratch_sizes(X.device.index, d.slots, K)
+    partial = None
+    if partial_bytes:
+        partial = torch.empty(partial_bytes, dtype=torch.uint8, device=X.device)
+        counters = _counters(X.device, raw, counter_bytes)
+        d.partial, d.counters = partial.data_ptr(), counters.data_ptr()
     _launch("tccl_expert_gemm", C.byref(d), raw)
 
 
@@ -375,12 +430,14 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
     shape = (slots.capacity, N // 2 if epi else N)
     if out is not None:
         _check_rows("out", out, shape, X)
-    with _on(stream, (X, W, slots.offsets, slots.token_of_slot, out)) as raw:
+    with _On(stream, (X, W, slots.offsets, slots.token_of_slot, out)) as raw:
         if out is None:
             out = torch.empty(shape, dtype=X.dtype, device=X.device)
-        if rows == "tokens" and slots.capacity > GATHER_IN_KERNEL_SLOTS:
-            X, rows = _gather(X, slots, raw), "slots"
-        _product(X, W, slots, out, rows, b_is_nk, epi, None, raw)
+        # Tokens' rows are put in slot order by a copy kernel first.  (The product gathering them
+        # itself, with the TMA unit's four rows per copy or through the threads, measured slower at
+        # every size: 209 against 200 us for 8 tokens, 8.1 against 2.5 ms for 8192.)
+        xs = _gather(X, slots, raw) if rows == "tokens" else X
+        _product(xs, W, slots, out, b_is_nk, epi, None, raw)
     return out
 
 
@@ -398,7 +455,7 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
     E, K, N, epi = _check_product(X, W, slots, rows, b_is_nk, epilogue)
     _check_rows("grad_out", grad_out, (slots.capacity, N // 2 if epi else N), X)
     S = slots.capacity
-    with _on(stream, (X, W, grad_out, slots.offsets, slots.token_of_slot, slots.slot_of)) as raw:
+    with _On(stream, (X, W, grad_out, slots.offsets, slots.token_of_slot, slots.slot_of)) as raw:
         # (once in slot order for both products that read X)
         xs = _gather(X, slots, raw) if rows == "tokens" else X
         dy = grad_out
@@ -406,9 +463,9 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
             # gate and up again, their gradients straight from the accumulators (one rounding
             # to 16 bits: the operand type of the two products that follow)
             dy = torch.empty((S, N), dtype=X.dtype, device=X.device)
-            _product(xs, W, slots, dy, "slots", b_is_nk, _EPI_SILU_GATE_GRAD, grad_out, raw)
+            _product(xs, W, slots, dy, b_is_nk, _EPI_SILU_GATE_GRAD, grad_out, raw)
         grad_rows = torch.empty((S, K), dtype=X.dtype, device=X.device)
-        _product(dy, W, slots, grad_rows, "slots", not b_is_nk, 0, None, raw)
+        _product(dy, W, slots, grad_rows, not b_is_nk, 0, None, raw)
         grad_X = grad_rows
         if rows == "tokens":
             grad_X = torch.empty((slots.tokens, K), dtype=X.dtype, device=X.device)
@@ -466,7 +523,7 @@ def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.
         _check_rows("add", add, shape, H)
     if out is not None:
         _check_rows("out", out, shape, H)
-    with _on(stream, (H, weights, add, slots.slot_of, out)) as raw:
+    with _On(stream, (H, weights, add, slots.slot_of, out)) as raw:
         if out is None:
             out = torch.empty(shape, dtype=H.dtype, device=H.device)
         _combine(H, slots, weights, add, out, raw)
@@ -483,7 +540,7 @@ def expert_combine_backward(grad_out: torch.Tensor, H: torch.Tensor, slots: Expe
         raise ValueError("weights must be a 2-D tensor")
     _check_combine(H, slots, weights)
     _check_rows("grad_out", grad_out, (slots.tokens, H.shape[1]), H)
-    with _on(stream, (H, weights, grad_out, slots.slot_of)) as raw:
+    with _On(stream, (H, weights, grad_out, slots.slot_of)) as raw:
         grad_H = torch.empty(H.shape, dtype=H.dtype, device=H.device)
         grad_weights = torch.empty(weights.shape, dtype=torch.float32, device=H.device)
         _launch("tccl_expert_combine_backward", grad_out.data_ptr(), _aligned("grad_out", grad_out),
