@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include "../api.h"
+#include "../device/symm_ptr.cuh"
 #include "../device/tile_compute.cuh"
 #include "../runtime/errors.h"
 
@@ -33,67 +34,122 @@ struct CombineParams {
   int32_t top_k, vecs, bf16;   // vecs: 16-byte vectors per row
 };
 
+// Rows of H are fetched kBatch at a time: the slots of a token first, then that many rows'
+// vectors, all in flight together.
+constexpr int kBatch = 8;
+
 __global__ void __launch_bounds__(kThreads) expert_combine_kernel(const CombineParams p) {
   const int64_t t = blockIdx.x;
   const int v = blockIdx.y * kThreads + threadIdx.x;
   if (v >= p.vecs) return;
+  const bool bf16 = p.bf16 != 0;
   float acc[8] = {};
-  if (p.add != nullptr) tile_accumulate_16x8(p.bf16 != 0, acc, p.add[t * p.add_ld + v]);
-  for (int j = 0; j < p.top_k; ++j) {
-    const int32_t s = p.slot_of[t * p.top_k + j];
-    if (s < 0 || s >= p.slots) continue;
-    const float w = p.weights != nullptr ? p.weights[t * p.top_k + j] : 1.f;
-    float x[8] = {};
-    tile_accumulate_16x8(p.bf16 != 0, x, p.h[s * p.h_ld + v]);
+  uint4 base = make_uint4(0, 0, 0, 0);
+  if (p.add != nullptr) base = p.add[t * p.add_ld + v];
+  for (int j0 = 0; j0 < p.top_k; j0 += kBatch) {
+    int32_t s[kBatch];
+    float w[kBatch];
+    uint4 x[kBatch];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, x[i], acc[i]);
+    for (int j = 0; j < kBatch; ++j) {
+      s[j] = j0 + j < p.top_k ? p.slot_of[t * p.top_k + j0 + j] : -1;
+      if (s[j] >= p.slots) s[j] = -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (s[j] >= 0) {
+        x[j] = ld_stream_v4(p.h + s[j] * p.h_ld + v);
+        w[j] = p.weights != nullptr ? p.weights[t * p.top_k + j0 + j] : 1.f;
+      }
+    if (j0 == 0) tile_accumulate_16x8(bf16, acc, base);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (s[j] >= 0) {
+        float f[8] = {};
+        tile_accumulate_16x8(bf16, f, x[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+      }
   }
-  p.out[t * p.out_ld + v] = tile_cast_f32x8(p.bf16 != 0, acc);
+  p.out[t * p.out_ld + v] = tile_cast_f32x8(bf16, acc);
 }
 
+// One CTA per token.  A batch of choices at a time: dy stays in registers, every row of H is
+// read once, and the dot products of the batch meet in one reduction.
 __global__ void __launch_bounds__(kThreads) expert_combine_backward_kernel(const CombineParams p) {
-  __shared__ float part[kThreads / 32];
+  __shared__ float part[kThreads / 32][kBatch];
   const int64_t t = blockIdx.x;
-  for (int j = 0; j < p.top_k; ++j) {
-    const int32_t s = p.slot_of[t * p.top_k + j];
-    float dot = 0.f;
-    if (s >= 0 && s < p.slots) {
-      const float w = p.weights[t * p.top_k + j];
-      for (int v = threadIdx.x; v < p.vecs; v += kThreads) {
-        float g[8] = {}, x[8] = {};
-        tile_accumulate_16x8(p.bf16 != 0, g, p.dy[t * p.dy_ld + v]);
-        tile_accumulate_16x8(p.bf16 != 0, x, p.h[s * p.h_ld + v]);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool bf16 = p.bf16 != 0;
+  for (int j0 = 0; j0 < p.top_k; j0 += kBatch) {
+    int32_t s[kBatch];
+    float w[kBatch], dot[kBatch];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dot = fmaf(g[i], x[i], dot);
-          g[i] *= w;
+    for (int j = 0; j < kBatch; ++j) {
+      s[j] = j0 + j < p.top_k ? p.slot_of[t * p.top_k + j0 + j] : -1;
+      if (s[j] >= p.slots) s[j] = -1;
+      w[j] = s[j] >= 0 ? p.weights[t * p.top_k + j0 + j] : 0.f;
+      dot[j] = 0.f;
+    }
+    for (int v = threadIdx.x; v < p.vecs; v += kThreads) {
+      uint4 x[kBatch];
+      const uint4 dy = p.dy[t * p.dy_ld + v];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (s[j] >= 0) x[j] = ld_stream_v4(p.h + s[j] * p.h_ld + v);
+      float g[8] = {};
+      tile_accumulate_16x8(bf16, g, dy);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (s[j] >= 0) {
+          float f[8] = {};
+          tile_accumulate_16x8(bf16, f, x[j]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dot[j] = fmaf(g[i], f[i], dot[j]);
+            f[i] = g[i] * w[j];
+          }
+          p.dh[s[j] * p.dh_ld + v] = tile_cast_f32x8(bf16, f);
         }
-        p.dh[s * p.dh_ld + v] = tile_cast_f32x8(p.bf16 != 0, g);
-      }
     }
+    if (j0 > 0) __syncthreads();                 // `part` of the previous batch has been read
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      float sum = 0.f;
-      for (int w = 0; w < kThreads / 32; ++w) sum += part[w];
-      p.dw[t * p.top_k + j] = sum;
+    for (int j = 0; j < kBatch; ++j) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+      if (lane == 0) part[warp][j] = dot[j];
     }
     __syncthreads();
+    if (threadIdx.x < kBatch && j0 + threadIdx.x < p.top_k) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) sum += part[i][threadIdx.x];
+      p.dw[t * p.top_k + j0 + threadIdx.x] = sum;
+    }
   }
 }
 
 // out[s] = x[token of slot s]; zeros for a token that does not exist, nothing behind the last
-// slot (token -1).
+// slot (token -1).  A CTA takes kGatherRows rows, so that as many vectors per thread are in
+// flight.
+constexpr int kGatherRows = 4;
+
 __global__ void __launch_bounds__(kThreads) expert_gather_kernel(
     const uint4* x, int64_t x_ld, int64_t x_rows, const int32_t* token_of_slot, uint4* out,
-    int64_t out_ld, int32_t vecs) {
-  const int64_t s = blockIdx.x;
-  const int32_t t = token_of_slot[s];
-  if (t < 0) return;
+    int64_t out_ld, int64_t slots, int32_t vecs) {
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kGatherRows;
   const int v = blockIdx.y * kThreads + threadIdx.x;
-  if (v < vecs) out[s * out_ld + v] = t < x_rows ? x[t * x_ld + v] : make_uint4(0, 0, 0, 0);
+  if (v >= vecs) return;
+  int32_t t[kGatherRows];
+  uint4 r[kGatherRows];
+#pragma unroll
+  for (int i = 0; i < kGatherRows; ++i) t[i] = s0 + i < slots ? token_of_slot[s0 + i] : -1;
+#pragma unroll
+  for (int i = 0; i < kGatherRows; ++i)
+    r[i] = t[i] >= 0 && t[i] < x_rows ? x[t[i] * x_ld + v] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < kGatherRows; ++i)
+    if (t[i] >= 0) out[(s0 + i) * out_ld + v] = r[i];
 }
 
 int check(const CombineParams& p) {
@@ -195,10 +251,11 @@ extern "C" int tccl_expert_gather(uint64_t x, int64_t x_ld, int64_t x_rows, uint
   TCCL_CHECK_ARG(vecs <= 65535 * kThreads, "rows are too long");
   if (slots == 0) return kOk;
   TCCL_CHECK_ARG(x != 0 && token_of_slot != 0 && out != 0, "null argument");
-  const dim3 grid(static_cast<unsigned>(slots), (vecs + kThreads - 1) / kThreads);
+  const dim3 grid(static_cast<unsigned>((slots + kGatherRows - 1) / kGatherRows),
+                  (vecs + kThreads - 1) / kThreads);
   expert_gather_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       reinterpret_cast<const uint4*>(x), x_ld / 8, x_rows,
-      reinterpret_cast<const int32_t*>(token_of_slot), reinterpret_cast<uint4*>(out), out_ld / 8, vecs);
+      reinterpret_cast<const int32_t*>(token_of_slot), reinterpret_cast<uint4*>(out), out_ld / 8, slots, vecs);
   TCCL_CHECK_CUDA(cudaGetLastError());
   return kOk;
 }

@@ -5,13 +5,19 @@
 //   p = softmax(l)  or  p = 1 / (1 + e^-l);   key = p + bias;   ids = the k largest keys
 //   w_j = scale * p[id_j]  or, renormalised,  scale * p[id_j] / sum_i p[id_i]
 //
-// One warp per token; lane i holds experts i, i + 32, ...
+// A warp takes a token at a time.  The choice has to be the one that exact arithmetic makes, ties
+// to the lower index.  It is made on approximate 32-bit keys first: every lane sorts the few it
+// holds, then k + 1 rounds take the largest head of the 32 lists.  Where two neighbours of that
+// order (or the last group kept and the first dropped) are closer than the keys' error, the row
+// is decided again on 64-bit keys (about one row in a hundred with 256 sigmoid scores).  16-bit
+// logits that compete without a bias need no scores: their own order is exact.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
 #include "../api.h"
+#include "../device/tile_compute.cuh"
 #include "../runtime/errors.h"
 
 namespace tileccl {
@@ -33,6 +39,8 @@ struct RouteParams {
   void* grad_logits;          // backward only, [tokens, experts] contiguous
   int64_t tokens;
   int32_t experts, top_k, dtype, sigmoid, groups, top_groups, group_max, renormalize;
+  int32_t fast;               // the groups share the lanes evenly
+  int32_t wide, wide_out;     // a lane's logits (gradients) can be moved in whole pieces
   float scale;
 };
 
@@ -71,88 +79,63 @@ __device__ __forceinline__ float sigmoid_scaled(float l, float m) {
   return l > 0.f ? 1.f / (1.f + expf(-l)) : expf(l - s) / (1.f + expf(l));
 }
 
-// Keys are compared as unsigned integers of the same order.  0 = the expert is not available
-// (logit or bias of -inf, or outside the chosen groups); 1 = the key is not a number: it ranks
-// behind every number, so ids stay distinct and in range.
-__device__ __forceinline__ uint64_t order_key(double x) {
+// Numbers as unsigned integers of the same order.
+__device__ __forceinline__ uint32_t order32(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);     // (-0 becomes +0)
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float value32(uint32_t u) {
+  return __uint_as_float(u ^ ((u >> 31) ? 0x80000000u : 0xffffffffu));
+}
+// 64-bit keys: 0 = the expert is not available (logit or bias of -inf, or outside the chosen
+// groups); 1 = the key is not a number: it ranks behind every number, so ids stay distinct and
+// in range.
+__device__ __forceinline__ uint64_t order64(double x) {
   if (x != x) return 1;
   if (x == -CUDART_INF) return 0;
   const uint64_t b = static_cast<uint64_t>(__double_as_longlong(x == 0.0 ? 0.0 : x));
   return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
+__device__ __forceinline__ double value64(uint64_t u) {
+  return __longlong_as_double(static_cast<long long>((u >> 63) ? u & 0x7fffffffffffffffull : ~u));
+}
 
-template <int EPL>
-__global__ void __launch_bounds__(kWarpsPerCta * 32)
-expert_route_kernel(const RouteParams p) {
-  extern __shared__ double smem_keys[];   // [warps][experts], only used with groups
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + warp;
-  if (t >= p.tokens) return;
-  float* const out_w = p.weights + t * p.top_k;
-  int32_t* const out_i = p.ids + t * p.top_k;
-  if (p.mask != nullptr && p.mask[t] == 0) {
-    if (lane < p.top_k) { out_w[lane] = 0.f; out_i[lane] = -1; }
-    return;
-  }
-  float l[EPL];
-  bool nan_row = false;
-  float m = -CUDART_INF_F;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    l[i] = e < p.experts ? load_logit(p.logits, t * p.ld + e, p.dtype) : -CUDART_INF_F;
-    nan_row = nan_row || l[i] != l[i];
-    m = fmaxf(m, l[i]);
-  }
-  nan_row = __any_sync(kAll, nan_row);
-  m = warp_max(m);
-
-  // The choice is made on 64-bit keys: scores of two experts may differ by less than a 32-bit
-  // exponential can tell.  Without a bias the score grows with the logit, which is then the key.
+// The row's choice on 64-bit keys (`keys`: one per expert in shared memory); lane j returns the
+// j-th id.  `top` is the row's largest logit.
+__device__ __noinline__ int choose_exactly(const RouteParams& p, int64_t t, float top, uint64_t* keys) {
+  const int lane = threadIdx.x & 31;
   const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_max != 0);
-  double key[EPL];
-  double total = 0.0;
-  if (!by_logit) {
+  double total = 1.0;
+  if (!by_logit && !p.sigmoid) {
     double part = 0.0;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      key[i] = p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l[i])))
-                         : exp(static_cast<double>(l[i]) - static_cast<double>(m));
-      part += key[i];
+    for (int e = lane; e < p.experts; e += 32) {
+      const float l = load_logit(p.logits, t * p.ld + e, p.dtype);
+      if (l != -CUDART_INF_F) part += exp(static_cast<double>(l) - static_cast<double>(top));
     }
     total = warp_sum(part);
   }
-  uint64_t rank[EPL];
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    double k = by_logit ? static_cast<double>(l[i]) : p.sigmoid ? key[i] : key[i] / total;
-    if (p.bias != nullptr && e < p.experts) k += static_cast<double>(p.bias[e]);
-    key[i] = k;
-    rank[i] = (e >= p.experts || l[i] == -CUDART_INF_F) ? 0 : order_key(k);
+  for (int e = lane; e < p.experts; e += 32) {
+    const float l = load_logit(p.logits, t * p.ld + e, p.dtype);
+    double k = l;
+    if (!by_logit)
+      k = p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l)))
+                    : exp(static_cast<double>(l) - static_cast<double>(top)) / total;
+    if (p.bias != nullptr) k += static_cast<double>(p.bias[e]);
+    keys[e] = l == -CUDART_INF_F ? 0 : order64(k);
   }
+  __syncwarp();
   if (p.groups > 1) {
-    double* const mine = smem_keys + static_cast<int64_t>(warp) * p.experts;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 32 * i;
-      if (e < p.experts) mine[e] = rank[i] == 0 ? -CUDART_INF : key[i];
-    }
-    __syncwarp();
     const int per = p.experts / p.groups;
     // lane g: score of group g = its largest key, or the sum of its two largest available keys
     uint64_t score = 0;
     if (lane < p.groups) {
-      double a = -CUDART_INF, b = -CUDART_INF;
-      bool bad = false;
+      uint64_t a = 0, b = 0;
       for (int i = 0; i < per; ++i) {
-        const double x = mine[lane * per + i];
-        if (x != x) bad = true;
-        else if (x > a) { b = a; a = x; }
+        const uint64_t x = keys[lane * per + i];
+        if (x > a) { b = a; a = x; }
         else if (x > b) b = x;
       }
-      const double s = p.group_max || b == -CUDART_INF ? a : a + b;
-      score = a == -CUDART_INF ? (bad ? 1 : 0) : order_key(s);
+      score = p.group_max || b <= 1 ? a : order64(value64(a) + value64(b));
     }
     int ahead = 0;
     for (int g = 0; g < p.groups; ++g) {
@@ -160,54 +143,246 @@ expert_route_kernel(const RouteParams p) {
       ahead += (other > score || (other == score && g < lane)) ? 1 : 0;
     }
     const uint32_t keep = __ballot_sync(kAll, lane < p.groups && ahead < p.top_groups);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 32 * i;
-      if (e < p.experts && ((keep >> (e / per)) & 1u) == 0) rank[i] = 0;
-    }
+    for (int e = lane; e < p.experts; e += 32)
+      if (((keep >> (e / per)) & 1u) == 0) keys[e] = 0;
+    __syncwarp();
   }
-
-  // k rounds: the warp's best remaining expert, the lowest index among equals
-  int my_id = -1;
-  float my_l = -CUDART_INF_F;
+  int mine = -1;
   for (int j = 0; j < p.top_k; ++j) {
     uint64_t best = 0;
-    int at = -1;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (rank[i] > best) { best = rank[i]; at = i; }
-    const uint64_t top = warp_max(best);
-    if (top == 0) break;
-    const uint32_t cand = best == top ? static_cast<uint32_t>(lane + 32 * at) : kAll;
-    const uint32_t id = __reduce_min_sync(kAll, cand);
-    float chosen = 0.f;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (lane + 32 * i == static_cast<int>(id)) { rank[i] = 0; chosen = l[i]; }
-    chosen = __shfl_sync(kAll, chosen, id & 31);
-    if (lane == j) { my_id = static_cast<int>(id); my_l = chosen; }
+    int at = 0;
+    for (int e = lane; e < p.experts; e += 32)
+      if (keys[e] > best) { best = keys[e]; at = e; }
+    const uint64_t round = warp_max(best);
+    if (round == 0) break;
+    const uint32_t id = __reduce_min_sync(kAll, best == round ? static_cast<uint32_t>(at) : kAll);
+    if (static_cast<int>(id & 31u) == lane) keys[id] = 0;
+    __syncwarp();
+    if (lane == j) mine = static_cast<int>(id);
   }
+  __syncwarp();
+  return mine;
+}
 
-  // weights: lane j holds the j-th choice
-  float w = 0.f;
-  if (p.renormalize) {
-    const float top = warp_max(my_l);
-    const float s = my_id < 0 ? 0.f : p.sigmoid ? sigmoid_scaled(my_l, top) : expf(my_l - top);
-    const float sum = warp_sum(s);
-    w = s / sum;
-  } else if (p.sigmoid) {
-    w = sigmoid_f(my_l);
-  } else {
-    float part = 0.f;
+// Lane `lane` holds the logits first .. first + n - 1 (n <= EPL) of its row, -inf behind them.
+template <int EPL>
+__device__ __forceinline__ void load_logits(const RouteParams& p, int64_t at, int n, float (&l)[EPL]) {
+  if (p.wide && n == EPL) {
+    if (p.dtype == kF32) {
+      if constexpr (EPL >= 4) {
+        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.logits) + at);
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) part += lane + 32 * i < p.experts ? expf(l[i] - m) : 0.f;
-    const float sum = warp_sum(part);
-    w = expf(my_l - m) / sum;
+        for (int i = 0; i < EPL / 4; ++i) {
+          const float4 v = src[i];
+          l[4 * i] = v.x; l[4 * i + 1] = v.y; l[4 * i + 2] = v.z; l[4 * i + 3] = v.w;
+        }
+        return;
+      }
+    } else if constexpr (EPL >= 2) {
+      alignas(16) uint32_t w[EPL / 2];
+      const char* src = static_cast<const char*>(p.logits) + 2 * at;
+      if constexpr (EPL == 2) w[0] = *reinterpret_cast<const uint32_t*>(src);
+      else if constexpr (EPL == 4) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
+      else {
+#pragma unroll
+        for (int i = 0; i < EPL / 8; ++i)
+          reinterpret_cast<uint4*>(w)[i] = reinterpret_cast<const uint4*>(src)[i];
+      }
+#pragma unroll
+      for (int i = 0; i < EPL / 2; ++i) {
+        const float2 v = unpack_16x2(p.dtype == kBF16, w[i]);
+        l[2 * i] = v.x; l[2 * i + 1] = v.y;
+      }
+      return;
+    }
   }
-  w *= p.scale;
-  if (nan_row || (!p.sigmoid && m == CUDART_INF_F)) w = CUDART_NAN_F;   // as the formula has it
-  if (my_id < 0) w = 0.f;
-  if (lane < p.top_k) { out_w[lane] = w; out_i[lane] = my_id; }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) l[i] = i < n ? load_logit(p.logits, at + i, p.dtype) : -CUDART_INF_F;
+}
+
+// Descending order of a lane's list (odd-even merge sort).
+template <int N>
+__device__ __forceinline__ void sort_descending(uint32_t (&v)[N]) {
+#pragma unroll
+  for (int q = 1; q < N; q <<= 1)
+#pragma unroll
+    for (int k = q; k >= 1; k >>= 1)
+#pragma unroll
+      for (int j = k % q; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * q) == (i + j + k) / (2 * q)) {
+            const uint32_t hi = max(v[i + j], v[i + j + k]), lo = min(v[i + j], v[i + j + k]);
+            v[i + j] = hi;
+            v[i + j + k] = lo;
+          }
+}
+
+// EPL: experts per lane (a power of two).  The lanes are shared out evenly among the groups;
+// within a group lane i holds the experts i * EPL, i * EPL + 1, ...
+template <int EPL>
+__global__ void __launch_bounds__(kWarpsPerCta * 32)
+expert_route_kernel(const __grid_constant__ RouteParams p) {
+  extern __shared__ uint64_t smem_keys[];   // [warps][experts]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* const keys64 = smem_keys + static_cast<int64_t>(warp) * p.experts;
+  const int lanes = p.fast ? 32 / p.groups : 32;                  // per group
+  const int per = p.fast ? p.experts / p.groups : p.experts;
+  const int group = lane / lanes;
+  const int in_group = (lane - group * lanes) * EPL;
+  const int first = group * per + in_group;
+  const int n = min(max(per - in_group, 0), EPL);
+  const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_max != 0);
+  const bool exact = by_logit && p.dtype != kF32;
+  // Error of a key: the bits that hold the place in the list (2^-23 EPL of the key, twice), and
+  // that of its score: sigmoid 1/4 (2 + 1.2 |l|) 2^-23 and a sum and a division, below 2^-20;
+  // softmax, whose sum carries the errors of all terms, below 2^-18.
+  const float key_error = by_logit ? 0.f : 4.f * EPL * 0x1p-23f;
+  const float score_error = by_logit ? 0.f : p.sigmoid ? 0x1p-19f : 0x1p-17f;
+  float bias[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) bias[i] = p.bias != nullptr && i < n ? p.bias[first + i] : 0.f;
+
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + warp; t < p.tokens;
+       t += static_cast<int64_t>(gridDim.x) * kWarpsPerCta) {
+    float* const out_w = p.weights + t * p.top_k;
+    int32_t* const out_i = p.ids + t * p.top_k;
+    if (p.mask != nullptr && p.mask[t] == 0) {
+      if (lane < p.top_k) { out_w[lane] = 0.f; out_i[lane] = -1; }
+      continue;
+    }
+    float l[EPL];
+    load_logits<EPL>(p, t * p.ld + first, n, l);
+    float top = l[0];
+    if (!p.sigmoid || !p.fast) {
+#pragma unroll
+      for (int i = 1; i < EPL; ++i) top = fmaxf(top, l[i]);
+      top = value32(__reduce_max_sync(kAll, top != top ? 0u : order32(top)));
+    }
+
+    // approximate keys, packed with the place in the lane's list
+    uint32_t key[EPL];
+    bool odd = !p.fast;                    // something the approximate way does not cover
+    float inv = 1.f;
+    float x[EPL];
+    if (by_logit) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) x[i] = l[i];
+    } else if (p.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) x[i] = __fdividef(1.f, 1.f + __expf(-l[i]));
+    } else {
+      float part = 0.f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) part += x[i] = __expf(l[i] - top);
+      inv = __fdividef(1.f, warp_sum(part));
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const float k = by_logit ? x[i] : fmaf(x[i], inv, bias[i]);
+      const bool there = i < n && l[i] != -CUDART_INF_F && bias[i] != -CUDART_INF_F;
+      odd = odd || (there && !(fabsf(k) < CUDART_INF_F));
+      key[i] = there ? (order32(k) & ~(EPL - 1u)) | (EPL - 1u - i) : 0u;
+    }
+    bool close = false;
+    sort_descending(key);
+    if (p.groups > 1 && p.fast) {
+      uint32_t a = key[0], b = EPL > 1 ? key[EPL > 1 ? 1 : 0] : 0u;
+      for (int o = 1; o < lanes; o <<= 1) {
+        const uint32_t c = __shfl_xor_sync(kAll, a, o), d = __shfl_xor_sync(kAll, b, o);
+        b = max(min(a, c), max(b, d));
+        a = max(a, c);
+      }
+      const float va = value32(a & ~(EPL - 1u)), vb = value32(b & ~(EPL - 1u));
+      const uint32_t score = a == 0 ? 0u : order32(p.group_max || b == 0 ? va : va + vb);
+      int ahead = 0;
+      for (int g = 0; g < p.groups; ++g) {
+        const uint32_t other = __shfl_sync(kAll, score, g * lanes);
+        ahead += (other > score || (other == score && g < group)) ? 1 : 0;
+      }
+      const bool keep = ahead < p.top_groups;
+      const uint32_t worst = __reduce_min_sync(kAll, keep ? score : kAll);
+      const uint32_t next = __reduce_max_sync(kAll, keep ? 0u : score);
+      if (!exact && next != 0) {
+        const float w = value32(worst), v = value32(next);
+        const float size = fmaxf(fabsf(w), fabsf(v)) + (p.group_max ? 0.f : 2.f * fabsf(va) + 2.f * fabsf(vb));
+        close = !(w - v > size * key_error + 2.f * score_error);
+      }
+      if (!keep) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) key[i] = 0u;
+      }
+    }
+    // k rounds (and one to see who comes next): the largest head, the lowest lane among equals
+    int id = -1;
+    uint32_t mine = 0, after = 0;
+    const int rounds = p.top_k + (exact ? 0 : 1);
+    for (int j = 0; j < rounds; ++j) {
+      const uint32_t head = key[0] & ~(EPL - 1u);     // (places compare within a lane only)
+      const uint32_t best = __reduce_max_sync(kAll, head);
+      if (best == 0) break;
+      const int from = __ffs(__ballot_sync(kAll, head == best)) - 1;
+      if (j == p.top_k) { after = best; break; }
+      const int e = __shfl_sync(kAll, first + (EPL - 1) - static_cast<int>(key[0] & (EPL - 1u)), from);
+      if (lane == j) { id = e; mine = best; }
+      if (lane == from) {
+#pragma unroll
+        for (int i = 0; i + 1 < EPL; ++i) key[i] = key[i + 1];
+        key[EPL - 1] = 0u;
+      }
+    }
+    float my_l = id >= 0 ? load_logit(p.logits, t * p.ld + id, p.dtype) : -CUDART_INF_F;
+    if (!exact) {
+      uint32_t below = __shfl_down_sync(kAll, mine, 1);
+      if (lane == p.top_k - 1) below = after;
+      if (lane < p.top_k && below != 0) {
+        const float w = value32(mine), v = value32(below);
+        close = close || !(w - v > fmaxf(fabsf(w), fabsf(v)) * key_error + score_error);
+      }
+      // two of the chosen that agree in logit and bias are equal exactly: in place already
+      if (__any_sync(kAll, close)) {
+        const float next_l = __shfl_down_sync(kAll, my_l, 1);
+        const float my_b = p.bias != nullptr && id >= 0 ? p.bias[id] : 0.f;
+        const float next_b = __shfl_down_sync(kAll, my_b, 1);
+        if (lane < p.top_k - 1 && mine != 0 && p.groups == 1 && my_l == next_l && my_b == next_b)
+          close = false;
+      }
+    }
+    bool broken = false;                   // a row without numbers for weights
+    if (__any_sync(kAll, odd || close)) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) broken = broken || l[i] != l[i];
+      broken = __any_sync(kAll, broken);
+      if (p.sigmoid && p.fast) {
+#pragma unroll
+        for (int i = 1; i < EPL; ++i) top = fmaxf(top, l[i]);
+        top = warp_max(top);
+      }
+      if (!p.sigmoid && top == CUDART_INF_F) broken = true;     // as the formula has it
+      id = choose_exactly(p, t, top, keys64);
+      my_l = id >= 0 ? load_logit(p.logits, t * p.ld + id, p.dtype) : -CUDART_INF_F;
+    }
+
+    // weights: lane j holds the j-th choice
+    float w = 0.f;
+    if (p.renormalize) {
+      const float m = value32(__reduce_max_sync(kAll, my_l != my_l ? 0u : order32(my_l)));
+      const float sc = id < 0 ? 0.f : p.sigmoid ? sigmoid_scaled(my_l, m) : expf(my_l - m);
+      w = sc / warp_sum(sc);
+    } else if (p.sigmoid) {
+      w = sigmoid_f(my_l);
+    } else {
+      float part = 0.f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) part += i < n ? expf(l[i] - top) : 0.f;
+      const float sum = warp_sum(part);
+      w = expf(my_l - top) / sum;
+    }
+    w *= p.scale;
+    if (broken) w = CUDART_NAN_F;
+    if (id < 0) w = 0.f;
+    if (lane < p.top_k) { out_w[lane] = w; out_i[lane] = id; }
+  }
 }
 
 // dL/dl of a row from dL/dw of its k weights.  With n_j = w_j / scale and g_j = dL/dw_j:
@@ -221,37 +396,35 @@ expert_route_backward_kernel(const RouteParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + warp;
   if (t >= p.tokens) return;
+  const int first = lane * EPL, count = min(max(p.experts - first, 0), EPL);
+  const bool dense = !p.sigmoid && !p.renormalize;     // every logit of the row counts
   int id = -1;
   float g = 0.f;
   if (lane < p.top_k) {
     id = p.ids[t * p.top_k + lane];
-    if (id < 0 || id >= p.experts) id = -1;
-    else g = p.grad_weights[t * p.top_k + lane];
+    g = p.grad_weights[t * p.top_k + lane];
   }
-  const bool routed = __any_sync(kAll, id >= 0);
   float l[EPL];
-  float m = -CUDART_INF_F;
+  if (dense) load_logits<EPL>(p, t * p.ld + first, count, l);
+  if (id < 0 || id >= p.experts) { id = -1; g = 0.f; }
+  const bool routed = __any_sync(kAll, id >= 0);
+  const float my_l = id >= 0 ? load_logit(p.logits, t * p.ld + id, p.dtype) : -CUDART_INF_F;
+  float m = 0.f, sum = 0.f;
+  if (dense) {
+    m = l[0];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    l[i] = routed && e < p.experts ? load_logit(p.logits, t * p.ld + e, p.dtype) : -CUDART_INF_F;
-    m = fmaxf(m, l[i]);
-  }
-  m = warp_max(m);
-  float prob[EPL];
-  float sum = 0.f;
-  if (!p.sigmoid && !p.renormalize) {
+    for (int i = 1; i < EPL; ++i) m = fmaxf(m, l[i]);
+    m = value32(__reduce_max_sync(kAll, m != m ? 0u : order32(m)));
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      prob[i] = l[i] == -CUDART_INF_F ? 0.f : expf(l[i] - m);
-      sum += prob[i];
+      l[i] = l[i] == -CUDART_INF_F ? 0.f : expf(l[i] - m);
+      sum += l[i];
     }
     sum = warp_sum(sum);
   }
-  const float my_l = id >= 0 ? load_logit(p.logits, t * p.ld + id, p.dtype) : -CUDART_INF_F;
   float n = 0.f;
   if (p.renormalize) {
-    const float top = warp_max(my_l);
+    const float top = value32(__reduce_max_sync(kAll, my_l != my_l ? 0u : order32(my_l)));
     const float s = id < 0 || my_l == -CUDART_INF_F ? 0.f
                     : p.sigmoid ? sigmoid_scaled(my_l, top) : expf(my_l - top);
     const float all = warp_sum(s);
@@ -261,29 +434,45 @@ expert_route_backward_kernel(const RouteParams p) {
   }
   const float dot = p.sigmoid && !p.renormalize ? 0.f : warp_sum(id >= 0 ? g * n : 0.f);
   // lane j's share of dl at its expert; the dense softmax adds -p_i * dot everywhere
-  float mine = p.scale * n * (!p.sigmoid && !p.renormalize ? g : g - dot);
+  float mine = p.scale * n * (dense ? g : g - dot);
   if (p.sigmoid) mine *= sigmoid_f(-my_l);
   if (id < 0 || my_l == -CUDART_INF_F) mine = 0.f;
   float d[EPL];
+  const float all = -p.scale * dot / sum;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    d[i] = 0.f;
-    if (!p.sigmoid && !p.renormalize && routed && l[i] != -CUDART_INF_F)
-      d[i] = -p.scale * (prob[i] / sum) * dot;
-  }
+  for (int i = 0; i < EPL; ++i) d[i] = dense && routed && l[i] != 0.f ? all * l[i] : 0.f;
   for (int j = 0; j < p.top_k; ++j) {
     const int e = __shfl_sync(kAll, id, j);
     const float v = __shfl_sync(kAll, mine, j);
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
-      if (e == lane + 32 * i) d[i] += v;
+      if (e == first + i) d[i] += v;
+  }
+  const int64_t at = t * p.experts + first;
+  if (p.wide_out && count == EPL) {
+    if (p.dtype == kF32) {
+      if constexpr (EPL >= 4) {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.grad_logits) + at);
+#pragma unroll
+        for (int i = 0; i < EPL / 4; ++i)
+          dst[i] = make_float4(d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]);
+        return;
+      }
+    } else if constexpr (EPL >= 8) {
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(p.grad_logits) + 2 * at);
+#pragma unroll
+      for (int i = 0; i < EPL / 8; ++i) dst[i] = tile_cast_f32x8(p.dtype == kBF16, d + 8 * i);
+      return;
+    }
   }
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    if (e < p.experts) store_logit(p.grad_logits, t * p.experts + e, p.dtype, d[i]);
-  }
+  for (int i = 0; i < EPL; ++i)
+    if (i < count) store_logit(p.grad_logits, at + i, p.dtype, d[i]);
 }
+
+// CTAs of a forward launch: enough warps to fill the SMs, each with several rows, so that the
+// bias is loaded once.
+constexpr int64_t kMaxCtas = 148 * 8;
 
 template <int EPL>
 cudaError_t launch(const RouteParams& p, bool backward, cudaStream_t s) {
@@ -291,18 +480,29 @@ cudaError_t launch(const RouteParams& p, bool backward, cudaStream_t s) {
   if (backward) {
     expert_route_backward_kernel<EPL><<<static_cast<unsigned>(blocks), kWarpsPerCta * 32, 0, s>>>(p);
   } else {
-    const size_t smem = p.groups > 1 ? sizeof(double) * kWarpsPerCta * p.experts : 0;
-    expert_route_kernel<EPL><<<static_cast<unsigned>(blocks), kWarpsPerCta * 32, smem, s>>>(p);
+    const size_t smem = sizeof(uint64_t) * kWarpsPerCta * p.experts;
+    expert_route_kernel<EPL><<<static_cast<unsigned>(blocks < kMaxCtas ? blocks : kMaxCtas),
+                               kWarpsPerCta * 32, smem, s>>>(p);
   }
   return cudaGetLastError();
 }
 
-cudaError_t dispatch(const RouteParams& p, bool backward, cudaStream_t s) {
-  const int epl = (p.experts + 31) / 32;
-  if (epl <= 1) return launch<1>(p, backward, s);
-  if (epl <= 2) return launch<2>(p, backward, s);
-  if (epl <= 4) return launch<4>(p, backward, s);
-  if (epl <= 8) return launch<8>(p, backward, s);
+cudaError_t dispatch(RouteParams& p, bool backward, cudaStream_t s) {
+  const int lanes = p.fast ? 32 / p.groups : 32;
+  const int per = p.fast ? p.experts / p.groups : p.experts;
+  const int need = (per + lanes - 1) / lanes;
+  int epl = 1;
+  while (epl < need) epl <<= 1;
+  // every lane's piece is a power of two long; it is loaded whole if all pieces are aligned
+  const int64_t elem = p.dtype == kF32 ? 4 : 2;
+  const int64_t piece = epl * elem < 16 ? epl * elem : 16;
+  p.wide = per % epl == 0 && (p.ld * elem) % piece == 0 &&
+           reinterpret_cast<uint64_t>(p.logits) % piece == 0 ? 1 : 0;
+  p.wide_out = per % epl == 0 && (p.experts * elem) % 16 == 0 ? 1 : 0;
+  if (epl == 1) return launch<1>(p, backward, s);
+  if (epl == 2) return launch<2>(p, backward, s);
+  if (epl == 4) return launch<4>(p, backward, s);
+  if (epl == 8) return launch<8>(p, backward, s);
   return launch<16>(p, backward, s);
 }
 
@@ -356,6 +556,7 @@ extern "C" int tccl_expert_route(uint64_t logits, int64_t ld, uint64_t bias, uin
   TCCL_CHECK_ARG(groups >= 1 && groups <= 32 && experts % groups == 0,
                  "groups must be 1..32 and divide the experts");
   TCCL_CHECK_ARG(top_groups >= 1 && top_groups <= groups, "top_groups must be 1..groups");
+  p.fast = (groups & (groups - 1)) == 0 ? 1 : 0;
   if (tokens == 0) return kOk;
   TCCL_CHECK_ARG(logits != 0 && weights != 0 && ids != 0, "null argument");
   TCCL_CHECK_CUDA(dispatch(p, false, reinterpret_cast<cudaStream_t>(stream)));
@@ -378,7 +579,7 @@ extern "C" int tccl_expert_route_backward(uint64_t grad_weights, uint64_t logits
   p.top_k = top_k;
   p.dtype = dtype;
   p.sigmoid = sigmoid;
-  p.groups = 1;
+  p.groups = p.fast = 1;
   p.renormalize = renormalize;
   p.scale = scale;
   const int rc = check(p);

@@ -30,72 +30,86 @@ struct SlotParams {
   int32_t* token_of_slot;   // [entries]
   int32_t* slot_of;         // [entries]
   int32_t* counts;          // [CTAs][experts], null with a single CTA
-  int64_t run;              // entries per CTA
 };
 
-__device__ __forceinline__ int local_expert(const SlotParams& p, int64_t i) {
-  const int64_t e = static_cast<int64_t>(p.ids[i]) - p.first;
-  return e >= 0 && e < p.experts ? static_cast<int>(e) : -1;
+// Entries a lane keeps: a warp's segment is 32 * kPerLane long, a CTA's run kRun.
+constexpr int kPerLane = 8;
+constexpr int64_t kRun = kSlotWarps * 32 * kPerLane;
+
+// This lane's entries of its warp's segment as local experts (-1: none), 32 apart.
+__device__ __forceinline__ void load_entries(const SlotParams& p, int (&e)[kPerLane]) {
+  const int64_t at = blockIdx.x * kRun + (threadIdx.x >> 5) * (32 * kPerLane) + (threadIdx.x & 31);
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int64_t id = at + 32 * i < p.entries ? static_cast<int64_t>(p.ids[at + 32 * i]) - p.first : -1;
+    e[i] = id >= 0 && id < p.experts ? static_cast<int>(id) : -1;
+  }
 }
 
 // cnt[w][e] = entries of expert e in warp w's segment of this CTA's run
-__device__ void count_segments(const SlotParams& p, int64_t begin, int64_t end, int64_t seg,
-                               int32_t* cnt) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__device__ __forceinline__ void count_segments(const SlotParams& p, const int (&e)[kPerLane], int32_t* cnt) {
   for (int i = threadIdx.x; i < kSlotWarps * p.experts; i += kSlotThreads) cnt[i] = 0;
   __syncthreads();
-  int32_t* const mine = cnt + warp * p.experts;
-  const int64_t a = begin + warp * seg, b = a + seg < end ? a + seg : end;
-  for (int64_t i = a; i < b; i += 32) {
-    const int e = i + lane < b ? local_expert(p, i + lane) : -1;
-    if (e >= 0) atomicAdd(mine + e, 1);   // (a sum of ones: its order does not show)
-  }
+  int32_t* const mine = cnt + (threadIdx.x >> 5) * p.experts;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i)
+    if (e[i] >= 0) atomicAdd(mine + e[i], 1);   // (a sum of ones: its order does not show)
   __syncthreads();
 }
 
 __global__ void __launch_bounds__(kSlotThreads) expert_slot_count_kernel(const SlotParams p) {
   extern __shared__ int32_t cnt[];
-  const int64_t begin = blockIdx.x * p.run;
-  const int64_t end = begin + p.run < p.entries ? begin + p.run : p.entries;
-  count_segments(p, begin, end, (p.run + kSlotWarps - 1) / kSlotWarps, cnt);
+  int entry[kPerLane];
+  load_entries(p, entry);
+  count_segments(p, entry, cnt);
   for (int e = threadIdx.x; e < p.experts; e += kSlotThreads) {
     int32_t s = 0;
+#pragma unroll
     for (int w = 0; w < kSlotWarps; ++w) s += cnt[w * p.experts + e];
     p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e] = s;
   }
 }
 
 __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const SlotParams p) {
-  extern __shared__ int32_t cnt[];                 // [warps][experts], then [experts + 1]
-  int32_t* const start = cnt + kSlotWarps * p.experts;
-  __shared__ int32_t warp_total[kSlotWarps];
+  extern __shared__ int32_t cnt[];                 // [warps][experts], [experts], [experts]
+  int32_t* const all = cnt + kSlotWarps * p.experts;      // per expert: all entries
+  int32_t* const before = all + p.experts;                // and those in the runs of earlier CTAs
+  __shared__ int32_t warp_total[kSlotWarps], used;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t begin = blockIdx.x * p.run;
-  const int64_t end = begin + p.run < p.entries ? begin + p.run : p.entries;
-  const int64_t seg = (p.run + kSlotWarps - 1) / kSlotWarps;
-  count_segments(p, begin, end, seg, cnt);
+  int entry[kPerLane];
+  load_entries(p, entry);
+  for (int e = threadIdx.x; e < p.experts; e += kSlotThreads) all[e] = before[e] = 0;
+  count_segments(p, entry, cnt);
 
-  // per expert: all entries, and those in the runs of earlier CTAs
-  int32_t all[kMaxExperts / kSlotThreads], before[kMaxExperts / kSlotThreads];
+  if (p.counts == nullptr) {
+    for (int e = threadIdx.x; e < p.experts; e += kSlotThreads) {
+      int32_t c = 0;
+#pragma unroll
+      for (int w = 0; w < kSlotWarps; ++w) c += cnt[w * p.experts + e];
+      all[e] = c;
+    }
+  } else {
+    // the counts of all CTAs, as many rows at a time as the threads cover
+    const int rows = max(kSlotThreads / p.experts, 1), row = threadIdx.x / p.experts;
+    for (int e = threadIdx.x - row * p.experts; e < p.experts && row < rows; e += kSlotThreads) {
+      int32_t a = 0, b = 0;
+#pragma unroll 8
+      for (int c = row; c < static_cast<int>(gridDim.x); c += rows) {
+        const int32_t v = p.counts[static_cast<int64_t>(c) * p.experts + e];
+        a += v;
+        if (c < static_cast<int>(blockIdx.x)) b += v;
+      }
+      atomicAdd(all + e, a);
+      atomicAdd(before + e, b);
+    }
+  }
+  __syncthreads();
+  // exclusive scan of `all` over the experts
+  constexpr int kPer = kMaxExperts / kSlotThreads;
   int32_t sum = 0;
 #pragma unroll
-  for (int i = 0; i < kMaxExperts / kSlotThreads; ++i) {
-    const int e = threadIdx.x * (kMaxExperts / kSlotThreads) + i;
-    all[i] = before[i] = 0;
-    if (e < p.experts) {
-      if (p.counts == nullptr) {
-        for (int w = 0; w < kSlotWarps; ++w) all[i] += cnt[w * p.experts + e];
-      } else {
-        for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
-          const int32_t c = p.counts[static_cast<int64_t>(b) * p.experts + e];
-          all[i] += c;
-          if (b < static_cast<int>(blockIdx.x)) before[i] += c;
-        }
-      }
-    }
-    sum += all[i];
-  }
-  // exclusive scan of `sum` over the threads
+  for (int i = 0; i < kPer; ++i)
+    if (threadIdx.x * kPer + i < p.experts) sum += all[threadIdx.x * kPer + i];
   int32_t scan = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -107,29 +121,32 @@ __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const S
   int32_t base = scan - sum;
   for (int w = 0; w < warp; ++w) base += warp_total[w];
 #pragma unroll
-  for (int i = 0; i < kMaxExperts / kSlotThreads; ++i) {
-    const int e = threadIdx.x * (kMaxExperts / kSlotThreads) + i;
+  for (int i = 0; i < kPer; ++i) {
+    const int e = threadIdx.x * kPer + i;
     if (e < p.experts) {
+      const int32_t n = all[e];
       if (blockIdx.x == 0) p.offsets[e] = base;
-      int32_t at = base + before[i];
+      int32_t at = base + before[e];
+#pragma unroll
       for (int w = 0; w < kSlotWarps; ++w) {       // counts become starting slots
         const int32_t c = cnt[w * p.experts + e];
         cnt[w * p.experts + e] = at;
         at += c;
       }
-      base += all[i];
-      if (e == p.experts - 1) start[0] = base;
+      base += n;
+      if (e == p.experts - 1) {
+        used = base;
+        if (blockIdx.x == 0) p.offsets[p.experts] = base;
+      }
     }
   }
   __syncthreads();
-  const int32_t used = start[0];
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.offsets[p.experts] = used;
 
   int32_t* const mine = cnt + warp * p.experts;
-  const int64_t a = begin + warp * seg, b = a + seg < end ? a + seg : end;
-  for (int64_t i0 = a; i0 < b; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const int e = i < b ? local_expert(p, i) : -1;
+  const int64_t at = blockIdx.x * kRun + warp * (32 * kPerLane) + lane;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int e = entry[i];
     const uint32_t same = __match_any_sync(kAll, e);
     const int ahead = __popc(same & ((1u << lane) - 1u));
     int32_t slot = -1;
@@ -137,16 +154,17 @@ __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const S
     __syncwarp();
     if (e >= 0 && ahead == 0) mine[e] += __popc(same);
     __syncwarp();
-    if (i < b) {
-      p.slot_of[i] = slot;
-      if (slot >= 0) p.token_of_slot[slot] = static_cast<int32_t>(i / p.top_k);
-      // slots behind the last one hold -1 (slot i is written by whoever owns entry i)
-      if (i >= used) p.token_of_slot[i] = -1;
+    const int64_t j = at + 32 * i;
+    if (j < p.entries) {
+      p.slot_of[j] = slot;
+      if (slot >= 0) p.token_of_slot[slot] = static_cast<int32_t>(j / p.top_k);
+      // slots behind the last one hold -1 (slot j is written by whoever owns entry j)
+      if (j >= used) p.token_of_slot[j] = -1;
     }
   }
 }
 
-size_t slot_smem(int experts) { return sizeof(int32_t) * (kSlotWarps * experts + experts + 1); }
+size_t slot_smem(int experts) { return sizeof(int32_t) * (kSlotWarps + 2) * experts; }
 
 cudaError_t attrs_once() {
   static bool done[64] = {};
@@ -161,9 +179,7 @@ cudaError_t attrs_once() {
   return e;
 }
 
-// Entries one CTA takes; up to this many the map is built by a single launch of one CTA.
-constexpr int64_t kRun = 4096;
-
+// Up to kRun entries the map is built by a single launch of one CTA.
 int64_t slot_ctas(int64_t entries) { return entries <= kRun ? 1 : (entries + kRun - 1) / kRun; }
 
 }  // namespace
@@ -205,7 +221,6 @@ extern "C" int tccl_expert_slots(uint64_t ids, int64_t tokens, int32_t top_k, in
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   TCCL_CHECK_ARG(p.entries == 0 || (ids != 0 && token_of_slot != 0 && slot_of != 0), "null argument");
   const int64_t ctas = slot_ctas(p.entries);
-  p.run = ctas == 1 ? (p.entries > 0 ? p.entries : 1) : kRun;
   if (ctas > 1) {
     TCCL_CHECK_ARG(workspace != 0, "this many entries need a workspace");
     p.counts = reinterpret_cast<int32_t*>(workspace);
