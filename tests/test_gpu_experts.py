@@ -623,3 +623,30 @@ def test_backward_repeats_and_captures():
         torch.cuda.synchronize()
         assert torch.equal(gx, first[0]) and torch.equal(gw, first[1])
         assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups, top_groups", [(1, 1), (4, 2), (8, 3), (5, 2)])
+def test_route_decides_crowded_rows_exactly(score, groups, top_groups):
+    """Many keys within a few 2^-24 of one another, and many that are equal: at the border of
+    the choice, inside it, and between groups; also more near-equal keys than lanes."""
+    from tileccl_b200 import ops
+
+    E, k, T = 40 * groups if groups != 5 else 100, 6, 48
+    g = _gen(groups)
+    level = torch.randint(0, 3, (T, E), device="cuda", generator=g).float()
+    tiny = torch.randint(-2, 3, (T, E), device="cuda", generator=g).float() * 2 ** -22
+    logits = level + tiny
+    logits[::4] = level[::4]                              # exact ties only
+    bias = torch.where(torch.rand(E, device="cuda", generator=g) < 0.5, 0.0, 2 ** -23)
+    for b in (bias, torch.zeros_like(bias), None):
+        w, ids = ops.route_experts(logits, k, score=score, bias=b, groups=groups, top_groups=top_groups)
+        _, want = _route64(logits, k, score, b, groups, top_groups, "top2", True, 1.0, None)
+        same = ids == want
+        # Keys that differ by less than 2^-50 depend on the last bit of a 64-bit exponential: there
+        # either order is right, so compare the keys of the chosen, in order.
+        p = (torch.softmax(logits.double(), 1) if score == "softmax" else torch.sigmoid(logits.double()))
+        key = p + (0.0 if b is None else b.double())
+        got_k, want_k = key.gather(1, ids.long()), key.gather(1, want.long())
+        assert ((got_k - want_k).abs() <= 2 ** -50)[~same].all()
+        assert same.float().mean() > 0.99

@@ -24,9 +24,13 @@ namespace tileccl {
 namespace {
 
 constexpr int kWarpsPerCta = 4;
+constexpr int kMaxRouted = 512;          // experts at most (a power of two)
 constexpr uint32_t kAll = 0xffffffffu;
 
 enum RouteDtype : int { kF16 = 0, kBF16 = 1, kF32 = 2 };
+// What experts compete with: the logit itself (it orders like the score), or a score and a bias.
+// kExact: 16-bit logits, whose keys leave room for the whole index and need no second look.
+enum RouteMode : int { kByLogit = 0, kSigmoid = 1, kSoftmax = 2, kExact = 3 };
 
 struct RouteParams {
   const void* logits;
@@ -39,7 +43,7 @@ struct RouteParams {
   void* grad_logits;          // backward only, [tokens, experts] contiguous
   int64_t tokens;
   int32_t experts, top_k, dtype, sigmoid, groups, top_groups, group_max, renormalize;
-  int32_t fast;               // the groups share the lanes evenly
+  int32_t fast, lane_shift;   // the groups share the lanes evenly: 2^lane_shift lanes each
   int32_t wide, wide_out;     // a lane's logits (gradients) can be moved in whole pieces
   float scale;
 };
@@ -76,7 +80,19 @@ __device__ __forceinline__ float sigmoid_f(float x) { return 1.f / (1.f + expf(-
 // precision where both underflow.
 __device__ __forceinline__ float sigmoid_scaled(float l, float m) {
   const float s = fminf(m, 0.f);
-  return l > 0.f ? 1.f / (1.f + expf(-l)) : expf(l - s) / (1.f + expf(l));
+  return (l > 0.f ? 1.f : expf(l - s)) / (1.f + expf(-fabsf(l)));
+}
+
+// Approximations for keys (denormals count as zero: far below the keys' error).
+__device__ __forceinline__ float exp_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Numbers as unsigned integers of the same order.
@@ -164,6 +180,68 @@ __device__ __noinline__ int choose_exactly(const RouteParams& p, int64_t t, floa
   return mine;
 }
 
+// A key in 64 bits; `total` = sum of exp(l - top) over the row (softmax).
+__device__ __forceinline__ double key64(const RouteParams& p, int mode, float l, float bias, float top,
+                                        double total) {
+  if (mode == kByLogit) return l;      // (kExact never asks)
+  const double x = static_cast<double>(l);
+  const double s = mode == kSigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - static_cast<double>(top)) / total;
+  return s + static_cast<double>(bias);
+}
+// Sum of the row's exponentials in 64 bits; lane: logits first .. first + n - 1 of the row.
+__device__ __noinline__ double softmax_total(const RouteParams& p, int64_t at, int n, float top) {
+  double part = 0.0;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float l = load_logit(p.logits, at + i, p.dtype);
+    if (l != -CUDART_INF_F) part += exp(static_cast<double>(l) - static_cast<double>(top));
+  }
+  return warp_sum(part);
+}
+// Score of this lane's group in 64 bits; lane as above, `lanes` lanes per group.
+__device__ __noinline__ uint64_t group_score64(const RouteParams& p, int mode, int64_t at, int n, int first,
+                                               int lanes, float top, double total) {
+  uint64_t a = 0, b = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float l = load_logit(p.logits, at + i, p.dtype);
+    const float bias = p.bias != nullptr ? p.bias[first + i] : 0.f;
+    const uint64_t x = l == -CUDART_INF_F ? 0 : order64(key64(p, mode, l, bias, top, total));
+    b = b > (a < x ? a : x) ? b : (a < x ? a : x);
+    a = a > x ? a : x;
+  }
+  for (int o = 1; o < lanes; o <<= 1) {
+    const uint64_t c = __shfl_xor_sync(kAll, a, o), d = __shfl_xor_sync(kAll, b, o);
+    const uint64_t lower = a < c ? a : c, second = b > d ? b : d;
+    b = lower > second ? lower : second;
+    a = a > c ? a : c;
+  }
+  return p.group_max || b <= 1 ? a : order64(value64(a) + value64(b));
+}
+// Lane j holds candidate j (`id`, -1 = none).  Returns the candidates in the order of their
+// 64-bit keys, the lower index first among equals.
+__device__ __noinline__ int order_candidates(const RouteParams& p, int mode, int64_t row, int id, float top,
+                                             double total) {
+  uint64_t k = 0;
+  if (id >= 0)
+    k = order64(key64(p, mode, load_logit(p.logits, row + id, p.dtype), p.bias != nullptr ? p.bias[id] : 0.f,
+                      top, total));
+  int ahead = 0;
+  for (int i = 0; i < 32; ++i) {
+    const uint64_t other = __shfl_sync(kAll, k, i);
+    const int other_id = __shfl_sync(kAll, id, i);
+    ahead += other_id >= 0 && (other > k || (other == k && other_id < id)) ? 1 : 0;
+  }
+  const int lane = threadIdx.x & 31;
+  int out = -1;
+  for (int i = 0; i < 32; ++i) {
+    const int place = __shfl_sync(kAll, id >= 0 ? ahead : -1, i);
+    const int other_id = __shfl_sync(kAll, id, i);
+    if (place == lane) out = other_id;
+  }
+  return out;
+}
+
 // Lane `lane` holds the logits first .. first + n - 1 (n <= EPL) of its row, -inf behind them.
 template <int EPL>
 __device__ __forceinline__ void load_logits(const RouteParams& p, int64_t at, int n, float (&l)[EPL]) {
@@ -220,28 +298,28 @@ __device__ __forceinline__ void sort_descending(uint32_t (&v)[N]) {
 
 // EPL: experts per lane (a power of two).  The lanes are shared out evenly among the groups;
 // within a group lane i holds the experts i * EPL, i * EPL + 1, ...
-template <int EPL>
-__global__ void __launch_bounds__(kWarpsPerCta * 32)
+template <int EPL, int kMode>
+__global__ void __launch_bounds__(kWarpsPerCta * 32, EPL < 16 ? 8 : 4)
 expert_route_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ uint64_t smem_keys[];   // [warps][experts]
+  constexpr bool kByKey = kMode == kByLogit || kMode == kExact;
+  // low bits of a key: the place in the lane's list, or the whole index, the lowest on top
+  constexpr uint32_t kPlace = kMode == kExact ? kMaxRouted - 1u : EPL - 1u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint64_t* const keys64 = smem_keys + static_cast<int64_t>(warp) * p.experts;
-  const int lanes = p.fast ? 32 / p.groups : 32;                  // per group
+  const int lanes = 1 << p.lane_shift;                            // per group
   const int per = p.fast ? p.experts / p.groups : p.experts;
-  const int group = lane / lanes;
+  const int group = lane >> p.lane_shift;
   const int in_group = (lane - group * lanes) * EPL;
   const int first = group * per + in_group;
   const int n = min(max(per - in_group, 0), EPL);
-  const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_max != 0);
-  const bool exact = by_logit && p.dtype != kF32;
-  // Error of a key: the bits that hold the place in the list (2^-23 EPL of the key, twice), and
-  // that of its score: sigmoid 1/4 (2 + 1.2 |l|) 2^-23 and a sum and a division, below 2^-20;
-  // softmax, whose sum carries the errors of all terms, below 2^-18.
-  const float key_error = by_logit ? 0.f : 4.f * EPL * 0x1p-23f;
-  const float score_error = by_logit ? 0.f : p.sigmoid ? 0x1p-19f : 0x1p-17f;
+  // Error of a pair of keys: the bits that hold the place (2^-23 EPL of each), and that of the
+  // scores: sigmoid 1/4 (2 + 1.2 |l|) 2^-23, a sum and a division, below 2^-20 each; softmax,
+  // whose sum carries the errors of all terms, below 2^-18 each.
+  constexpr float kKeyError = kByKey ? 0.f : 4.f * EPL * 0x1p-23f;
+  constexpr float kScoreError = kByKey ? 0.f : kMode == kSigmoid ? 0x1p-19f : 0x1p-17f;
   float bias[EPL];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) bias[i] = p.bias != nullptr && i < n ? p.bias[first + i] : 0.f;
+  for (int i = 0; i < EPL; ++i) bias[i] = !kByKey && p.bias != nullptr && i < n ? p.bias[first + i] : 0.f;
 
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + warp; t < p.tokens;
        t += static_cast<int64_t>(gridDim.x) * kWarpsPerCta) {
@@ -251,10 +329,11 @@ expert_route_kernel(const __grid_constant__ RouteParams p) {
       if (lane < p.top_k) { out_w[lane] = 0.f; out_i[lane] = -1; }
       continue;
     }
+    const int64_t row = t * p.ld;
     float l[EPL];
-    load_logits<EPL>(p, t * p.ld + first, n, l);
+    load_logits<EPL>(p, row + first, n, l);
     float top = l[0];
-    if (!p.sigmoid || !p.fast) {
+    if (!p.sigmoid) {
 #pragma unroll
       for (int i = 1; i < EPL; ++i) top = fmaxf(top, l[i]);
       top = value32(__reduce_max_sync(kAll, top != top ? 0u : order32(top)));
@@ -262,105 +341,135 @@ expert_route_kernel(const __grid_constant__ RouteParams p) {
 
     // approximate keys, packed with the place in the lane's list
     uint32_t key[EPL];
-    bool odd = !p.fast;                    // something the approximate way does not cover
-    float inv = 1.f;
     float x[EPL];
-    if (by_logit) {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) x[i] = l[i];
-    } else if (p.sigmoid) {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) x[i] = __fdividef(1.f, 1.f + __expf(-l[i]));
-    } else {
+    float inv = 1.f;
+    if (kMode == kSoftmax) {
       float part = 0.f;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) part += x[i] = __expf(l[i] - top);
-      inv = __fdividef(1.f, warp_sum(part));
+      for (int i = 0; i < EPL; ++i) part += x[i] = exp_approx(l[i] - top);
+      inv = rcp_approx(warp_sum(part));
     }
+    float finite = 0.f;                    // NaN if a key is infinite or not a number
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const float k = by_logit ? x[i] : fmaf(x[i], inv, bias[i]);
-      const bool there = i < n && l[i] != -CUDART_INF_F && bias[i] != -CUDART_INF_F;
-      odd = odd || (there && !(fabsf(k) < CUDART_INF_F));
-      key[i] = there ? (order32(k) & ~(EPL - 1u)) | (EPL - 1u - i) : 0u;
+      float k = l[i];
+      if (kMode == kSigmoid) k = rcp_approx(1.f + exp_approx(-l[i])) + bias[i];
+      if (kMode == kSoftmax) k = fmaf(x[i], inv, bias[i]);
+      const bool there = l[i] != -CUDART_INF_F && (kByKey || k != -CUDART_INF_F);   // (-inf behind the row)
+      finite = fmaf(there ? k : 0.f, 0.f, finite);
+      const uint32_t place = kMode == kExact ? kPlace - first - i : kPlace - i;
+      key[i] = there ? (order32(k) & ~kPlace) | place : 0u;
     }
-    bool close = false;
-    sort_descending(key);
-    if (p.groups > 1 && p.fast) {
-      uint32_t a = key[0], b = EPL > 1 ? key[EPL > 1 ? 1 : 0] : 0u;
-      for (int o = 1; o < lanes; o <<= 1) {
-        const uint32_t c = __shfl_xor_sync(kAll, a, o), d = __shfl_xor_sync(kAll, b, o);
-        b = max(min(a, c), max(b, d));
-        a = max(a, c);
-      }
-      const float va = value32(a & ~(EPL - 1u)), vb = value32(b & ~(EPL - 1u));
-      const uint32_t score = a == 0 ? 0u : order32(p.group_max || b == 0 ? va : va + vb);
-      int ahead = 0;
-      for (int g = 0; g < p.groups; ++g) {
-        const uint32_t other = __shfl_sync(kAll, score, g * lanes);
-        ahead += (other > score || (other == score && g < group)) ? 1 : 0;
-      }
-      const bool keep = ahead < p.top_groups;
-      const uint32_t worst = __reduce_min_sync(kAll, keep ? score : kAll);
-      const uint32_t next = __reduce_max_sync(kAll, keep ? 0u : score);
-      if (!exact && next != 0) {
-        const float w = value32(worst), v = value32(next);
-        const float size = fmaxf(fabsf(w), fabsf(v)) + (p.group_max ? 0.f : 2.f * fabsf(va) + 2.f * fabsf(vb));
-        close = !(w - v > size * key_error + 2.f * score_error);
-      }
-      if (!keep) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) key[i] = 0u;
-      }
-    }
-    // k rounds (and one to see who comes next): the largest head, the lowest lane among equals
+    const bool odd = !p.fast || __any_sync(kAll, finite != 0.f);
     int id = -1;
-    uint32_t mine = 0, after = 0;
-    const int rounds = p.top_k + (exact ? 0 : 1);
-    for (int j = 0; j < rounds; ++j) {
-      const uint32_t head = key[0] & ~(EPL - 1u);     // (places compare within a lane only)
-      const uint32_t best = __reduce_max_sync(kAll, head);
-      if (best == 0) break;
-      const int from = __ffs(__ballot_sync(kAll, head == best)) - 1;
-      if (j == p.top_k) { after = best; break; }
-      const int e = __shfl_sync(kAll, first + (EPL - 1) - static_cast<int>(key[0] & (EPL - 1u)), from);
-      if (lane == j) { id = e; mine = best; }
-      if (lane == from) {
-#pragma unroll
-        for (int i = 0; i + 1 < EPL; ++i) key[i] = key[i + 1];
-        key[EPL - 1] = 0u;
-      }
-    }
-    float my_l = id >= 0 ? load_logit(p.logits, t * p.ld + id, p.dtype) : -CUDART_INF_F;
-    if (!exact) {
-      uint32_t below = __shfl_down_sync(kAll, mine, 1);
-      if (lane == p.top_k - 1) below = after;
-      if (lane < p.top_k && below != 0) {
-        const float w = value32(mine), v = value32(below);
-        close = close || !(w - v > fmaxf(fabsf(w), fabsf(v)) * key_error + score_error);
-      }
-      // two of the chosen that agree in logit and bias are equal exactly: in place already
-      if (__any_sync(kAll, close)) {
-        const float next_l = __shfl_down_sync(kAll, my_l, 1);
-        const float my_b = p.bias != nullptr && id >= 0 ? p.bias[id] : 0.f;
-        const float next_b = __shfl_down_sync(kAll, my_b, 1);
-        if (lane < p.top_k - 1 && mine != 0 && p.groups == 1 && my_l == next_l && my_b == next_b)
-          close = false;
-      }
-    }
     bool broken = false;                   // a row without numbers for weights
-    if (__any_sync(kAll, odd || close)) {
+    float my_l = -CUDART_INF_F;
+    if (odd) {
 #pragma unroll
       for (int i = 0; i < EPL; ++i) broken = broken || l[i] != l[i];
-      broken = __any_sync(kAll, broken);
-      if (p.sigmoid && p.fast) {
+      broken = __any_sync(kAll, broken) || (!p.sigmoid && top == CUDART_INF_F);   // as the formula has it
+      id = choose_exactly(p, t, top, smem_keys + static_cast<int64_t>(warp) * p.experts);
+      if (id >= 0) my_l = load_logit(p.logits, row + id, p.dtype);
+    } else {
+      sort_descending(key);
+      double total = 1.0;
+      bool have_total = kMode != kSoftmax;
+      if (p.groups > 1) {
+        uint32_t a = key[0], b = EPL > 1 ? key[EPL > 1 ? 1 : 0] : 0u;
+        for (int o = 1; o < lanes; o <<= 1) {
+          const uint32_t c = __shfl_xor_sync(kAll, a, o), d = __shfl_xor_sync(kAll, b, o);
+          b = max(min(a, c), max(b, d));
+          a = max(a, c);
+        }
+        const float va = value32(a & ~kPlace), vb = value32(b & ~kPlace);
+        const uint32_t score = a == 0 ? 0u : order32(p.group_max || b == 0 ? va : va + vb);
+        int ahead = 0;
+        for (int g = 0; g < p.groups; ++g) {
+          const uint32_t other = __shfl_sync(kAll, score, g * lanes);
+          ahead += other > score || (other == score && g < group) ? 1 : 0;
+        }
+        bool keep = ahead < p.top_groups;
+        if (kMode != kExact) {
+          const uint32_t worst = __reduce_min_sync(kAll, keep ? score : kAll);
+          const uint32_t next = __reduce_max_sync(kAll, keep ? 0u : score);
+          const float w = value32(worst), v = value32(next);
+          const float size = fmaxf(fabsf(w), fabsf(v)) + (p.group_max ? 0.f : 2.f * fabsf(va) + 2.f * fabsf(vb));
+          if (__any_sync(kAll, next != 0 && !(w - v > size * kKeyError + 2.f * kScoreError))) {
+            if (!have_total) total = softmax_total(p, row + first, n, top);
+            have_total = true;
+            const uint64_t mine = group_score64(p, kMode, row + first, n, first, lanes, top, total);
+            ahead = 0;
+            for (int g = 0; g < p.groups; ++g) {
+              const uint64_t other = __shfl_sync(kAll, mine, g * lanes);
+              ahead += other > mine || (other == mine && g < group) ? 1 : 0;
+            }
+            keep = ahead < p.top_groups;
+          }
+        }
+        if (!keep) {
 #pragma unroll
-        for (int i = 1; i < EPL; ++i) top = fmaxf(top, l[i]);
-        top = warp_max(top);
+          for (int i = 0; i < EPL; ++i) key[i] = 0u;
+        }
       }
-      if (!p.sigmoid && top == CUDART_INF_F) broken = true;     // as the formula has it
-      id = choose_exactly(p, t, top, keys64);
-      my_l = id >= 0 ? load_logit(p.logits, t * p.ld + id, p.dtype) : -CUDART_INF_F;
+      // k rounds, each takes the largest head; with inexact keys they go on while the next is too
+      // close to the k-th to tell them apart.
+      uint32_t mine = 0;
+      int from = 0;                        // lane that held this lane's choice
+      float limit = -CUDART_INF_F;
+      bool close = false, many = false;
+      for (int j = 0;; ++j) {
+        if (kMode == kExact && j == p.top_k) break;
+        const uint32_t best = __reduce_max_sync(kAll, key[0]);
+        if (best == 0) break;
+        if (kMode != kExact && j >= p.top_k) {
+          if (value32(best & ~kPlace) < limit) break;
+          close = true;
+          if (j == 32) { many = true; break; }
+        }
+        bool winner = key[0] == best;
+        int at = 0;
+        if (kMode != kExact) {             // (equal heads of two lanes are close: any goes first)
+          at = __ffs(__ballot_sync(kAll, winner)) - 1;
+          winner = lane == at;
+        }
+        if (lane == j) { mine = best; from = at; }
+        if (winner) {
+#pragma unroll
+          for (int i = 0; i + 1 < EPL; ++i) key[i] = key[i + 1];
+          key[EPL - 1] = 0u;
+        }
+        if (kMode != kExact && j == p.top_k - 1) {
+          const float v = value32(best & ~kPlace);
+          limit = kByKey ? v : v - (fabsf(v) * kKeyError + kScoreError);
+        }
+      }
+      if (mine != 0) {
+        const int place = static_cast<int>(kPlace - (mine & kPlace));
+        id = kMode == kExact ? place : (from >> p.lane_shift) * per + (from & (lanes - 1)) * EPL + place;
+        mine &= ~kPlace;
+      }
+      if (id >= 0) my_l = load_logit(p.logits, row + id, p.dtype);
+      if (kMode != kExact) {
+        const uint32_t below = __shfl_down_sync(kAll, mine, 1);
+        const float w = value32(mine), v = value32(below);
+        const bool pair = lane < p.top_k - 1 && below != 0 &&
+                    !(w - v > fmaxf(fabsf(w), fabsf(v)) * kKeyError + kScoreError);
+        if (__any_sync(kAll, pair)) {
+          // two of the chosen that agree in logit and bias are equal exactly: the index decides
+          const int next_id = __shfl_down_sync(kAll, id, 1);
+          const float my_b = !kByKey && p.bias != nullptr && id >= 0 ? p.bias[id] : 0.f;
+          const float next_l = __shfl_down_sync(kAll, my_l, 1), next_b = __shfl_down_sync(kAll, my_b, 1);
+          close = close || __any_sync(kAll, pair && !(my_l == next_l && my_b == next_b && id < next_id));
+        }
+        if (many) {
+          id = choose_exactly(p, t, top, smem_keys + static_cast<int64_t>(warp) * p.experts);
+        } else if (close) {
+          if (!have_total) total = softmax_total(p, row + first, n, top);
+          id = order_candidates(p, kMode, row, id, top, total);
+        }
+        if (lane >= p.top_k) id = -1;
+        if (close) my_l = id >= 0 ? load_logit(p.logits, row + id, p.dtype) : -CUDART_INF_F;
+      }
     }
 
     // weights: lane j holds the j-th choice
@@ -392,7 +501,7 @@ expert_route_kernel(const __grid_constant__ RouteParams p) {
 //   sigmoid                 dl_i = scale g_i p_i (1 - p_i)                      i chosen
 template <int EPL>
 __global__ void __launch_bounds__(kWarpsPerCta * 32)
-expert_route_backward_kernel(const RouteParams p) {
+expert_route_backward_kernel(const __grid_constant__ RouteParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + warp;
   if (t >= p.tokens) return;
@@ -476,13 +585,17 @@ constexpr int64_t kMaxCtas = 148 * 8;
 
 template <int EPL>
 cudaError_t launch(const RouteParams& p, bool backward, cudaStream_t s) {
+  const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_max != 0);
   const int64_t blocks = (p.tokens + kWarpsPerCta - 1) / kWarpsPerCta;
   if (backward) {
     expert_route_backward_kernel<EPL><<<static_cast<unsigned>(blocks), kWarpsPerCta * 32, 0, s>>>(p);
   } else {
     const size_t smem = sizeof(uint64_t) * kWarpsPerCta * p.experts;
-    expert_route_kernel<EPL><<<static_cast<unsigned>(blocks < kMaxCtas ? blocks : kMaxCtas),
-                               kWarpsPerCta * 32, smem, s>>>(p);
+    const unsigned grid = static_cast<unsigned>(blocks < kMaxCtas ? blocks : kMaxCtas);
+    if (by_logit && p.dtype != kF32) expert_route_kernel<EPL, kExact><<<grid, kWarpsPerCta * 32, smem, s>>>(p);
+    else if (by_logit) expert_route_kernel<EPL, kByLogit><<<grid, kWarpsPerCta * 32, smem, s>>>(p);
+    else if (p.sigmoid) expert_route_kernel<EPL, kSigmoid><<<grid, kWarpsPerCta * 32, smem, s>>>(p);
+    else expert_route_kernel<EPL, kSoftmax><<<grid, kWarpsPerCta * 32, smem, s>>>(p);
   }
   return cudaGetLastError();
 }
@@ -491,6 +604,8 @@ cudaError_t dispatch(RouteParams& p, bool backward, cudaStream_t s) {
   const int lanes = p.fast ? 32 / p.groups : 32;
   const int per = p.fast ? p.experts / p.groups : p.experts;
   const int need = (per + lanes - 1) / lanes;
+  p.lane_shift = 0;
+  while ((1 << p.lane_shift) < lanes) ++p.lane_shift;
   int epl = 1;
   while (epl < need) epl <<= 1;
   // every lane's piece is a power of two long; it is loaded whole if all pieces are aligned
@@ -508,7 +623,7 @@ cudaError_t dispatch(RouteParams& p, bool backward, cudaStream_t s) {
 
 int check(const RouteParams& p) {
   TCCL_CHECK_ARG(p.tokens >= 0 && p.tokens < (int64_t(1) << 31), "tokens out of range");
-  TCCL_CHECK_ARG(p.experts >= 1 && p.experts <= 512, "experts must be 1..512");
+  TCCL_CHECK_ARG(p.experts >= 1 && p.experts <= kMaxRouted, "experts must be 1..512");
   TCCL_CHECK_ARG(p.top_k >= 1 && p.top_k <= 32 && p.top_k <= p.experts,
                  "top_k must be 1..min(32, experts)");
   TCCL_CHECK_ARG(p.dtype >= 0 && p.dtype <= 2, "dtype must be 0 (fp16), 1 (bf16) or 2 (fp32)");
@@ -520,7 +635,7 @@ int check(const RouteParams& p) {
 
 cudaError_t preload_expert_route_kernels() {
   cudaFuncAttributes a;
-  cudaError_t e = cudaFuncGetAttributes(&a, expert_route_kernel<8>);
+  cudaError_t e = cudaFuncGetAttributes(&a, expert_route_kernel<8, kByLogit>);
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_route_backward_kernel<8>);
   return e;
 }
