@@ -34,48 +34,57 @@ struct CombineParams {
   int32_t top_k, vecs, bf16;   // vecs: 16-byte vectors per row
 };
 
-// Rows of H are fetched kBatch at a time: the slots of a token first, then that many rows'
-// vectors, all in flight together.
-constexpr int kBatch = 8;
-
+// A thread sums kVecs vectors of a token's row, kThreads apart.  The rows of H are fetched kBatch
+// at a time: their slots first, then all of their vectors, in flight together; kBatch * kVecs is
+// 8, which is what the registers of a full SM have room for.
+template <int kBatch>
 __global__ void __launch_bounds__(kThreads) expert_combine_kernel(const CombineParams p) {
+  constexpr int kVecs = 8 / kBatch;
   const int64_t t = blockIdx.x;
-  const int v = blockIdx.y * kThreads + threadIdx.x;
-  if (v >= p.vecs) return;
+  const int v0 = blockIdx.y * (kThreads * kVecs) + threadIdx.x;
   const bool bf16 = p.bf16 != 0;
-  float acc[8] = {};
-  uint4 base = make_uint4(0, 0, 0, 0);
-  if (p.add != nullptr) base = p.add[t * p.add_ld + v];
+  float acc[kVecs][8] = {};
+#pragma unroll
+  for (int c = 0; c < kVecs; ++c)
+    if (p.add != nullptr && v0 + c * kThreads < p.vecs)
+      tile_accumulate_16x8(bf16, acc[c], p.add[t * p.add_ld + v0 + c * kThreads]);
   for (int j0 = 0; j0 < p.top_k; j0 += kBatch) {
     int32_t s[kBatch];
     float w[kBatch];
-    uint4 x[kBatch];
+    uint4 x[kBatch][kVecs];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       s[j] = j0 + j < p.top_k ? p.slot_of[t * p.top_k + j0 + j] : -1;
       if (s[j] >= p.slots) s[j] = -1;
+      w[j] = s[j] < 0 ? 0.f : p.weights != nullptr ? p.weights[t * p.top_k + j0 + j] : 1.f;
     }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
-      if (s[j] >= 0) {
-        x[j] = ld_stream_v4(p.h + s[j] * p.h_ld + v);
-        w[j] = p.weights != nullptr ? p.weights[t * p.top_k + j0 + j] : 1.f;
-      }
-    if (j0 == 0) tile_accumulate_16x8(bf16, acc, base);
+#pragma unroll
+      for (int c = 0; c < kVecs; ++c)
+        if (s[j] >= 0 && v0 + c * kThreads < p.vecs)
+          x[j][c] = ld_stream_v4(p.h + s[j] * p.h_ld + v0 + c * kThreads);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
       if (s[j] >= 0) {
-        float f[8] = {};
-        tile_accumulate_16x8(bf16, f, x[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+        for (int c = 0; c < kVecs; ++c) {
+          float f[8] = {};
+          tile_accumulate_16x8(bf16, f, x[j][c]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[c][i] = fmaf(w[j], f[i], acc[c][i]);
+        }
       }
   }
-  p.out[t * p.out_ld + v] = tile_cast_f32x8(bf16, acc);
+#pragma unroll
+  for (int c = 0; c < kVecs; ++c)
+    if (v0 + c * kThreads < p.vecs)
+      p.out[t * p.out_ld + v0 + c * kThreads] = tile_cast_f32x8(bf16, acc[c]);
 }
 
 // One CTA per token.  A batch of choices at a time: dy stays in registers, every row of H is
 // read once, and the dot products of the batch meet in one reduction.
+template <int kBatch>
 __global__ void __launch_bounds__(kThreads) expert_combine_backward_kernel(const CombineParams p) {
   __shared__ float part[kThreads / 32][kBatch];
   const int64_t t = blockIdx.x;
@@ -163,8 +172,8 @@ int check(const CombineParams& p) {
 
 cudaError_t preload_expert_combine_kernels() {
   cudaFuncAttributes a;
-  cudaError_t e = cudaFuncGetAttributes(&a, expert_combine_kernel);
-  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_combine_backward_kernel);
+  cudaError_t e = cudaFuncGetAttributes(&a, expert_combine_kernel<8>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_combine_backward_kernel<8>);
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_gather_kernel);
   return e;
 }
@@ -199,8 +208,14 @@ extern "C" int tccl_expert_combine(uint64_t h, int64_t h_ld, uint64_t slot_of, u
   if (rc) return rc;
   if (tokens == 0) return kOk;
   TCCL_CHECK_ARG(h != 0 && slot_of != 0 && out != 0, "null argument");
-  const dim3 grid(static_cast<unsigned>(tokens), (p.vecs + kThreads - 1) / kThreads);
-  expert_combine_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  // (few tokens: narrow pieces, so that a row is spread over more SMs)
+  const int batch = top_k > 4 || tokens < 256 ? 8 : top_k > 2 ? 4 : 2;
+  const int piece = kThreads * (8 / batch);
+  const dim3 grid(static_cast<unsigned>(tokens), (p.vecs + piece - 1) / piece);
+  const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+  if (batch == 8) expert_combine_kernel<8><<<grid, kThreads, 0, cs>>>(p);
+  else if (batch == 4) expert_combine_kernel<4><<<grid, kThreads, 0, cs>>>(p);
+  else expert_combine_kernel<2><<<grid, kThreads, 0, cs>>>(p);
   TCCL_CHECK_CUDA(cudaGetLastError());
   return kOk;
 }
@@ -234,8 +249,11 @@ extern "C" int tccl_expert_combine_backward(uint64_t dy, int64_t dy_ld, uint64_t
   if (tokens == 0) return kOk;
   TCCL_CHECK_ARG(h != 0 && slot_of != 0 && weights != 0 && dy != 0 && dh != 0 && dw != 0,
                  "null argument");
-  expert_combine_backward_kernel<<<static_cast<unsigned>(tokens), kThreads, 0,
-                                   reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(tokens);
+  if (top_k > 4) expert_combine_backward_kernel<8><<<grid, kThreads, 0, cs>>>(p);
+  else if (top_k > 2) expert_combine_backward_kernel<4><<<grid, kThreads, 0, cs>>>(p);
+  else expert_combine_backward_kernel<2><<<grid, kThreads, 0, cs>>>(p);
   TCCL_CHECK_CUDA(cudaGetLastError());
   return kOk;
 }

@@ -517,13 +517,20 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
         if (s.words[2] == 0) continue;
         __threadfence();
       }
-      for (int c0 = 0; c0 <= last_c0; c0 += kChunk) {
-        uint4 dh = make_uint4(0, 0, 0, 0);
-        if (kEpi == kSiluGateGrad && c0 + me / kVecs < it.rows)      // (one vector per thread)
-          dh = __ldg(reinterpret_cast<const uint4*>(
+      // The gate's gradient reads dL/dout one step ahead (one vector per thread and step).
+      auto load_dh = [&](int c0) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (kEpi == kSiluGateGrad && c0 + me / kVecs < it.rows)
+          x = __ldg(reinterpret_cast<const uint4*>(
               static_cast<const char*>(p.dh) +
               2 * (static_cast<int64_t>(it.row0 + c0 + me / kVecs) * p.ld_dh + it.f0 / 2 + cta * 64 +
                    me % kVecs * 8)));
+        return x;
+      };
+      uint4 dh_next = load_dh(0);
+      for (int c0 = 0; c0 <= last_c0; c0 += kChunk) {
+        const uint4 dh = dh_next;
+        dh_next = load_dh(c0 + kChunk);
         float v[kChunk];
         if (it.parts > 1) {
           for (int i = 0; i < it.parts; ++i) {
