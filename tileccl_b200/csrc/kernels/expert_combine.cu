@@ -14,7 +14,7 @@
 namespace tileccl {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct CombineParams {
   const uint4* h;            // [slots] rows of `n` 16-bit values
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads) expert_combine_backward_kernel(const
       const uint4 dy = p.dy[t * p.dy_ld + v];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
-        if (s[j] >= 0) x[j] = ld_stream_v4(p.h + s[j] * p.h_ld + v);
+        if (s[j] >= 0) x[j] = p.h[s[j] * p.h_ld + v];
       float g[8] = {};
       tile_accumulate_16x8(bf16, g, dy);
 #pragma unroll
