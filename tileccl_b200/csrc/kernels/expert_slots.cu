@@ -24,8 +24,8 @@ constexpr uint32_t kAll = 0xffffffffu;
 
 struct SlotParams {
   const int32_t* ids;       // [entries]
-  int64_t entries;
-  int32_t top_k, experts, first;
+  uint32_t entries, top_k;
+  int32_t experts, first;
   int32_t* offsets;         // [experts + 1]
   int32_t* token_of_slot;   // [entries]
   int32_t* slot_of;         // [entries]
@@ -36,13 +36,21 @@ struct SlotParams {
 constexpr int kPerLane = 8;
 constexpr int64_t kRun = kSlotWarps * 32 * kPerLane;
 
+// This lane's first entry.  Entries are counted in 32 bits: there are less than 2^31, and a 64-bit
+// division per entry took a quarter of the placing kernel.
+__device__ __forceinline__ uint32_t first_entry() {
+  return blockIdx.x * static_cast<uint32_t>(kRun) + (threadIdx.x >> 5) * (32 * kPerLane) + (threadIdx.x & 31);
+}
+
 // This lane's entries of its warp's segment as local experts (-1: none), 32 apart.
 __device__ __forceinline__ void load_entries(const SlotParams& p, int (&e)[kPerLane]) {
-  const int64_t at = blockIdx.x * kRun + (threadIdx.x >> 5) * (32 * kPerLane) + (threadIdx.x & 31);
+  const uint32_t at = first_entry();
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
-    const int64_t id = at + 32 * i < p.entries ? static_cast<int64_t>(p.ids[at + 32 * i]) - p.first : -1;
-    e[i] = id >= 0 && id < p.experts ? static_cast<int>(id) : -1;
+    // (an id below `first` wraps around to a large number)
+    const int32_t id = at + 32 * i < p.entries ? p.ids[at + 32 * i] : -1;
+    const uint32_t local = static_cast<uint32_t>(id) - static_cast<uint32_t>(p.first);
+    e[i] = id >= 0 && local < static_cast<uint32_t>(p.experts) ? static_cast<int>(local) : -1;
   }
 }
 
@@ -79,8 +87,26 @@ __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const S
   int entry[kPerLane];
   load_entries(p, entry);
   for (int e = threadIdx.x; e < p.experts; e += kSlotThreads) all[e] = before[e] = 0;
+  // The counts of all CTAs, as many rows at a time as the threads cover; they come in while this
+  // CTA counts its own.
+  const int rows = max(kSlotThreads / p.experts, 1), row = threadIdx.x / p.experts;
+  const int column = threadIdx.x - row * p.experts;
+  constexpr int kPer = kMaxExperts / kSlotThreads;
+  int32_t sum_all[kPer] = {}, sum_before[kPer] = {};
+  if (p.counts != nullptr && row < rows) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = column + i * kSlotThreads;
+      if (e >= p.experts) continue;
+#pragma unroll 16
+      for (int c = row; c < static_cast<int>(gridDim.x); c += rows) {
+        const int32_t v = p.counts[static_cast<int64_t>(c) * p.experts + e];
+        sum_all[i] += v;
+        if (c < static_cast<int>(blockIdx.x)) sum_before[i] += v;
+      }
+    }
+  }
   count_segments(p, entry, cnt);
-
   if (p.counts == nullptr) {
     for (int e = threadIdx.x; e < p.experts; e += kSlotThreads) {
       int32_t c = 0;
@@ -88,24 +114,17 @@ __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const S
       for (int w = 0; w < kSlotWarps; ++w) c += cnt[w * p.experts + e];
       all[e] = c;
     }
-  } else {
-    // the counts of all CTAs, as many rows at a time as the threads cover
-    const int rows = max(kSlotThreads / p.experts, 1), row = threadIdx.x / p.experts;
-    for (int e = threadIdx.x - row * p.experts; e < p.experts && row < rows; e += kSlotThreads) {
-      int32_t a = 0, b = 0;
-#pragma unroll 8
-      for (int c = row; c < static_cast<int>(gridDim.x); c += rows) {
-        const int32_t v = p.counts[static_cast<int64_t>(c) * p.experts + e];
-        a += v;
-        if (c < static_cast<int>(blockIdx.x)) b += v;
-      }
-      atomicAdd(all + e, a);
-      atomicAdd(before + e, b);
+  } else if (row < rows) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = column + i * kSlotThreads;
+      if (e >= p.experts) continue;
+      atomicAdd(all + e, sum_all[i]);
+      atomicAdd(before + e, sum_before[i]);
     }
   }
   __syncthreads();
   // exclusive scan of `all` over the experts
-  constexpr int kPer = kMaxExperts / kSlotThreads;
   int32_t sum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
@@ -143,7 +162,7 @@ __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const S
   __syncthreads();
 
   int32_t* const mine = cnt + warp * p.experts;
-  const int64_t at = blockIdx.x * kRun + warp * (32 * kPerLane) + lane;
+  const uint32_t at = first_entry();
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
     const int e = entry[i];
@@ -154,12 +173,12 @@ __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const S
     __syncwarp();
     if (e >= 0 && ahead == 0) mine[e] += __popc(same);
     __syncwarp();
-    const int64_t j = at + 32 * i;
+    const uint32_t j = at + 32 * i;
     if (j < p.entries) {
       p.slot_of[j] = slot;
       if (slot >= 0) p.token_of_slot[slot] = static_cast<int32_t>(j / p.top_k);
       // slots behind the last one hold -1 (slot j is written by whoever owns entry j)
-      if (j >= used) p.token_of_slot[j] = -1;
+      if (j >= static_cast<uint32_t>(used)) p.token_of_slot[j] = -1;
     }
   }
 }
@@ -211,7 +230,7 @@ extern "C" int tccl_expert_slots(uint64_t ids, int64_t tokens, int32_t top_k, in
   TCCL_CHECK_ARG(offsets != 0, "null argument");
   SlotParams p = {};
   p.ids = reinterpret_cast<const int32_t*>(ids);
-  p.entries = tokens * top_k;
+  p.entries = static_cast<uint32_t>(tokens * top_k);
   p.top_k = top_k;
   p.experts = experts;
   p.first = first;
