@@ -142,7 +142,7 @@ def test_native_entries_check_their_arguments():
     d = _native.ExpertGemm()
     fields = dict(dtype=0, epilogue=0, experts=3, w_nk=0, k=16, n=24, slots=8, offsets=64, x=64, w=64, out=64, dh=0, ldx=16, ldw=24, w_expert=384, ldo=24, partial=0,
                   counters=0)
-    for name, bad in [("dtype", 2), ("epilogue", 3), ("epilogue", 1), ("experts", 0),
+    for name, bad in [("dtype", 2), ("epilogue", 4), ("epilogue", 1), ("experts", 0),
                       ("experts", 1025), ("k", 12), ("n", 20), ("k", 0), ("ldx", 12), ("x", 72),
                       ("slots", -1), ("slots", 1 << 31), ("x", 0), ("offsets", 0),
                       ("partial", 64)]:
@@ -153,6 +153,6 @@ def test_native_entries_check_their_arguments():
     assert lib.tccl_expert_slots(64, 4, 2, 1025, 0, 64, 64, 64, 0, 0) == 1
     assert lib.tccl_expert_slots(64, 1 << 30, 2, 8, 0, 64, 64, 64, 0, 0) == 1
     assert lib.tccl_expert_slots(64, 1 << 16, 2, 8, 0, 64, 64, 64, 0, 0) == 1   # no workspace
-    assert lib.tccl_expert_combine(64, 16, 64, 64, 0, 0, 64, 16, 4, 8, 2, 12, 0, 0) == 1
-    assert lib.tccl_expert_combine(64, 16, 64, 64, 0, 0, 64, 16, 4, 8, 2, 16, 2, 0) == 1
+    assert lib.tccl_expert_combine(64, 16, 64, 64, 0, 0, 64, 16, 4, 8, 2, 12, 0, 0, 0) == 1
+    assert lib.tccl_expert_combine(64, 16, 64, 64, 0, 0, 64, 16, 4, 8, 2, 16, 2, 0, 0) == 1
     assert b"" != lib.tccl_last_error()

@@ -360,7 +360,9 @@ def test_expert_gemm_empty_experts_and_tokens():
 
 
 @pytest.mark.parametrize("case", [(1, 1, 1, 64, 256, 0.0), (70, 2, 4, 136, 512, 0.2),
-                                  (300, 3, 7, 256, 256, 0.0), (900, 2, 3, 512, 768, 0.0)])
+                                  (300, 3, 7, 256, 256, 0.0), (900, 2, 3, 512, 768, 0.0),
+                                  # few rows per expert: every block is an expert's last one
+                                  (150, 4, 40, 264, 1024, 0.0)])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("b_is_nk", [False, True])
 @pytest.mark.parametrize("rows", ["tokens", "slots"])
@@ -407,7 +409,8 @@ def test_expert_gemm_backward(case, dtype, b_is_nk, rows, epilogue):
             dy, err = d, err * 1.01 + (d.abs() + err) * u + 2 ** -25
         dx = dy @ w.t()
         bx = _sum_bound(dy.abs() + err, w.t(), N) + err @ w.t().abs()
-        bx = bx + (dx.abs() + bx) * u                     # slot rows are held in 16 bits
+        if rows == "slots":
+            bx = bx + (dx.abs() + bx) * u                 # the result; token rows are summed in fp32
         dw = x.t() @ dy
         bw = _sum_bound(x.t(), dy.abs() + err, b - a) + x.t().abs() @ err
         got_w = gw[e].t() if b_is_nk else gw[e]
@@ -418,7 +421,8 @@ def test_expert_gemm_backward(case, dtype, b_is_nk, rows, epilogue):
         else:
             want_x[a:b], bound_x[a:b] = dx, bx
     if rows == "tokens":
-        _within(gx, want_x, bound_x * 1.001 + want_x.abs() * u + 2 ** -25)
+        # (the bound of the fp32 products covers the sum of at most three of them)
+        _within(gx, want_x, bound_x + (want_x.abs() + bound_x) * u + 2 ** -25)
     else:
         _within(gx[:off[E]], want_x[:off[E]], bound_x[:off[E]] + 2 ** -25)
 

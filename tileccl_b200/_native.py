@@ -268,7 +268,8 @@ def _declare(lib: C.CDLL) -> None:
         "tccl_expert_gemm_scratch": [i64, i64, C.POINTER(i64), C.POINTER(i64)],
         "tccl_expert_weight_grad": [C.POINTER(ExpertWeightGrad), u64],
         "tccl_expert_gather": [u64, i64, i64, u64, u64, i64, i64, i32, u64],
-        "tccl_expert_combine": [u64, i64, u64, u64, u64, i64, u64, i64, i64, i64, i32, i32, i32, u64],
+        "tccl_expert_combine": [u64, i64, u64, u64, u64, i64, u64, i64, i64, i64, i32, i32, i32, i32,
+                                u64],
         "tccl_expert_combine_backward": [u64, i64, u64, i64, u64, u64, u64, i64, u64, i64, i64, i32,
                                          i32, i32, u64],
         "tccl_plan_tile_order": [i32, i32, i32, i32, i32, i32, C.POINTER(i32), i32],

@@ -326,7 +326,8 @@ int tccl_expert_slots(uint64_t ids, int64_t tokens, int32_t top_k, int32_t exper
                       uint64_t workspace, uint64_t stream);
 
 typedef struct TcclExpertGemm {
-  int32_t dtype, epilogue;    // epilogue: 0 none, 1 SiLU gate, 2 gradient of the SiLU gate
+  int32_t dtype, epilogue;    // epilogue: 0 none, 1 SiLU gate, 2 gradient of the SiLU
+                              // gate, 3 none, `out` in fp32
   int32_t experts, w_nk;      // w_nk: W is [experts, N, K], else [experts, K, N]
   int64_t k, n, slots;
   uint64_t offsets;           // int32[experts + 1]
@@ -355,9 +356,11 @@ int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_t stream);
 // out[s] = x[token of slot s]; rows behind the last slot are left as they are.
 int tccl_expert_gather(uint64_t x, int64_t x_ld, int64_t x_rows, uint64_t token_of_slot,
                        uint64_t out, int64_t out_ld, int64_t slots, int32_t n, uint64_t stream);
+// h_float: h is fp32, otherwise it has the type of `dtype` as `add` and `out` do.
 int tccl_expert_combine(uint64_t h, int64_t h_ld, uint64_t slot_of, uint64_t weights, uint64_t add,
                         int64_t add_ld, uint64_t out, int64_t out_ld, int64_t tokens,
-                        int64_t slots, int32_t top_k, int32_t n, int32_t dtype, uint64_t stream);
+                        int64_t slots, int32_t top_k, int32_t n, int32_t dtype, int32_t h_float,
+                        uint64_t stream);
 int tccl_expert_combine_backward(uint64_t dy, int64_t dy_ld, uint64_t h, int64_t h_ld,
                                  uint64_t slot_of, uint64_t weights, uint64_t dh, int64_t dh_ld,
                                  uint64_t dw, int64_t tokens, int64_t slots, int32_t top_k,

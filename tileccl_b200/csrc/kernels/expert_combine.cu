@@ -1,6 +1,7 @@
 // Weighted sum of a token's expert outputs and its gradient, and tokens' rows in slot order.
 //
-//   y[t] = add[t] + sum_j w[t][j] * h[slot_of[t][j]]        (choices without a slot add nothing)
+//   y[t] = add[t] + sum_j w[t][j] * h[slot_of[t][j]]        (choices without a slot add nothing;
+//                                                           h in 16 bits or in fp32)
 //   dh[slot_of[t][j]] = w[t][j] * dy[t]      dw[t][j] = <dy[t], h[slot_of[t][j]]>
 //
 // Sums run in fp32 in the order of the choices and are rounded once.
@@ -17,7 +18,7 @@ namespace {
 constexpr int kThreads = 128;
 
 struct CombineParams {
-  const uint4* h;            // [slots] rows of `n` 16-bit values
+  const uint4* h;            // [slots] rows of `n` 16-bit or fp32 values
   int64_t h_ld;              // 16-byte vectors between rows, likewise below
   const int32_t* slot_of;    // [tokens][top_k]
   const float* weights;      // [tokens][top_k] or null (all ones)
@@ -34,12 +35,13 @@ struct CombineParams {
   int32_t top_k, vecs, bf16;   // vecs: 16-byte vectors per row
 };
 
-// A thread sums kVecs vectors of a token's row, kThreads apart.  The rows of H are fetched kBatch
-// at a time: their slots first, then all of their vectors, in flight together; kBatch * kVecs is
-// 8, which is what the registers of a full SM have room for.
-template <int kBatch>
+// A thread sums kVecs pieces of eight values of a token's row, kThreads apart.  The rows of H are
+// fetched kBatch at a time: their slots first, then all of their pieces, in flight together;
+// kBatch * kVecs is 8 (4 with fp32 rows), which is what the registers of a full SM have room for.
+template <int kBatch, bool kFloatRows>
 __global__ void __launch_bounds__(kThreads) expert_combine_kernel(const CombineParams p) {
-  constexpr int kVecs = 8 / kBatch;
+  constexpr int kVecs = (kFloatRows ? 4 : 8) / kBatch;
+  constexpr int kWords = kFloatRows ? 2 : 1;               // 16-byte vectors per piece
   const int64_t t = blockIdx.x;
   const int v0 = blockIdx.y * (kThreads * kVecs) + threadIdx.x;
   const bool bf16 = p.bf16 != 0;
@@ -51,7 +53,7 @@ __global__ void __launch_bounds__(kThreads) expert_combine_kernel(const CombineP
   for (int j0 = 0; j0 < p.top_k; j0 += kBatch) {
     int32_t s[kBatch];
     float w[kBatch];
-    uint4 x[kBatch][kVecs];
+    uint4 x[kBatch][kVecs][kWords];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       s[j] = j0 + j < p.top_k ? p.slot_of[t * p.top_k + j0 + j] : -1;
@@ -62,15 +64,28 @@ __global__ void __launch_bounds__(kThreads) expert_combine_kernel(const CombineP
     for (int j = 0; j < kBatch; ++j)
 #pragma unroll
       for (int c = 0; c < kVecs; ++c)
-        if (s[j] >= 0 && v0 + c * kThreads < p.vecs)
-          x[j][c] = ld_stream_v4(p.h + s[j] * p.h_ld + v0 + c * kThreads);
+        if (s[j] >= 0 && v0 + c * kThreads < p.vecs) {
+          const uint4* src = p.h + s[j] * p.h_ld + (v0 + c * kThreads) * kWords;
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) x[j][c][i] = ld_stream_v4(src + i);
+        }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
       if (s[j] >= 0) {
 #pragma unroll
         for (int c = 0; c < kVecs; ++c) {
           float f[8] = {};
-          tile_accumulate_16x8(bf16, f, x[j][c]);
+          if (kFloatRows) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              f[4 * i] = __uint_as_float(x[j][c][i].x);
+              f[4 * i + 1] = __uint_as_float(x[j][c][i].y);
+              f[4 * i + 2] = __uint_as_float(x[j][c][i].z);
+              f[4 * i + 3] = __uint_as_float(x[j][c][i].w);
+            }
+          } else {
+            tile_accumulate_16x8(bf16, f, x[j][c][0]);
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) acc[c][i] = fmaf(w[j], f[i], acc[c][i]);
         }
@@ -172,7 +187,7 @@ int check(const CombineParams& p) {
 
 cudaError_t preload_expert_combine_kernels() {
   cudaFuncAttributes a;
-  cudaError_t e = cudaFuncGetAttributes(&a, expert_combine_kernel<8>);
+  cudaError_t e = cudaFuncGetAttributes(&a, expert_combine_kernel<8, false>);
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_combine_backward_kernel<8>);
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_gather_kernel);
   return e;
@@ -185,14 +200,14 @@ using namespace tileccl;
 extern "C" int tccl_expert_combine(uint64_t h, int64_t h_ld, uint64_t slot_of, uint64_t weights,
                                    uint64_t add, int64_t add_ld, uint64_t out, int64_t out_ld,
                                    int64_t tokens, int64_t slots, int32_t top_k, int32_t n,
-                                   int32_t dtype, uint64_t stream) {
+                                   int32_t dtype, int32_t h_float, uint64_t stream) {
   TCCL_CHECK_ARG(dtype == 0 || dtype == 1, "dtype must be 0 (fp16) or 1 (bf16)");
   TCCL_CHECK_ARG(n % 8 == 0 && h_ld % 8 == 0 && add_ld % 8 == 0 && out_ld % 8 == 0,
                  "row lengths and pitches must be multiples of 8 elements");
   TCCL_CHECK_ARG(h % 16 == 0 && add % 16 == 0 && out % 16 == 0, "rows must be 16-byte aligned");
   CombineParams p = {};
   p.h = reinterpret_cast<const uint4*>(h);
-  p.h_ld = h_ld / 8;
+  p.h_ld = h_float ? h_ld / 4 : h_ld / 8;
   p.slot_of = reinterpret_cast<const int32_t*>(slot_of);
   p.weights = reinterpret_cast<const float*>(weights);
   p.add = reinterpret_cast<const uint4*>(add);
@@ -209,13 +224,19 @@ extern "C" int tccl_expert_combine(uint64_t h, int64_t h_ld, uint64_t slot_of, u
   if (tokens == 0) return kOk;
   TCCL_CHECK_ARG(h != 0 && slot_of != 0 && out != 0, "null argument");
   // (few tokens: narrow pieces, so that a row is spread over more SMs)
-  const int batch = top_k > 4 || tokens < 256 ? 8 : top_k > 2 ? 4 : 2;
-  const int piece = kThreads * (8 / batch);
+  const int most = h_float ? 4 : 8;
+  const int batch = tokens < 256 || top_k > most / 2 ? most : top_k > 2 ? 4 : 2;
+  const int piece = kThreads * (most / batch);
   const dim3 grid(static_cast<unsigned>(tokens), (p.vecs + piece - 1) / piece);
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  if (batch == 8) expert_combine_kernel<8><<<grid, kThreads, 0, cs>>>(p);
-  else if (batch == 4) expert_combine_kernel<4><<<grid, kThreads, 0, cs>>>(p);
-  else expert_combine_kernel<2><<<grid, kThreads, 0, cs>>>(p);
+  if (h_float) {
+    if (batch == 4) expert_combine_kernel<4, true><<<grid, kThreads, 0, cs>>>(p);
+    else expert_combine_kernel<2, true><<<grid, kThreads, 0, cs>>>(p);
+  } else {
+    if (batch == 8) expert_combine_kernel<8, false><<<grid, kThreads, 0, cs>>>(p);
+    else if (batch == 4) expert_combine_kernel<4, false><<<grid, kThreads, 0, cs>>>(p);
+    else expert_combine_kernel<2, false><<<grid, kThreads, 0, cs>>>(p);
+  }
   TCCL_CHECK_CUDA(cudaGetLastError());
   return kOk;
 }

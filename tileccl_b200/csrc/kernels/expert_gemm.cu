@@ -7,6 +7,7 @@
 //   gradient of the gate: gate and up are computed again and with dh[s] = dL/dout[s]
 //              dgate = dh * up * sg * (1 + gate * (1 - sg)),  dup = dh * gate * sg,
 //              sg = 1 / (1 + e^-gate), packed like W's columns
+//   out in fp32: for sums over a token's slots that are rounded once at their end
 //   dW[e] = sum over the slots s of e of a[s]^T b[s]
 //
 // Both kernels are persistent: a cluster of two CTAs per tile, tcgen05.mma.cta_group::2, a TMA
@@ -23,7 +24,7 @@
 namespace tileccl {
 namespace {
 
-enum Epilogue : int { kNone = 0, kSiluGate = 1, kSiluGateGrad = 2 };
+enum Epilogue : int { kNone = 0, kSiluGate = 1, kSiluGateGrad = 2, kFloat = 3 };
 
 constexpr int kMaxExperts = 1024;
 constexpr int kThreads = 256;            // warp 0 TMA, 1 MMA, 2 TMEM, 3 idle, 4-7 epilogue
@@ -149,7 +150,7 @@ __device__ __forceinline__ Pipe make_pipe(uint8_t* raw, int staging_bytes) {
   s.full = s.ctl;
   s.empty = s.full + 8 * kStages;
   s.tail = s.empty + 8 * kStages;
-  s.acc_full = s.tail + 8;
+  s.acc_full = s.tail + 8 * kStages;
   s.acc_empty = s.acc_full + 16;
   s.drain = s.acc_empty + 16;
   s.tmem_slot = s.drain + 8;
@@ -167,12 +168,12 @@ __device__ __forceinline__ uint32_t pipe_start(const Pipe& s) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(s.full + 8 * i, 1);
       mbar_init(s.empty + 8 * i, 1);
+      mbar_init(s.tail + 8 * i, 2);          // the copying warps of both CTAs
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s.acc_full + 8 * i, 1);
       mbar_init(s.acc_empty + 8 * i, 8);     // four epilogue warps of both CTAs
     }
-    mbar_init(s.tail, 2);                    // the copying warps of both CTAs
     mbar_init(s.drain, 1);
     s.words[1] = 0;
     mbar_fence_init();
@@ -399,7 +400,8 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
           if (leader) mbar_expect_tx(s.full + 8 * stage, 2 * (kOperandBytes + mine * 128));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int f = kEpi == kNone ? it.f0 + cta * 128 + h * 64 : it.f0 + h * 128 + cta * 64;
+            const int f = kEpi == kNone || kEpi == kFloat ? it.f0 + cta * 128 + h * 64
+                                                          : it.f0 + h * 128 + cta * 64;
             if (p.w_nk) tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, kb * kBK, f, it.e, bar);
             else tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, f, kb * kBK, it.e, bar);
           }
@@ -469,7 +471,8 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
     const int q = warp - 4, me = threadIdx.x - 128;
     float* const staging = reinterpret_cast<float*>(smem_raw + (s.staging - smem_u32(smem_raw)));
     const bool bf16 = p.bf16 != 0;
-    constexpr int kVecs = kEpi == kNone ? 16 : 8;          // 8-feature vectors per token
+    constexpr bool kPlain = kEpi == kNone || kEpi == kFloat;
+    constexpr int kVecs = kPlain ? 16 : 8;                 // 8-feature vectors per token
     uint32_t acc = 0, acc_phase = 0, buf = 0;
     while (advance(w, it)) {
       if (!epilogue_all(mbar_wait(s.acc_full + 8 * acc, acc_phase, wb))) {
@@ -561,9 +564,16 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
           const float4* src = reinterpret_cast<const float4*>(sbuf + tok * kStageLd + vec * 8);
           *reinterpret_cast<float4*>(a) = src[0];
           *reinterpret_cast<float4*>(a + 4) = src[1];
-          if (kEpi == kNone) {
+          if (kPlain) {
             const int f = it.f0 + cta * 128 + vec * 8;
-            if (f < p.n) store_row8(p.out, slot * p.ldo + f, bf16, a);
+            if (f >= p.n) continue;
+            if (kEpi == kNone) {
+              store_row8(p.out, slot * p.ldo + f, bf16, a);
+            } else {
+              float4* const dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + slot * p.ldo + f);
+              dst[0] = *reinterpret_cast<const float4*>(a);
+              dst[1] = *reinterpret_cast<const float4*>(a + 4);
+            }
             continue;
           }
           float u[8];
@@ -656,7 +666,8 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
     // ----------------------- MMA issuer (leader CTA only) -----------------------
     if (elect_one_sync()) {
       const uint32_t idesc = umma_idesc_f16(p.bf16, 1, 1, kTile, kTile);
-      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, tail_phase = 0;
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      uint32_t tail_phases = 0;           // one bit per stage: copied blocks use it now and then
       bool ok = true;
       for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
         const int e = t / per_expert;
@@ -673,8 +684,8 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
         for (int kb = 0; kb < blocks; ++kb) {
           bool full = mbar_wait(s.full + 8 * stage, phase, wb);
           if (full && kb * kBK + kBK > rows) {           // the copied block
-            full = wait_cluster(s.tail, tail_phase, wb);
-            tail_phase ^= 1u;
+            full = wait_cluster(s.tail + 8 * stage, (tail_phases >> stage) & 1u, wb);
+            tail_phases ^= 1u << stage;
           }
           if (!full) {
             report_status(p.status, kStatusTimeoutMbarrier, 113, blocks, kb, 0, t);
@@ -705,7 +716,9 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
     // ------------- copying warps: the partial block at the end of an expert -------------
     // Thread c copies 16-byte chunk c % 8 of one half of the columns (c / 8 % 2) of the rows
     // c / 16, c / 16 + 8, ... of both operands.  The arrival at the other CTA is a release at
-    // cluster scope, about a microsecond; it comes once per tile and runs ahead of the MMAs.
+    // cluster scope, about a microsecond; it comes once per tile and runs ahead of the MMAs.  It
+    // goes to a barrier of the stage: experts with few rows have copied blocks in several stages
+    // at a time, and the stage's own use keeps the phases of its barrier apart.
     const int c = threadIdx.x - kThreads, chunk = c & 7, h = (c >> 3) & 1, row = c >> 4;
     const uint32_t dst = h * kHalfBytes + row * 128 + ((chunk ^ row) << 4);
     uint32_t stage = 0, phase = 0;
@@ -735,7 +748,7 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
           copy_wait_all();
           fence_proxy_async_smem();
           copiers_all(true);
-          if (c == 0) mbar_arrive_cluster(mapa_shared(s.tail, 0));
+          if (c == 0) mbar_arrive_cluster(mapa_shared(s.tail + 8 * stage, 0));
         }
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
@@ -832,9 +845,10 @@ int encode(CUtensorMap* map, bool bf16, uint64_t base, uint64_t cols, uint64_t r
 
 using GemmKernel = void (*)(const GemmParams);
 GemmKernel gemm_kernel(int epilogue) {
-  return epilogue == kNone       ? expert_gemm_kernel<kNone>
-         : epilogue == kSiluGate ? expert_gemm_kernel<kSiluGate>
-                                 : expert_gemm_kernel<kSiluGateGrad>;
+  return epilogue == kNone           ? expert_gemm_kernel<kNone>
+         : epilogue == kSiluGate     ? expert_gemm_kernel<kSiluGate>
+         : epilogue == kSiluGateGrad ? expert_gemm_kernel<kSiluGateGrad>
+                                     : expert_gemm_kernel<kFloat>;
 }
 
 cudaError_t attrs_once(int* sms) {
@@ -844,7 +858,7 @@ cudaError_t attrs_once(int* sms) {
   if (e != cudaSuccess) return e;
   if (dev < 64 && count[dev] != 0) { *sms = count[dev]; return cudaSuccess; }
   e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
-  for (int i = 0; i < 3 && e == cudaSuccess; ++i)
+  for (int i = 0; i < 4 && e == cudaSuccess; ++i)
     e = cudaFuncSetAttribute(gemm_kernel(i),
                              cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
   if (e == cudaSuccess)
@@ -888,7 +902,7 @@ cudaError_t preload_expert_gemm_kernels() {
   cudaFuncAttributes a;
   int sms = 0;
   cudaError_t e = cudaFuncGetAttributes(&a, expert_weight_grad_kernel);
-  for (int i = 0; i < 3 && e == cudaSuccess; ++i) e = cudaFuncGetAttributes(&a, gemm_kernel(i));
+  for (int i = 0; i < 4 && e == cudaSuccess; ++i) e = cudaFuncGetAttributes(&a, gemm_kernel(i));
   if (e == cudaSuccess) e = attrs_once(&sms);
   return e;
 }
@@ -918,7 +932,7 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   TCCL_CHECK_ARG(desc != nullptr, "null argument");
   const TcclExpertGemm& d = *desc;
   TCCL_CHECK_ARG(d.dtype == 0 || d.dtype == 1, "dtype must be 0 (fp16) or 1 (bf16)");
-  TCCL_CHECK_ARG(d.epilogue >= kNone && d.epilogue <= kSiluGateGrad, "epilogue must be 0..2");
+  TCCL_CHECK_ARG(d.epilogue >= kNone && d.epilogue <= kFloat, "epilogue must be 0..3");
   TCCL_CHECK_ARG(d.experts >= 1 && d.experts <= kMaxExperts, "experts must be 1..1024");
   TCCL_CHECK_ARG(d.k >= 1 && d.n >= 1 && d.k < (int64_t(1) << 31) && d.n < (int64_t(1) << 31) - kTile,
                  "K and N must be 1..2^31");
@@ -929,7 +943,7 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
                  "leading dimensions must be multiples of 8 elements");
   TCCL_CHECK_ARG(d.x % 16 == 0 && d.w % 16 == 0 && d.out % 16 == 0 && d.dh % 16 == 0,
                  "operands must be 16-byte aligned");
-  TCCL_CHECK_ARG(d.epilogue == kNone || d.n % 256 == 0,
+  TCCL_CHECK_ARG(d.epilogue == kNone || d.epilogue == kFloat || d.n % 256 == 0,
                  "SiLU-gate epilogue needs N to be a multiple of 256");
   TCCL_CHECK_ARG(d.slots >= 0 && d.slots < (int64_t(1) << 31) - kTile, "too many rows");
   if (d.slots == 0) return kOk;
