@@ -93,7 +93,10 @@ def test_slot_refusals():
     (dict(X=torch.zeros(4, 12).half(), W=torch.zeros(3, 12, 24).half()), ValueError),
     (dict(W=torch.zeros(3, 16, 20).half()), ValueError),
     (dict(out=torch.zeros(8, 23).half()), ValueError),
-    (dict(out=torch.zeros(8, 24)), TypeError),
+    (dict(out=torch.zeros(8, 24).double()), TypeError),
+    (dict(out=torch.zeros(8, 24), out_dtype=torch.float16), TypeError),
+    (dict(out_dtype=torch.bfloat16), TypeError),
+    (dict(W=torch.zeros(3, 16, 256).half(), epilogue="silu_gate", out_dtype=torch.float32), TypeError),
     (dict(out=torch.zeros(8, 28).half()[:, :24]), ValueError),   # rows not 16-byte aligned
     (dict(slots=None), ValueError),
     (dict(), ValueError),                                        # right, but on the CPU
@@ -156,3 +159,21 @@ def test_native_entries_check_their_arguments():
     assert lib.tccl_expert_combine(64, 16, 64, 64, 0, 0, 64, 16, 4, 8, 2, 12, 0, 0, 0) == 1
     assert lib.tccl_expert_combine(64, 16, 64, 64, 0, 0, 64, 16, 4, 8, 2, 16, 2, 0, 0) == 1
     assert b"" != lib.tccl_last_error()
+
+
+class _Rank:
+    """What a block reads of a context before it allocates anything."""
+
+    def __init__(self, rank=0, world_size=2):
+        self.rank, self.world_size = rank, world_size
+
+
+@pytest.mark.parametrize("change", [dict(tokens=7), dict(ffn=257), dict(ffn=384), dict(hidden=60),
+                                    dict(experts=6), dict(top_k=0), dict(top_k=9)])
+def test_moe_block_refusals(change):
+    from tileccl_b200.models import TPMoE
+
+    args = dict(tokens=8, hidden=64, ffn=512, experts=8, top_k=2)
+    args.update(change)
+    with pytest.raises(ValueError):
+        TPMoE(_Rank(), **args)

@@ -654,3 +654,60 @@ def test_route_decides_crowded_rows_exactly(score, groups, top_groups):
         got_k, want_k = key.gather(1, ids.long()), key.gather(1, want.long())
         assert ((got_k - want_k).abs() <= 2 ** -50)[~same].all()
         assert same.float().mean() > 0.99
+
+
+def test_expert_gemm_fp32_result():
+    from tileccl_b200 import ops
+
+    g = _gen(31)
+    T, E, K, N = 300, 3, 136, 72
+    slots = _make_slots(g, T, 2, E)
+    X, W = _randn(g, T, K, dtype=torch.bfloat16), _randn(g, E, K, N, dtype=torch.bfloat16)
+    big = torch.full((2 * T, N + 8), 3.0, device="cuda")
+    out = big[:, 4:4 + N]
+    got = ops.expert_gemm(X, W, slots, out)               # (the type of `out` counts)
+    again = ops.expert_gemm(X, W, slots, out_dtype=torch.float32)
+    assert got is out and torch.equal(again, out) and (big[:, :4] == 3).all() and (big[:, 4 + N:] == 3).all()
+    off, tok = slots.offsets.tolist(), slots.token_of_slot.long()
+    for e in range(E):
+        x = X[tok[off[e]:off[e + 1]]].double()
+        _within(out[off[e]:off[e + 1]], x @ W[e].double(), _sum_bound(x, W[e].double(), K))
+
+
+@pytest.mark.parametrize("ws", [1, 2, 4])
+def test_tp_moe_matches_fp32_reference(ws):
+    import tileccl_b200 as tccl
+    from tileccl_b200.models.tp_moe import smoke_moe_forward
+
+    ctxs = tccl.init_local(ws, 256 << 20)
+    try:
+        smoke_moe_forward(ctxs)
+        smoke_moe_forward(ctxs, tokens=ws, experts=16, top_k=3)       # one token per rank
+    finally:
+        for d in range(torch.cuda.device_count()):
+            torch.cuda.synchronize(d)
+        for c in ctxs:
+            c.heap.cleanup()
+
+
+def test_tp_moe_in_a_graph():
+    import tileccl_b200 as tccl
+    from tileccl_b200.models import TPMoE
+
+    ctx = tccl.init_local(1, 64 << 20)[0]
+    try:
+        moe = TPMoE(ctx, tokens=48, hidden=256, ffn=512, experts=8, top_k=2, balance=True, groups=4,
+                    top_groups=2, score="sigmoid")
+        xs = [_randn(_gen(i), 48, 256, dtype=torch.bfloat16) for i in range(3)]
+        want = [moe(x).clone() for x in xs]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            moe.forward()
+        for x, y in zip(xs, want):
+            moe.x_local.copy_(x)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(moe.y, y)
+    finally:
+        torch.cuda.synchronize()
+        ctx.heap.cleanup()

@@ -343,8 +343,8 @@ def _check_product(X, W, slots, rows, b_is_nk, epilogue):
     return E, K, N, epi
 
 
-def _check_rows(name, t, shape, like):
-    _check_tensor(name, t, 2, (like.dtype,), like.device)
+def _check_rows(name, t, shape, like, dtype=None):
+    _check_tensor(name, t, 2, (dtype or like.dtype,), like.device)
     if tuple(t.shape) != shape:
         raise ValueError(f"{name} is {tuple(t.shape)}, expected {shape}")
     return _aligned(name, t)
@@ -416,6 +416,7 @@ def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
 def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
                 out: Optional[torch.Tensor] = None, *, rows: str = "tokens",
                 b_is_nk: bool = False, epilogue: str = "none",
+                out_dtype: Optional[torch.dtype] = None,
                 stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """``out[s] = X[row of slot s] @ W[expert of slot s]`` (fp16 / bf16, fp32 accumulation).
 
@@ -424,15 +425,24 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
     K]`` with ``b_is_nk``.  ``epilogue="silu_gate"`` takes every 256 columns of the product as
     128 gate columns followed by 128 up columns (``models.pack_gate_up`` of every expert) and
     writes ``silu(gate) * up``, half as wide.  Rows of ``out [tokens * top_k, N]`` behind the
-    last slot keep what they held.  ``out`` must not overlap an input.
+    last slot keep what they held.  ``out`` must not overlap an input.  ``out_dtype``:
+    ``X.dtype`` (default, or that of ``out``) or, without the gate, ``torch.float32``.
     """
     E, K, N, epi = _check_product(X, W, slots, rows, b_is_nk, epilogue)
     shape = (slots.capacity, N // 2 if epi else N)
+    if out_dtype is None:
+        out_dtype = X.dtype if out is None else out.dtype
+    if out_dtype not in (X.dtype, torch.float32):
+        raise TypeError(f"out_dtype must be {X.dtype} or torch.float32, got {out_dtype}")
+    if out_dtype == torch.float32:
+        if epi:
+            raise TypeError("epilogue 'silu_gate' writes the operands' dtype")
+        epi = _EPI_FLOAT
     if out is not None:
-        _check_rows("out", out, shape, X)
+        _check_rows("out", out, shape, X, out_dtype)
     with _On(stream, (X, W, slots.offsets, slots.token_of_slot, out)) as raw:
         if out is None:
-            out = torch.empty(shape, dtype=X.dtype, device=X.device)
+            out = torch.empty(shape, dtype=out_dtype, device=X.device)
         # Tokens' rows are put in slot order by a copy kernel first.  (The product gathering them
         # itself, with the TMA unit's four rows per copy or through the threads, measured slower at
         # every size: 209 against 200 us for 8 tokens, 8.1 against 2.5 ms for 8192.)

@@ -126,12 +126,16 @@ def describe_runtime_support(ctx: Any = None) -> RuntimeSupportMatrix:
 
     fused = gate(True, "fused tcgen05 GEMM + collective")
     coll = gate(True, "tile collective kernel")
+    moe = gate(False, "mixture-of-experts kernel")
     ops = {
         "gemm_allscatter": fused, "gemm_allscatter_sharded": fused, "gemm_allgather": fused,
         "gemm_allgather_rows": fused, "gemm_reducescatter": fused, "gemm_reducescatter_rows": fused,
         "allgather_gemm_reducescatter": fused, "allgather": coll, "allreduce": coll,
         "reduce_scatter": coll, "broadcast": coll, "scatter": coll,
         "models.TPMLP": fused,
+        "route_experts": moe, "route_experts_backward": moe, "expert_slots": moe,
+        "expert_gemm": moe, "expert_gemm_backward": moe, "expert_combine": moe,
+        "expert_combine_backward": moe, "models.TPMoE": coll,
     }
     contracts = {
         "gemm_allscatter.full/full": fused,
