@@ -275,6 +275,10 @@ PRODUCT_CASES = [
     (200, 2, 3, 320, 768, 0.0),
     (700, 3, 5, 1024, 512, 0.1),
     (1100, 1, 2, 512, 1024, 0.0),
+    # long contractions of few rows: tiles shared among the SMs
+    (1, 2, 8, 4096, 768, 0.0),
+    (5, 2, 8, 4168, 1280, 0.2),
+    (60, 2, 3, 4096, 256, 0.0),
 ]
 
 
@@ -711,3 +715,58 @@ def test_tp_moe_in_a_graph():
     finally:
         torch.cuda.synchronize()
         ctx.heap.cleanup()
+
+
+def test_shared_tiles_repeat_in_graphs_and_beside_each_other():
+    """Products whose tiles are shared (few rows, long contraction) leave their counters as they
+    found them: repeated, captured twice, replayed beside one another and beside eager calls."""
+    from tileccl_b200 import ops
+
+    g = _gen(41)
+    dtype, T, E, K, N = torch.bfloat16, 3, 8, 4608, 512
+    W = _randn(g, E, K, N, std=K ** -0.5, dtype=dtype)
+    data = [(_randn(g, T, K, dtype=dtype), _make_slots(g, T, 2, E)) for _ in range(3)]
+    want = [ops.expert_gemm(x, W, s).clone() for x, s in data]
+    graphs = []
+    for x, s in data[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [ops.expert_gemm(x, W, s) for _ in range(3)]
+        graphs.append((graph, outs))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = [ops.expert_gemm(*[data[2][0], W, data[2][1]], stream=streams[2]) for _ in range(3)]
+        torch.cuda.synchronize()
+        for (_, outs), y in zip(graphs, want):
+            assert all(torch.equal(o, y) for o in outs)
+        assert all(torch.equal(o, want[2]) for o in eager)
+    ops.check_expert_status()
+
+
+def test_counters_run_out(monkeypatch):
+    """Captured products beyond the prepared counters zero their own."""
+    from tileccl_b200 import ops
+    from tileccl_b200.kernels import experts
+
+    g = _gen(43)
+    x, W = _randn(g, 2, 4096, dtype=torch.float16), _randn(g, 4, 4096, 256, std=1 / 64, dtype=torch.float16)
+    slots = _make_slots(g, 2, 2, 4)
+    want = ops.expert_gemm(x, W, slots).clone()
+    arena = experts._ARENAS[x.device.index]
+    monkeypatch.setattr(arena, "used", arena.BYTES)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [ops.expert_gemm(x, W, slots) for _ in range(2)]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+    stream = torch.cuda.Stream()                          # a stream that has no piece yet
+    stream.wait_stream(torch.cuda.current_stream())
+    got = ops.expert_gemm(x, W, slots, stream=stream)
+    stream.synchronize()
+    assert torch.equal(got, want)

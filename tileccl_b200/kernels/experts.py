@@ -147,8 +147,8 @@ def check_expert_status(device=None) -> None:
     t = _STATUS.get(torch.cuda.current_device() if dev.index is None else dev.index)
     if t is not None:
         torch.cuda.synchronize(t.device)
-        if int(t[0]) != 0:
-            _COUNTERS.clear()             # (an abandoned call may have left some above zero)
+        if int(t[0]) != 0 and t.device.index in _ARENAS:
+            _ARENAS[t.device.index].words.zero_()     # (an abandoned call may have left some behind)
         _fg.raise_on_status(t)
 
 
@@ -203,8 +203,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
             raise ValueError(f"mask has {mask.shape[0]} entries for {tokens} tokens")
     ld = _pitch("logits", logits)
     with _On(stream, (logits, bias, mask)) as raw:
-        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((tokens, top_k), dtype=torch.int32, device=logits.device)
+        weights = logits.new_empty((tokens, top_k), dtype=torch.float32)
+        ids = logits.new_empty((tokens, top_k), dtype=torch.int32)
         _launch("tccl_expert_route", logits.data_ptr(), ld, _ptr(bias), _ptr(mask),
                 weights.data_ptr(), ids.data_ptr(), tokens, experts, top_k,
                 _LOGIT_DTYPES[logits.dtype], sig, groups, top_groups, by_max,
@@ -229,7 +229,7 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids
                          f"must both be {(tokens, top_k)}")
     ld = _pitch("logits", logits)
     with _On(stream, (logits, ids, grad_weights)) as raw:
-        grad = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
+        grad = logits.new_empty((tokens, experts))
         _launch("tccl_expert_route_backward", grad_weights.data_ptr(), logits.data_ptr(), ld,
                 ids.data_ptr(), grad.data_ptr(), tokens, experts, top_k,
                 _LOGIT_DTYPES[logits.dtype], sig, 1 if renormalize else 0, scale, raw)
@@ -305,8 +305,8 @@ def expert_slots(ids: torch.Tensor, num_experts: int, *, first_expert: int = 0,
         n = tokens * top_k
         need = _slots_scratch(n, num_experts)
         # one allocation for the three parts
-        slot_of, token_of_slot, offsets = torch.empty(
-            2 * n + num_experts + 1, dtype=torch.int32, device=dev).split((n, n, num_experts + 1))
+        slot_of, token_of_slot, offsets = ids.new_empty(
+            2 * n + num_experts + 1).split((n, n, num_experts + 1))
         slot_of = slot_of.view(tokens, top_k)
         scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _launch("tccl_expert_slots", ids.data_ptr(), tokens, top_k, num_experts, first_expert,
@@ -360,7 +360,7 @@ def _aligned(name, t) -> int:
 def _gather(X, slots, raw):
     """``X``'s rows in slot order."""
     S, K = slots.capacity, X.shape[1]
-    xs = torch.empty((S, K), dtype=X.dtype, device=X.device)
+    xs = X.new_empty((S, K))
     _launch("tccl_expert_gather", X.data_ptr(), _aligned("X", X), X.shape[0],
             slots.token_of_slot.data_ptr(), xs.data_ptr(), K, S, K, raw)
     return xs
@@ -373,20 +373,58 @@ def _scratch_sizes(device: int, slots: int, k: int) -> tuple:
     return a.value, b.value
 
 
-_COUNTERS: dict = {}
+class _CounterArena:
+    """Zeroed arrival counters of one device's products.  Every call leaves its counters at zero.
+    Calls on one stream follow one another and share a piece; a captured call gets a piece of its
+    own for good, because its graph may be replayed beside anything else."""
+
+    BYTES = 1 << 20                       # some 800 pieces
+
+    def __init__(self, dev):
+        self.words = torch.zeros(self.BYTES, dtype=torch.uint8, device=dev)
+        torch.cuda.current_stream(dev).synchronize()      # (once: other streams use it, too)
+        self.used, self.by_stream = 0, {}
+
+    def take(self, nbytes: int) -> int:
+        """Address of a new piece, 0 when none is left."""
+        at = self.used
+        if at + nbytes > self.BYTES:
+            return 0
+        self.used = at + -(-nbytes // 128) * 128
+        return self.words.data_ptr() + at
+
+
+_ARENAS: dict = {}
 
 
 def _counters(dev, raw, nbytes):
-    """Zeroed arrival counters of a product.  Calls on one stream follow one another and leave
-    the counters at zero, so a stream's are kept; a captured call gets its own, because its graph
-    may be replayed beside anything else."""
+    """(address, tensor to keep until the launch) of zeroed counters for one product."""
+    arena = _ARENAS.get(dev.index)
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-    key = (dev.index, raw)
-    t = _COUNTERS.get(key)
-    if t is None:
-        t = _COUNTERS[key] = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-    return t
+        address = arena.take(nbytes) if arena is not None else 0
+        if address:
+            return address, None
+        t = torch.zeros(nbytes, dtype=torch.uint8, device=dev)      # zeroed by the graph itself
+        return t.data_ptr(), t
+    if arena is None:
+        arena = _ARENAS[dev.index] = _CounterArena(dev)
+    address = arena.by_stream.get(raw)
+    if address is None:
+        address = arena.take(nbytes)
+        if not address:
+            t = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+            return t.data_ptr(), t
+        arena.by_stream[raw] = address
+    return address, None
+
+
+def _gather(X, slots, raw):
+    """``X``'s rows in slot order."""
+    S, K = slots.capacity, X.shape[1]
+    xs = X.new_empty((S, K))
+    _launch("tccl_expert_gather", X.data_ptr(), _aligned("X", X), X.shape[0],
+            slots.token_of_slot.data_ptr(), xs.data_ptr(), K, S, K, raw)
+    return xs
 
 
 def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
@@ -408,8 +446,8 @@ def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
     partial = None
     if partial_bytes:
         partial = torch.empty(partial_bytes, dtype=torch.uint8, device=X.device)
-        counters = _counters(X.device, raw, counter_bytes)
-        d.partial, d.counters = partial.data_ptr(), counters.data_ptr()
+        d.counters, keep = _counters(X.device, raw, counter_bytes)
+        d.partial = partial.data_ptr()
     _launch("tccl_expert_gemm", C.byref(d), raw)
 
 
@@ -442,7 +480,7 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
         _check_rows("out", out, shape, X, out_dtype)
     with _On(stream, (X, W, slots.offsets, slots.token_of_slot, out)) as raw:
         if out is None:
-            out = torch.empty(shape, dtype=out_dtype, device=X.device)
+            out = X.new_empty(shape, dtype=out_dtype)
         # Tokens' rows are put in slot order by a copy kernel first.  (The product gathering them
         # itself, with the TMA unit's four rows per copy or through the threads, measured slower at
         # every size: 209 against 200 us for 8 tokens, 8.1 against 2.5 ms for 8192.)
@@ -472,18 +510,17 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
         if epi:
             # gate and up again, their gradients straight from the accumulators (one rounding
             # to 16 bits: the operand type of the two products that follow)
-            dy = torch.empty((S, N), dtype=X.dtype, device=X.device)
+            dy = X.new_empty((S, N))
             _product(xs, W, slots, dy, b_is_nk, _EPI_SILU_GATE_GRAD, grad_out, raw)
         # A token's slots are summed in fp32 and rounded once: with 16-bit rows in between the
         # error grew by a quarter, the call is 3 % faster.
-        grad_rows = torch.empty((S, K), dtype=torch.float32 if rows == "tokens" else X.dtype,
-                                device=X.device)
+        grad_rows = X.new_empty((S, K), dtype=torch.float32 if rows == "tokens" else X.dtype)
         _product(dy, W, slots, grad_rows, not b_is_nk, _EPI_FLOAT if rows == "tokens" else 0, None, raw)
         grad_X = grad_rows
         if rows == "tokens":
-            grad_X = torch.empty((slots.tokens, K), dtype=X.dtype, device=X.device)
+            grad_X = X.new_empty((slots.tokens, K))
             _combine(grad_rows, slots, None, None, grad_X, raw)
-        grad_W = torch.empty(W.shape, dtype=X.dtype, device=X.device)
+        grad_W = X.new_empty(W.shape)
         a, b = (dy, xs) if b_is_nk else (xs, dy)
         d = _native.ExpertWeightGrad()
         d.dtype, d.experts, d.slots = _fg.dtype_code(X.dtype), E, S
@@ -538,7 +575,7 @@ def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.
         _check_rows("out", out, shape, H)
     with _On(stream, (H, weights, add, slots.slot_of, out)) as raw:
         if out is None:
-            out = torch.empty(shape, dtype=H.dtype, device=H.device)
+            out = H.new_empty(shape)
         _combine(H, slots, weights, add, out, raw)
     return out
 
@@ -554,8 +591,8 @@ def expert_combine_backward(grad_out: torch.Tensor, H: torch.Tensor, slots: Expe
     _check_combine(H, slots, weights)
     _check_rows("grad_out", grad_out, (slots.tokens, H.shape[1]), H)
     with _On(stream, (H, weights, grad_out, slots.slot_of)) as raw:
-        grad_H = torch.empty(H.shape, dtype=H.dtype, device=H.device)
-        grad_weights = torch.empty(weights.shape, dtype=torch.float32, device=H.device)
+        grad_H = H.new_empty(H.shape)
+        grad_weights = weights.new_empty(weights.shape)
         _launch("tccl_expert_combine_backward", grad_out.data_ptr(), _aligned("grad_out", grad_out),
                 H.data_ptr(), _aligned("H", H), slots.slot_of.data_ptr(), weights.data_ptr(),
                 grad_H.data_ptr(), _aligned("grad_H", grad_H), grad_weights.data_ptr(),
