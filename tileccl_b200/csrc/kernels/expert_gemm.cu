@@ -161,9 +161,10 @@ __device__ __forceinline__ Pipe make_pipe(uint8_t* raw, int staging_bytes) {
   return s;
 }
 
-// Barriers and TMEM of a CTA pair; returns the TMEM base.  Ends in a barrier of the pair, so
-// what a thread wrote to shared memory before is visible to its CTA afterwards.
-__device__ __forceinline__ uint32_t pipe_start(const Pipe& s) {
+// Barriers and TMEM of a CTA pair: `pipe_start` sets them up, `pipe_meet` returns the TMEM base
+// once both CTAs have; what a thread wrote to shared memory in between is visible to its CTA
+// afterwards.
+__device__ __forceinline__ void pipe_start(const Pipe& s) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(s.full + 8 * i, 1);
@@ -182,6 +183,8 @@ __device__ __forceinline__ uint32_t pipe_start(const Pipe& s) {
     tmem_alloc_pair(s.tmem_slot, 2 * kAccCols);
     tmem_relinquish_pair();
   }
+}
+__device__ __forceinline__ uint32_t pipe_meet(const Pipe& s) {
   tcgen05_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -193,22 +196,28 @@ __device__ __forceinline__ int slot_bound(const int32_t* offsets, int e, int slo
   return min(max(offsets[e], 0), slots);
 }
 
-// The list of tiles: expert e has tiles_of(rows of e) of them.  The counts per expert live on
-// the GPU only, so every CTA derives the whole schedule from the offsets.
+// `pipe_start` and the list of tiles: expert e has tiles_of(rows of e) of them.  The counts per
+// expert live on the GPU only, so every CTA derives the whole schedule from the offsets.
 template <typename F>
 __device__ __forceinline__ void list_tiles(const Pipe& s, const int32_t* offsets, int slots,
                                            int experts, F tiles_of) {
   __shared__ int32_t warp_sum[kThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kPer = kMaxExperts / kThreads;
-  int32_t count[kPer];
+  int32_t bound[kPer + 1], count[kPer];
   int32_t sum = 0;
+#pragma unroll
+  for (int i = 0; i <= kPer; ++i) {
+    const int e = threadIdx.x * kPer + i;
+    bound[i] = e <= experts ? offsets[e] : 0;
+  }
+  pipe_start(s);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = threadIdx.x * kPer + i;
     count[i] = 0;
     if (e < experts) {
-      const int a = slot_bound(offsets, e, slots), b = slot_bound(offsets, e + 1, slots);
+      const int a = min(max(bound[i], 0), slots), b = min(max(bound[i + 1], 0), slots);
       s.start[e] = a;
       if (e == experts - 1) s.start[experts] = b;
       count[i] = tiles_of(max(b - a, 0));
@@ -321,9 +330,14 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = static_cast<int>(cluster_ctarank());
   const bool leader = cta == 0;
+  if (threadIdx.x == 96) {
+    tma_prefetch_desc(&p.tma_w);
+    for (int i = 0; i < 4; ++i) tma_prefetch_desc(&p.tma_x[i]);
+  }
+  // (the offsets come in while the barriers and TMEM are set up)
   list_tiles(s, p.offsets, p.slots, p.experts,
              [&](int rows) { return (rows + kTile - 1) / kTile * p.f_tiles; });
-  const uint32_t tmem_base = pipe_start(s);
+  const uint32_t tmem_base = pipe_meet(s);
   WaitBudget wb;
   wb.start(p.budget_ns, s.words + 1);
 
@@ -624,7 +638,13 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
   const int cta = static_cast<int>(cluster_ctarank());
   const bool leader = cta == 0;
   const int per_expert = p.m_tiles * p.n_tiles;
-  const uint32_t tmem_base = pipe_start(s);
+  if (threadIdx.x == 96) {
+    tma_prefetch_desc(&p.tma_a);
+    tma_prefetch_desc(&p.tma_b);
+    tma_prefetch_desc(&p.tma_out);
+  }
+  pipe_start(s);
+  const uint32_t tmem_base = pipe_meet(s);
   WaitBudget wb;
   wb.start(p.budget_ns, s.words + 1);
   const int total = p.experts * per_expert;
