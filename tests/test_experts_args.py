@@ -133,6 +133,27 @@ def test_backward_and_combine_refusals():
         ops.expert_combine_backward(torch.zeros(8, 16).half(), H, s, w)
 
 
+def test_results_may_lie_beside_their_inputs_but_not_over_them():
+    s = _slots(tokens=8, top_k=1)
+    big = torch.zeros(8, 64).half()
+    W = torch.zeros(3, 16, 24).half()
+    X, beside, over = big[:, :16], big[:, 16:40], big[:, 8:32]
+    with pytest.raises(ValueError, match="CUDA"):                # right, but on the CPU
+        ops.expert_gemm(X, W, s, beside)
+    with pytest.raises(ValueError, match="overlaps X"):
+        ops.expert_gemm(X, W, s, over)
+    with pytest.raises(ValueError, match="overlaps W"):
+        ops.expert_gemm(X, W, s, W.view(-1)[:8 * 24].view(8, 24))
+    H, add = big[:, :16], torch.zeros(8, 16).half()
+    with pytest.raises(ValueError, match="overlaps H"):
+        ops.expert_combine(H, s, None, H)
+    with pytest.raises(ValueError, match="CUDA"):                # in place over the residual
+        ops.expert_combine(H, s, None, add, add=add)
+    pair = torch.zeros(8, 24).half()
+    with pytest.raises(ValueError, match="overlaps add"):
+        ops.expert_combine(H, s, None, pair[:, :16], add=pair[:, 8:])
+
+
 def test_native_entries_check_their_arguments():
     """The C entries refuse on their own (another binding may call them)."""
     lib = _native.load()

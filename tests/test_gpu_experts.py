@@ -770,3 +770,53 @@ def test_counters_run_out(monkeypatch):
     got = ops.expert_gemm(x, W, slots, stream=stream)
     stream.synchronize()
     assert torch.equal(got, want)
+
+
+def test_the_same_expert_twice():
+    """A token that names an expert twice has two slots of it; gradients add up."""
+    from tileccl_b200 import ops
+
+    g = _gen(51)
+    ids = torch.tensor([[1, 1], [0, 1], [2, 2]], dtype=torch.int32, device="cuda")
+    slots = ops.expert_slots(ids, 3)
+    assert slots.offsets.tolist() == [0, 1, 4, 6] and slots.slot_of.tolist() == [[1, 2], [0, 3], [4, 5]]
+    X, W = _randn(g, 3, 64, dtype=torch.float16), _randn(g, 3, 64, 72, std=0.125, dtype=torch.float16)
+    y = ops.expert_gemm(X, W, slots)
+    assert torch.equal(y[1], y[2]) and torch.equal(y[4], y[5])
+    w = torch.tensor([[0.25, 0.75], [1.0, 1.0], [2.0, -1.0]], device="cuda")
+    out = ops.expert_combine(y, slots, w)
+    once = ops.expert_combine(y, slots, w.sum(1, keepdim=True) * torch.tensor([[1.0, 0.0]], device="cuda"))
+    assert torch.equal(out[0], once[0]) and torch.equal(out[2], once[2])
+    logits = _randn(g, 3, 8)
+    grad = torch.ones(3, 2, device="cuda")
+    d = ops.route_experts_backward(grad, logits, ids, score="sigmoid", renormalize=False)
+    p = torch.sigmoid(logits.double())
+    want = torch.zeros_like(p)
+    for t in range(3):
+        for j in range(2):
+            e = int(ids[t, j])
+            want[t, e] += p[t, e] * (1 - p[t, e])
+    _within(d, want, want * 2 ** -20)
+
+
+def test_malformed_maps_stay_in_bounds():
+    """Indices that no expert_slots would give are skipped or clamped, never followed."""
+    from tileccl_b200 import ops
+
+    T, k, E, K, N = 6, 2, 3, 64, 72
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    bad = ops.ExpertSlots(i32([5, -3, 400, 7]), i32([900, -7] + [0] * 10), i32([[99, -5]] * T))
+    X, W = torch.ones(T, K, device="cuda").half(), torch.ones(E, K, N, device="cuda").half()
+    guard = torch.full((T * k + 16, N), 4.0, device="cuda").half()
+    out = guard[8:8 + T * k]
+    ops.expert_gemm(X, W, bad, out)
+    gx, gw = ops.expert_gemm_backward(torch.ones(T * k, N, device="cuda").half(), X, W, bad)
+    assert (ops.expert_combine(out, bad, torch.ones(T, k, device="cuda")) == 0).all()
+    _, dw = ops.expert_combine_backward(torch.ones(T, N, device="cuda").half(), out, bad,
+                                        torch.ones(T, k, device="cuda"))
+    torch.cuda.synchronize()
+    ops.check_expert_status()
+    assert (guard[:8] == 4).all() and (guard[8 + T * k:] == 4).all() and (dw == 0).all()
+    d = ops.route_experts_backward(torch.ones(1, 2, device="cuda"), torch.zeros(1, 8, device="cuda"),
+                                   i32([[8, -9]]))
+    assert (d == 0).all()

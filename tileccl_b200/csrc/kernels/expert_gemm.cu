@@ -30,12 +30,17 @@ constexpr int kMaxExperts = 1024;
 constexpr int kThreads = 256;            // warp 0 TMA, 1 MMA, 2 TMEM, 3 idle, 4-7 epilogue
 constexpr int kCopyThreads = 128;        // warps 8-11 of the weight gradient
 constexpr int kEpiThreads = 128;         // warps 4-7
-constexpr int kStages = 6;
+constexpr int kStages = 6;               // 32 KB each
+constexpr int kFewStages = 9;            // 20 KB each: with at most kFewTokens rows per tile
+constexpr int kFewTokens = 64;
 constexpr int kBK = 64;                  // contraction elements per stage (one 128-byte row)
 constexpr int kUmmaK = 16;
 constexpr int kHalfBytes = 64 * 128;     // 64 rows of 128 bytes: one TMA box, 8 KB
 constexpr int kOperandBytes = 2 * kHalfBytes;
 constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kRingBytes = kStages * kStageBytes;
+constexpr int kFewBytes = kOperandBytes + kFewTokens / 2 * 128;
+static_assert(kFewStages * kFewBytes <= kRingBytes && kFewBytes % 1024 == 0, "ring of few tokens");
 constexpr int kTile = 256;               // features (M) and, at most, tokens (N) of a pair's tile
 constexpr int kAccCols = 256;            // TMEM columns of one accumulator
 constexpr int kBand = 16;                // token tiles that share a sweep over the features
@@ -51,7 +56,7 @@ constexpr int kGradSmem = kStages * kStageBytes + kGradStagingBytes + kCtlBytes 
 static_assert(kGemmSmem <= 232448 && kGradSmem <= 232448, "shared memory of one SM");
 
 struct GemmParams {
-  CUtensorMap tma_w;          // {columns, rows, experts}, box {64, 64, 1}, 128-byte swizzle
+  CUtensorMap tma_w;          // five dimensions, see weight_map
   CUtensorMap tma_x[4];       // {K, rows}, boxes {64, 128}, {64, 64}, {64, 32}, {64, 16}
   const int32_t* offsets;
   void* out;
@@ -61,22 +66,33 @@ struct GemmParams {
   int64_t ldo, ld_dh;
   int32_t partial_tokens;
   int32_t slots, experts, k_blocks, n, f_tiles, bf16, w_nk;
+  int32_t w_halves;           // a CTA's 128 features come as two boxes
   uint32_t* status;
   uint64_t budget_ns;
 };
 
 struct GradParams {
-  CUtensorMap tma_a, tma_b;   // {columns, rows}, box {64, 64}
+  CUtensorMap tma_a, tma_b;   // {64, rows, columns / 64}, box {64, 64, 2}; 64 does not divide the
+                              // columns: {columns, rows, 1}, box {64, 64, 1} twice
   CUtensorMap tma_out;        // {n, m, experts}, box {64, 32, 1}
   const int32_t* offsets;
   const void* a;
   const void* b;
   int64_t lda, ldb;
   int32_t slots, experts, m, n, m_tiles, n_tiles, bf16;
+  int32_t a_halves, b_halves;
   uint32_t* status;
   uint64_t budget_ns;
 };
 
+__device__ __forceinline__ void tma_load_5d_pair(uint32_t dst, const CUtensorMap* m, int x, int y,
+                                                 int z, int u, int v, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile"
+      ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* m, int x, int y,
                                                  int z, uint32_t bar) {
   asm volatile(
@@ -145,12 +161,12 @@ struct Pipe {
 __device__ __forceinline__ Pipe make_pipe(uint8_t* raw, int staging_bytes) {
   Pipe s;
   s.base = (smem_u32(raw) + 1023u) & ~1023u;
-  s.staging = s.base + kStages * kStageBytes;
+  s.staging = s.base + kRingBytes;
   s.ctl = s.staging + staging_bytes;
   s.full = s.ctl;
-  s.empty = s.full + 8 * kStages;
-  s.tail = s.empty + 8 * kStages;
-  s.acc_full = s.tail + 8 * kStages;
+  s.empty = s.full + 8 * kFewStages;
+  s.tail = s.empty + 8 * kFewStages;
+  s.acc_full = s.tail + 8 * kFewStages;
   s.acc_empty = s.acc_full + 16;
   s.drain = s.acc_empty + 16;
   s.tmem_slot = s.drain + 8;
@@ -166,7 +182,7 @@ __device__ __forceinline__ Pipe make_pipe(uint8_t* raw, int staging_bytes) {
 // afterwards.
 __device__ __forceinline__ void pipe_start(const Pipe& s) {
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kFewStages; ++i) {
       mbar_init(s.full + 8 * i, 1);
       mbar_init(s.empty + 8 * i, 1);
       mbar_init(s.tail + 8 * i, 2);          // the copying warps of both CTAs
@@ -294,18 +310,20 @@ __device__ __forceinline__ void store_row8(void* base, int64_t i, bool bf16, con
 // operand: M is fixed to 256 by the pair form of the instruction while N may be any multiple
 // of 32, so an expert's tile is as wide as its rows need.  With the gate a CTA's 128 features
 // are 64 gate columns and the 64 up columns that belong to them.
-// ---------------------------------------------------------------------------------------
 //
 // Schedule: tile t goes to pair t mod P.  With few tokens the time is that of streaming the
-// weights, and half of the SMs suffice to draw the full memory bandwidth: only a last round with
+// weights, and a third of the SMs nearly draws the full memory bandwidth: only a last round with
 // fewer tiles than that is worth spreading.  The first R = P + T mod P tiles (all of them when
 // T < P) are then cut into P equal runs of K blocks: a pair's run covers the end of one tile,
 // whole tiles, the start of another.  Parts of a tile are left in `partial` as fp32 sums;
 // whichever pair comes last (a counter per tile and CTA) adds them up in the order of K, so the
-// result does not depend on who that was.  Measured with one token (us, shared / whole): 2
-// experts of 14336 x 4096 47 / 56, 1 expert 28 / 55, 4 tokens of 2 104 / 129; against that 8
-// experts of 2048 x 1024 16 / 14 (short K), 8 of 4096 x 3584 50 / 45 (T = 1.5 P), and 512 tokens
-// of 2 204 / 158 (wide partial tiles), all of which stay whole.
+// result does not depend on who that was.  Measured (us, shared / whole): one token of 1 expert of
+// 14336 x 4096 27 / 46 (T = 0.2 P), 4 tokens of 2 experts 101 / 118 (T = 1.1 P); one token of 2
+// experts 47 / 47 (T = 0.4 P), of 8 of 4096 x 3584 48 / 45 (T = 1.5 P) and 512 tokens of 2 experts
+// 204 / 158 (wide partial tiles) stay whole.
+//
+// kFew: no tile is wider than kFewTokens, so the ring holds nine stages instead of six: what an SM
+// draws is what it has in flight (one token of 2 experts of 14336 x 4096: 53 -> 47 us).
 // ---------------------------------------------------------------------------------------
 struct Item {
   int e, row0, rows, n, f0;
@@ -322,9 +340,11 @@ struct Walker {
   int next;                  // next whole tile
 };
 
-template <int kEpi>
+template <int kEpi, bool kFew>
 __global__ void __launch_bounds__(kThreads, 1)
 expert_gemm_kernel(const __grid_constant__ GemmParams p) {
+  constexpr bool kPlain = kEpi == kNone || kEpi == kFloat;
+  constexpr int kRing = kFew ? kFewStages : kStages, kBytes = kFew ? kFewBytes : kStageBytes;
   extern __shared__ uint8_t smem_raw[];
   const Pipe s = make_pipe(smem_raw, kStagingBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -346,7 +366,7 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
   auto walk = [&]() {
     Walker w;
     const int over = total % pairs;
-    w.shared = p.partial == nullptr || 2 * over >= pairs ? 0 : total < pairs ? total : over > 0 ? pairs + over : 0;
+    w.shared = p.partial == nullptr || over == 0 || 3 * over >= pairs ? 0 : total < pairs ? total : pairs + over;
     const int blocks = w.shared * p.k_blocks;      // (at most 2 * pairs tiles)
     w.unit = max((blocks + pairs - 1) / pairs, min(kMinBlocks, p.k_blocks));
     w.pos = min(pair * w.unit, blocks);
@@ -402,23 +422,24 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
       while (ok && advance(w, it)) {
         const int mine = it.n >> 1;                          // token rows this CTA stages
         const int first = it.row0 + cta * mine;
+        // this CTA's 128 features in the coordinates of weight_map
+        const int f = it.f0 + cta * 128;
+        const int w_inner = !kPlain ? cta * 64 : p.w_nk || p.w_halves ? f : 0;
+        const int w_z = kPlain && !p.w_nk && !p.w_halves ? f / 64 : 0;
+        const int w_u = kPlain ? 0 : it.f0 / kTile;
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (!mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb)) {
             report_status(p.status, kStatusTimeoutMbarrier, 101, 0, kb, 0, it.row0);
             ok = false;
             break;
           }
-          const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+          const uint32_t sa = s.base + stage * kBytes, sb = sa + kOperandBytes;
           const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
           // the bytes of both CTAs are counted on the leader's barrier
           if (leader) mbar_expect_tx(s.full + 8 * stage, 2 * (kOperandBytes + mine * 128));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int f = kEpi == kNone || kEpi == kFloat ? it.f0 + cta * 128 + h * 64
-                                                          : it.f0 + h * 128 + cta * 64;
-            if (p.w_nk) tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, kb * kBK, f, it.e, bar);
-            else tma_load_3d_pair(sa + h * kHalfBytes, &p.tma_w, f, kb * kBK, it.e, bar);
-          }
+          const int wx = p.w_nk ? kb * kBK : w_inner, wy = p.w_nk ? w_inner : kb * kBK;
+          tma_load_5d_pair(sa, &p.tma_w, wx, wy, w_z, w_u, it.e, bar);
+          if (p.w_halves) tma_load_5d_pair(sa + kHalfBytes, &p.tma_w, wx + 64, wy, w_z, w_u, it.e, bar);
           // as few boxes as the row count has binary digits: a copy keeps the TMA unit busy for
           // some 70 cycles however small it is (boxes of 16 rows throughout: 999 instead of 1549
           // TFLOP/s; the unit's own gather, four rows per copy: 460)
@@ -430,7 +451,7 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
               at += 128 >> i;
             }
           }
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == kRing) { stage = 0; phase ^= 1u; }
         }
       }
       if (!ok) drain_copies();
@@ -456,7 +477,7 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
             break;
           }
           tcgen05_fence_after();
-          const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+          const uint32_t sa = s.base + stage * kBytes, sb = sa + kOperandBytes;
 #pragma unroll
           for (int k = 0; k < kBK / kUmmaK; ++k) {
             const uint64_t da = p.w_nk ? umma_smem_desc_sw128(sa + k * kUmmaK * 2, 16, 1024)
@@ -465,7 +486,7 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
             umma_f16_pair(d, da, db, idesc, kb > it.kb0 || k > 0 ? 1u : 0u);
           }
           umma_commit_pair(s.empty + 8 * stage, 3);
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == kRing) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
         umma_commit_pair(s.acc_full + 8 * acc, 3);
@@ -485,7 +506,6 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
     const int q = warp - 4, me = threadIdx.x - 128;
     float* const staging = reinterpret_cast<float*>(smem_raw + (s.staging - smem_u32(smem_raw)));
     const bool bf16 = p.bf16 != 0;
-    constexpr bool kPlain = kEpi == kNone || kEpi == kFloat;
     constexpr int kVecs = kPlain ? 16 : 8;                 // 8-feature vectors per token
     uint32_t acc = 0, acc_phase = 0, buf = 0;
     while (advance(w, it)) {
@@ -670,12 +690,13 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
           const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
           const bool whole = r0 + kBK <= row1;
           if (leader) mbar_expect_tx(s.full + 8 * stage, whole ? 2 * kStageBytes : 0);
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, bool halves) {
+            tma_load_3d_pair(dst, map, halves ? x : 0, r0, halves ? 0 : x / 64, bar);
+            if (halves) tma_load_3d_pair(dst + kHalfBytes, map, x + 64, r0, 0, bar);
+          };
           if (whole) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              tma_load_2d_pair(sa + h * kHalfBytes, &p.tma_a, x_a + h * 64, r0, bar);
-              tma_load_2d_pair(sb + h * kHalfBytes, &p.tma_b, x_b + h * 64, r0, bar);
-            }
+            load(sa, &p.tma_a, x_a, p.a_halves != 0);
+            load(sb, &p.tma_b, x_b, p.b_halves != 0);
           }
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
@@ -845,30 +866,75 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
 }
 
 // ------------------------------------------------------------------------------- host side
-int encode(CUtensorMap* map, bool bf16, uint64_t base, uint64_t cols, uint64_t rows,
-           uint64_t depth, uint64_t ld_bytes, uint64_t slab_bytes, uint32_t box_rows,
-           const char* what) {
+// 16-bit tensor of `rank` dimensions (unit stride innermost) with a box of 128-byte rows.
+int encode(CUtensorMap* map, bool bf16, uint64_t base, int rank, const cuuint64_t* dims,
+           const cuuint64_t* strides, const cuuint32_t* box, const char* what) {
   const DriverApi& d = driver();
-  cuuint64_t dims[3] = {cols, rows, depth};
-  cuuint64_t strides[2] = {ld_bytes, slab_bytes};
-  cuuint32_t box[3] = {64, box_rows, 1};
-  cuuint32_t es[3] = {1, 1, 1};
+  cuuint32_t es[5] = {1, 1, 1, 1, 1};
   const CUresult r = d.cuTensorMapEncodeTiled(
       map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-      depth > 0 ? 3 : 2, reinterpret_cast<void*>(base), dims, strides, box, es,
+      static_cast<cuuint32_t>(rank), reinterpret_cast<void*>(base), dims, strides, box, es,
       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(kErrCuda, std::string("cuTensorMapEncodeTiled(") + what + "): " + driver_error_string(r));
   return kOk;
 }
+int encode_rows(CUtensorMap* map, bool bf16, uint64_t base, uint64_t cols, uint64_t rows,
+                uint64_t ld_bytes, uint32_t box_rows, const char* what) {
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld_bytes};
+  const cuuint32_t box[2] = {64, box_rows};
+  return encode(map, bf16, base, 2, dims, strides, box, what);
+}
+
+// The weights as five dimensions in which a CTA's 128 features of a K block are one box: every
+// copy costs the TMA unit some 100 cycles, which shows where few tokens leave little else in a
+// stage (one token of one expert of 14336 x 4096, tiles whole: 54 us with two boxes, 46 with one).
+//   [N, K]           {K, N, 1, 1, E}             box {64, 128, 1, 1, 1}
+//   [N, K], gate     {K, 128, 2, N / 256, E}     box {64, 64, 2, 1, 1}   64 gate and 64 up rows
+//   [K, N]           {64, K, N / 64, 1, E}       box {64, 64, 2, 1, 1}   64 does not divide N:
+//                    {N, K, 1, 1, E}             box {64, 64, 1, 1, 1}   twice (w_halves)
+//   [K, N], gate     {128, K, 2, N / 256, E}     box {64, 64, 2, 1, 1}
+int weight_map(const TcclExpertGemm& d, GemmParams* p) {
+  const bool gate = d.epilogue == kSiluGate || d.epilogue == kSiluGateGrad;
+  const cuuint64_t ld = d.ldw * 2, slab = d.w_expert * 2, n = d.n, k = d.k, e = d.experts;
+  cuuint64_t dims[5] = {0, 0, 1, 1, e}, strides[4] = {ld, 16, 16, slab};
+  cuuint32_t box[5] = {64, 64, 2, 1, 1};
+  p->w_nk = d.w_nk ? 1 : 0;
+  p->w_halves = 0;
+  if (gate) {
+    dims[0] = d.w_nk ? k : 128;
+    dims[1] = d.w_nk ? 128 : k;
+    dims[2] = 2;
+    dims[3] = n / 256;
+    strides[1] = d.w_nk ? 128 * ld : 128 * 2;
+    strides[2] = 2 * strides[1];
+  } else if (d.w_nk) {
+    dims[0] = k;
+    dims[1] = n;
+    box[1] = 128;
+    box[2] = 1;
+  } else if (n % 64 == 0) {
+    dims[0] = 64;
+    dims[1] = k;
+    dims[2] = n / 64;
+    strides[1] = 64 * 2;
+  } else {
+    dims[0] = n;
+    dims[1] = k;
+    box[2] = 1;
+    p->w_halves = 1;
+  }
+  return encode(&p->tma_w, d.dtype == 1, d.w, 5, dims, strides, box, "W");
+}
 
 using GemmKernel = void (*)(const GemmParams);
+template <bool kFew>
 GemmKernel gemm_kernel(int epilogue) {
-  return epilogue == kNone           ? expert_gemm_kernel<kNone>
-         : epilogue == kSiluGate     ? expert_gemm_kernel<kSiluGate>
-         : epilogue == kSiluGateGrad ? expert_gemm_kernel<kSiluGateGrad>
-                                     : expert_gemm_kernel<kFloat>;
+  return epilogue == kNone           ? expert_gemm_kernel<kNone, kFew>
+         : epilogue == kSiluGate     ? expert_gemm_kernel<kSiluGate, kFew>
+         : epilogue == kSiluGateGrad ? expert_gemm_kernel<kSiluGateGrad, kFew>
+                                     : expert_gemm_kernel<kFloat, kFew>;
 }
 
 cudaError_t attrs_once(int* sms) {
@@ -878,8 +944,8 @@ cudaError_t attrs_once(int* sms) {
   if (e != cudaSuccess) return e;
   if (dev < 64 && count[dev] != 0) { *sms = count[dev]; return cudaSuccess; }
   e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
-  for (int i = 0; i < 4 && e == cudaSuccess; ++i)
-    e = cudaFuncSetAttribute(gemm_kernel(i),
+  for (int i = 0; i < 8 && e == cudaSuccess; ++i)
+    e = cudaFuncSetAttribute(i < 4 ? gemm_kernel<false>(i) : gemm_kernel<true>(i - 4),
                              cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(expert_weight_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -922,7 +988,8 @@ cudaError_t preload_expert_gemm_kernels() {
   cudaFuncAttributes a;
   int sms = 0;
   cudaError_t e = cudaFuncGetAttributes(&a, expert_weight_grad_kernel);
-  for (int i = 0; i < 4 && e == cudaSuccess; ++i) e = cudaFuncGetAttributes(&a, gemm_kernel(i));
+  for (int i = 0; i < 8 && e == cudaSuccess; ++i)
+    e = cudaFuncGetAttributes(&a, i < 4 ? gemm_kernel<false>(i) : gemm_kernel<true>(i - 4));
   if (e == cudaSuccess) e = attrs_once(&sms);
   return e;
 }
@@ -975,11 +1042,10 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   TCCL_REQUIRE_DRIVER();
   const bool bf16 = d.dtype == 1;
   GemmParams p;
-  int rc = encode(&p.tma_w, bf16, d.w, d.w_nk ? d.k : d.n, d.w_nk ? d.n : d.k, d.experts, d.ldw * 2,
-                  d.w_expert * 2, 64, "W");
+  int rc = weight_map(d, &p);
   if (rc) return rc;
   for (int i = 0; i < 4; ++i) {
-    rc = encode(&p.tma_x[i], bf16, d.x, d.k, d.slots, 0, d.ldx * 2, 0, 128 >> i, "X");
+    rc = encode_rows(&p.tma_x[i], bf16, d.x, d.k, d.slots, d.ldx * 2, 128 >> i, "X");
     if (rc) return rc;
   }
   p.offsets = reinterpret_cast<const int32_t*>(d.offsets);
@@ -997,7 +1063,6 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   p.n = static_cast<int32_t>(d.n);
   p.f_tiles = static_cast<int32_t>(f_tiles);
   p.bf16 = bf16 ? 1 : 0;
-  p.w_nk = d.w_nk ? 1 : 0;
   p.status = reinterpret_cast<uint32_t*>(d.status);
   p.budget_ns = kWaitBudgetNs;
   int sms = 0;
@@ -1005,7 +1070,9 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   // (a shared tile is cut into runs of kMinBlocks K blocks at least)
   const int64_t runs = p.partial == nullptr ? tiles : tiles * ((p.k_blocks + kMinBlocks - 1) / kMinBlocks);
   const int pairs = static_cast<int>(runs < sms / 2 ? runs : sms / 2);
-  TCCL_CHECK_CUDA(launch_pairs(gemm_kernel(d.epilogue), p, pairs,
+  const GemmKernel kernel =
+      d.slots <= kFewTokens ? gemm_kernel<true>(d.epilogue) : gemm_kernel<false>(d.epilogue);
+  TCCL_CHECK_CUDA(launch_pairs(kernel, p, pairs,
                                kThreads, kGemmSmem,
                                reinterpret_cast<cudaStream_t>(stream)));
   return kOk;
@@ -1035,9 +1102,23 @@ extern "C" int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_
   TCCL_REQUIRE_DRIVER();
   const bool bf16 = d.dtype == 1;
   GradParams p;
-  int rc = encode(&p.tma_a, bf16, d.a, d.m, d.slots, 0, d.lda * 2, 0, 64, "A");
-  if (!rc) rc = encode(&p.tma_b, bf16, d.b, d.n, d.slots, 0, d.ldb * 2, 0, 64, "B");
-  if (!rc) rc = encode(&p.tma_out, bf16, d.out, d.n, d.m, d.experts, d.n * 2, d.m * d.n * 2, 32, "out");
+  auto operand = [&](CUtensorMap* map, uint64_t base, uint64_t cols, uint64_t ld, int32_t* halves,
+                     const char* what) {
+    *halves = cols % 64 != 0 ? 1 : 0;
+    const cuuint64_t dims[3] = {*halves ? cols : 64, static_cast<cuuint64_t>(d.slots), *halves ? 1 : cols / 64};
+    const cuuint64_t strides[2] = {ld * 2, 128};
+    const cuuint32_t box[3] = {64, 64, *halves ? 1u : 2u};
+    return encode(map, bf16, base, 3, dims, strides, box, what);
+  };
+  int rc = operand(&p.tma_a, d.a, d.m, d.lda, &p.a_halves, "A");
+  if (!rc) rc = operand(&p.tma_b, d.b, d.n, d.ldb, &p.b_halves, "B");
+  if (!rc) {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d.n), static_cast<cuuint64_t>(d.m),
+                                static_cast<cuuint64_t>(d.experts)};
+    const cuuint64_t strides[2] = {dims[0] * 2, dims[0] * dims[1] * 2};
+    const cuuint32_t box[3] = {64, 32, 1};
+    rc = encode(&p.tma_out, bf16, d.out, 3, dims, strides, box, "out");
+  }
   if (rc) return rc;
   p.offsets = reinterpret_cast<const int32_t*>(d.offsets);
   p.a = reinterpret_cast<const void*>(d.a);

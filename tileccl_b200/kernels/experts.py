@@ -11,7 +11,8 @@ A layer runs them in this order::
 
 Nothing here synchronises with the host: how many rows an expert has stays on the GPU, and
 every shape depends on ``tokens * top_k`` alone, so a layer can be captured into a CUDA graph.
-All results repeat bit for bit from call to call.
+All results repeat bit for bit from call to call.  The functions record no autograd graph; each
+``*_backward`` takes what its forward function took.
 
 ``stream``: the stream to run on (default: the current stream of the tensors' device).  Results
 are allocated on that stream; the caller orders it behind the work that produced the inputs.
@@ -427,6 +428,26 @@ def _gather(X, slots, raw):
     return xs
 
 
+def _refuse_overlap(out, **inputs) -> None:
+    """``out`` is written while the inputs are read: it may lie beside them in one buffer (other
+    columns of the same rows), but not over them."""
+    a0, pitch = out.data_ptr(), out.stride(0) * out.element_size()
+    a1 = a0 + ((out.shape[0] - 1) * out.stride(0) + out.shape[1]) * out.element_size()
+    for name, t in inputs.items():
+        if t is None or t.numel() == 0 or out.numel() == 0:
+            continue
+        b0 = t.data_ptr()
+        b1 = b0 + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+        if a0 >= b1 or b0 >= a1:
+            continue
+        if t.dim() == 2 and t.shape[0] > 1 and out.shape[0] > 1 and t.stride(0) * t.element_size() == pitch:
+            shift = (b0 - a0) % pitch
+            if shift >= out.shape[1] * out.element_size() and \
+                    shift + t.shape[1] * t.element_size() <= pitch:
+                continue
+        raise ValueError(f"out overlaps {name}")
+
+
 def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
     """One launch of the grouped product; every argument is checked already."""
     E = W.shape[0]
@@ -465,6 +486,7 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
     writes ``silu(gate) * up``, half as wide.  Rows of ``out [tokens * top_k, N]`` behind the
     last slot keep what they held.  ``out`` must not overlap an input.  ``out_dtype``:
     ``X.dtype`` (default, or that of ``out``) or, without the gate, ``torch.float32``.
+    ``rows="tokens"`` takes scratch memory for ``tokens * top_k`` rows of ``X``.
     """
     E, K, N, epi = _check_product(X, W, slots, rows, b_is_nk, epilogue)
     shape = (slots.capacity, N // 2 if epi else N)
@@ -478,6 +500,7 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
         epi = _EPI_FLOAT
     if out is not None:
         _check_rows("out", out, shape, X, out_dtype)
+        _refuse_overlap(out, X=X, W=W)
     with _On(stream, (X, W, slots.offsets, slots.token_of_slot, out)) as raw:
         if out is None:
             out = X.new_empty(shape, dtype=out_dtype)
@@ -573,6 +596,8 @@ def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.
         _check_rows("add", add, shape, H)
     if out is not None:
         _check_rows("out", out, shape, H)
+        same = add is not None and out.data_ptr() == add.data_ptr() and out.stride() == add.stride()
+        _refuse_overlap(out, H=H, add=None if same else add, weights=weights)
     with _On(stream, (H, weights, add, slots.slot_of, out)) as raw:
         if out is None:
             out = H.new_empty(shape)
