@@ -176,6 +176,7 @@ class ExpertGemm(C.Structure):
         ("status", C.c_uint64),
         ("partial", C.c_uint64),
         ("counters", C.c_uint64),
+        ("wait_budget_ns", C.c_uint64),
     ]
 
 
@@ -193,6 +194,7 @@ class ExpertWeightGrad(C.Structure):
         ("lda", C.c_int64),
         ("ldb", C.c_int64),
         ("status", C.c_uint64),
+        ("wait_budget_ns", C.c_uint64),
     ]
 
 

@@ -262,10 +262,16 @@ __device__ __forceinline__ void list_tiles(const Pipe& s, const int32_t* offsets
 }
 
 // Neither CTA of a pair may retire while its partner can still read its operands or touch its
-// barriers; TMEM goes back after every MMA and TMEM read is done.
-__device__ __forceinline__ void pipe_end(uint32_t tmem_base) {
+// barriers; TMEM goes back after every MMA and TMEM read is done.  After a wait that gave up,
+// copies that are still on their way to either CTA get two milliseconds to land.
+__device__ __forceinline__ void pipe_end(const Pipe& s, uint32_t tmem_base) {
   tcgen05_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && s.words[1] != 0) {
+    const uint64_t until = globaltimer_ns() + 2000000ull;
+    for (int i = 0; i < 1000000 && globaltimer_ns() < until; ++i) __nanosleep(1000);
+  }
+  __syncwarp();
   cluster_sync_all();
   if ((threadIdx.x >> 5) == 2) {
     tcgen05_fence_after();
@@ -282,12 +288,6 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, cons
       return false;
     }
   }
-}
-
-// After a wait that gave up: copies still in flight get two milliseconds to land.
-__device__ __forceinline__ void drain_copies() {
-  const uint64_t until = globaltimer_ns() + 2000000ull;
-  for (int i = 0; i < 1000000 && globaltimer_ns() < until; ++i) __nanosleep(1000);
 }
 
 __device__ __forceinline__ int expert_of(const Pipe& s, int experts, int t) {
@@ -454,7 +454,6 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
           if (++stage == kRing) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok) drain_copies();
     }
   } else if (warp == 1 && leader) {
     // ----------------------- MMA issuer (leader CTA only) -----------------------
@@ -640,7 +639,7 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
       }
     }
   }
-  pipe_end(tmem_base);
+  pipe_end(s, tmem_base);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -701,7 +700,6 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok) drain_copies();
     }
   } else if (warp == 1 && leader) {
     // ----------------------- MMA issuer (leader CTA only) -----------------------
@@ -862,7 +860,7 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
     }
     if (lane == 0) tma_store_wait_all<0>();
   }
-  pipe_end(tmem_base);
+  pipe_end(s, tmem_base);
 }
 
 // ------------------------------------------------------------------------------- host side
@@ -1064,7 +1062,7 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   p.f_tiles = static_cast<int32_t>(f_tiles);
   p.bf16 = bf16 ? 1 : 0;
   p.status = reinterpret_cast<uint32_t*>(d.status);
-  p.budget_ns = kWaitBudgetNs;
+  p.budget_ns = d.wait_budget_ns ? d.wait_budget_ns : kWaitBudgetNs;
   int sms = 0;
   TCCL_CHECK_CUDA(attrs_once(&sms));
   // (a shared tile is cut into runs of kMinBlocks K blocks at least)
@@ -1133,7 +1131,7 @@ extern "C" int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_
   p.n_tiles = static_cast<int32_t>(n_tiles);
   p.bf16 = bf16 ? 1 : 0;
   p.status = reinterpret_cast<uint32_t*>(d.status);
-  p.budget_ns = kWaitBudgetNs;
+  p.budget_ns = d.wait_budget_ns ? d.wait_budget_ns : kWaitBudgetNs;
   int sms = 0;
   TCCL_CHECK_CUDA(attrs_once(&sms));
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);

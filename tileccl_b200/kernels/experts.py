@@ -142,8 +142,8 @@ def _status_ptr(dev: torch.device) -> int:
 
 def check_expert_status(device=None) -> None:
     """Synchronise and raise :class:`TileCCLTimeoutError` if a wait inside a grouped product on
-    ``device`` (default: the current one) ran out of its two-second budget since the last check;
-    the results of that call are then undefined."""
+    ``device`` (default: the current one) ran out of its budget (two seconds, or
+    ``TILECCL_WAIT_BUDGET_US``) since the last check; the results of that call are undefined."""
     dev = torch.device("cuda" if device is None else device)
     t = _STATUS.get(torch.cuda.current_device() if dev.index is None else dev.index)
     if t is not None:
@@ -305,13 +305,12 @@ def expert_slots(ids: torch.Tensor, num_experts: int, *, first_expert: int = 0,
     with _On(stream, (ids,)) as raw:
         n = tokens * top_k
         need = _slots_scratch(n, num_experts)
-        # one allocation for the three parts
-        slot_of, token_of_slot, offsets = ids.new_empty(
-            2 * n + num_experts + 1).split((n, n, num_experts + 1))
+        # one allocation for the three parts and the scratch
+        slot_of, token_of_slot, offsets, scratch = ids.new_empty(
+            2 * n + num_experts + 1 + need // 4).split((n, n, num_experts + 1, need // 4))
         slot_of = slot_of.view(tokens, top_k)
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _launch("tccl_expert_slots", ids.data_ptr(), tokens, top_k, num_experts, first_expert,
-                offsets.data_ptr(), token_of_slot.data_ptr(), slot_of.data_ptr(), _ptr(scratch), raw)
+                offsets.data_ptr(), token_of_slot.data_ptr(), slot_of.data_ptr(), scratch.data_ptr() if need else 0, raw)
     slots = object.__new__(ExpertSlots)           # (its parts need no second check)
     slots.__dict__.update(offsets=offsets, token_of_slot=token_of_slot, slot_of=slot_of)
     return slots
@@ -356,15 +355,6 @@ def _aligned(name, t) -> int:
     if ld % 8 or t.data_ptr() % 16:
         raise ValueError(f"{name} must have 16-byte aligned rows")
     return ld
-
-
-def _gather(X, slots, raw):
-    """``X``'s rows in slot order."""
-    S, K = slots.capacity, X.shape[1]
-    xs = X.new_empty((S, K))
-    _launch("tccl_expert_gather", X.data_ptr(), _aligned("X", X), X.shape[0],
-            slots.token_of_slot.data_ptr(), xs.data_ptr(), K, S, K, raw)
-    return xs
 
 
 @lru_cache(maxsize=4096)
@@ -462,7 +452,7 @@ def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
     if d.w_expert < (W.shape[1] - 1) * d.ldw + W.shape[2] or d.w_expert % 8:
         raise ValueError("W's experts overlap or are not 16-byte aligned")
     d.ld_dh = 0 if dh is None else _aligned("grad_out", dh)
-    d.status = _status_ptr(X.device)
+    d.status, d.wait_budget_ns = _status_ptr(X.device), _fg._config().wait_budget_ns
     partial_bytes, counter_bytes = _scratch_sizes(X.device.index, d.slots, K)
     partial = None
     if partial_bytes:
@@ -542,7 +532,7 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
         grad_X = grad_rows
         if rows == "tokens":
             grad_X = X.new_empty((slots.tokens, K))
-            _combine(grad_rows, slots, None, None, grad_X, raw)
+            _combine(grad_rows, K, slots, None, None, 0, grad_X, K, raw)
         grad_W = X.new_empty(W.shape)
         a, b = (dy, xs) if b_is_nk else (xs, dy)
         d = _native.ExpertWeightGrad()
@@ -551,16 +541,16 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
         d.m, d.n = a.shape[1], b.shape[1]
         d.a, d.b, d.out = a.data_ptr(), b.data_ptr(), grad_W.data_ptr()
         d.lda, d.ldb = _aligned("X", a), _aligned("X", b)
-        d.status = _status_ptr(X.device)
+        d.status, d.wait_budget_ns = _status_ptr(X.device), _fg._config().wait_budget_ns
         _launch("tccl_expert_weight_grad", C.byref(d), raw)
     return grad_X, grad_W
 
 
 # -------------------------------------------------------------------------- combine
-def _combine(H, slots, weights, add, out, raw):
-    _launch("tccl_expert_combine", H.data_ptr(), _aligned("H", H), slots.slot_of.data_ptr(),
-            _ptr(weights), _ptr(add), 0 if add is None else _aligned("add", add), out.data_ptr(),
-            _aligned("out", out), slots.tokens, slots.capacity, slots.top_k, H.shape[1],
+def _combine(H, ld_h, slots, weights, add, ld_add, out, ld_out, raw):
+    tokens, top_k = slots.slot_of.shape
+    _launch("tccl_expert_combine", H.data_ptr(), ld_h, slots.slot_of.data_ptr(), _ptr(weights),
+            _ptr(add), ld_add, out.data_ptr(), ld_out, tokens, tokens * top_k, top_k, H.shape[1],
             _fg.dtype_code(out.dtype), 1 if H.dtype == torch.float32 else 0, raw)
 
 
@@ -572,12 +562,12 @@ def _check_combine(H, slots, weights):
         raise ValueError(f"H has {H.shape[0]} rows, expected {slots.capacity}")
     if H.shape[1] < 8 or H.shape[1] % 8:
         raise ValueError(f"H has {H.shape[1]} columns, which must be a multiple of 8")
-    _aligned("H", H)
     if weights is not None:
         _check_tensor("weights", weights, 2, (torch.float32,), H.device, contiguous=True)
-        if tuple(weights.shape) != (slots.tokens, slots.top_k):
+        if weights.shape != slots.slot_of.shape:
             raise ValueError(f"weights are {tuple(weights.shape)}, expected "
-                             f"{(slots.tokens, slots.top_k)}")
+                             f"{tuple(slots.slot_of.shape)}")
+    return _aligned("H", H)
 
 
 def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.Tensor] = None,
@@ -590,18 +580,18 @@ def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.
     Choices without a slot add nothing.  ``out`` may be ``add`` (in place) but must not overlap
     ``H``.
     """
-    _check_combine(H, slots, weights)
+    ld_h = _check_combine(H, slots, weights)
     shape = (slots.tokens, H.shape[1])
-    if add is not None:
-        _check_rows("add", add, shape, H)
+    ld_add = 0 if add is None else _check_rows("add", add, shape, H)
+    ld_out = shape[1]
     if out is not None:
-        _check_rows("out", out, shape, H)
+        ld_out = _check_rows("out", out, shape, H)
         same = add is not None and out.data_ptr() == add.data_ptr() and out.stride() == add.stride()
         _refuse_overlap(out, H=H, add=None if same else add, weights=weights)
     with _On(stream, (H, weights, add, slots.slot_of, out)) as raw:
         if out is None:
             out = H.new_empty(shape)
-        _combine(H, slots, weights, add, out, raw)
+        _combine(H, ld_h, slots, weights, add, ld_add, out, ld_out, raw)
     return out
 
 
@@ -613,13 +603,13 @@ def expert_combine_backward(grad_out: torch.Tensor, H: torch.Tensor, slots: Expe
     ``add`` is ``grad_out`` itself.)"""
     if weights is None:
         raise ValueError("weights must be a 2-D tensor")
-    _check_combine(H, slots, weights)
-    _check_rows("grad_out", grad_out, (slots.tokens, H.shape[1]), H)
+    ld_h = _check_combine(H, slots, weights)
+    ld_dy = _check_rows("grad_out", grad_out, (slots.tokens, H.shape[1]), H)
     with _On(stream, (H, weights, grad_out, slots.slot_of)) as raw:
         grad_H = H.new_empty(H.shape)
         grad_weights = weights.new_empty(weights.shape)
-        _launch("tccl_expert_combine_backward", grad_out.data_ptr(), _aligned("grad_out", grad_out),
-                H.data_ptr(), _aligned("H", H), slots.slot_of.data_ptr(), weights.data_ptr(),
-                grad_H.data_ptr(), _aligned("grad_H", grad_H), grad_weights.data_ptr(),
+        _launch("tccl_expert_combine_backward", grad_out.data_ptr(), ld_dy, H.data_ptr(), ld_h,
+                slots.slot_of.data_ptr(), weights.data_ptr(), grad_H.data_ptr(), H.shape[1],
+                grad_weights.data_ptr(),
                 slots.tokens, slots.capacity, slots.top_k, H.shape[1], _fg.dtype_code(H.dtype), raw)
     return grad_H, grad_weights
