@@ -51,6 +51,7 @@ constexpr int kStagingBytes = 2 * kChunk * kStageLd * 4;
 constexpr int kCtlBytes = 512;
 constexpr int kListBytes = 2 * 4 * (kMaxExperts + 2);
 constexpr int kGemmSmem = kStages * kStageBytes + kStagingBytes + kCtlBytes + kListBytes + 1024;
+constexpr int kGradStages = kStages - 1; // the sixth stage takes the copied blocks
 constexpr int kGradStagingBytes = 4 * 2 * 4096;   // per epilogue warp two buffers of 32 x 64
 constexpr int kGradSmem = kStages * kStageBytes + kGradStagingBytes + kCtlBytes + 1024;
 static_assert(kGemmSmem <= 232448 && kGradSmem <= 232448, "shared memory of one SM");
@@ -152,7 +153,7 @@ __device__ __forceinline__ void epilogue_sync() { asm volatile("barrier.cta.sync
 // (signalled by multicast commits).
 struct Pipe {
   uint32_t base, staging, ctl;
-  uint32_t full, empty, tail, acc_full, acc_empty, drain, tmem_slot;
+  uint32_t full, empty, tail, tail_empty, acc_full, acc_empty, drain, tmem_slot;
   volatile uint32_t* words;        // generic view of tmem_slot: [0] TMEM base, [1] abort flag
   int32_t* start;                  // [experts + 1] first slot of every expert
   int32_t* tiles;                  // [experts + 1] tiles of all lower experts
@@ -166,7 +167,8 @@ __device__ __forceinline__ Pipe make_pipe(uint8_t* raw, int staging_bytes) {
   s.full = s.ctl;
   s.empty = s.full + 8 * kFewStages;
   s.tail = s.empty + 8 * kFewStages;
-  s.acc_full = s.tail + 8 * kFewStages;
+  s.tail_empty = s.tail + 8;
+  s.acc_full = s.tail_empty + 8;
   s.acc_empty = s.acc_full + 16;
   s.drain = s.acc_empty + 16;
   s.tmem_slot = s.drain + 8;
@@ -185,8 +187,9 @@ __device__ __forceinline__ void pipe_start(const Pipe& s) {
     for (int i = 0; i < kFewStages; ++i) {
       mbar_init(s.full + 8 * i, 1);
       mbar_init(s.empty + 8 * i, 1);
-      mbar_init(s.tail + 8 * i, 2);          // the copying warps of both CTAs
     }
+    mbar_init(s.tail, 2);                    // the copying warps of both CTAs
+    mbar_init(s.tail_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s.acc_full + 8 * i, 1);
       mbar_init(s.acc_empty + 8 * i, 8);     // four epilogue warps of both CTAs
@@ -646,8 +649,13 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
 // out[e] = sum over the slots s of e of a[s]^T b[s]
 //
 // 256 x 256 tiles of out[e]; the contraction runs over the expert's rows, 64 per stage, so both
-// operands are MN-major (a row of 64 columns is 128 bytes of a stage).  The last block of an
-// expert is copied row by row, with zeros in place of the next expert's rows.
+// operands are MN-major (a row of 64 columns is 128 bytes of a stage).  The last, partial block of
+// an expert is copied row by row, with zeros in place of the next expert's rows, into a stage of
+// its own: the copies and their report to the other CTA (a release at cluster scope) take two
+// microseconds, which that stage has a whole tile's time for and one of the ring's has not (8
+// experts of 1024 rows, 4096 x 3584: 179 us with the copies in the ring, 168 with a stage of their
+// own, 1436 TFLOP/s).  With few rows the result bounds it, which the card writes at 3.9 TB/s at
+// most: 82 us for 16 to 64 rows per expert, 60 for the writes alone.
 // ---------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(kThreads + kCopyThreads, 1)
 expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
@@ -679,7 +687,7 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
         const int x_a = local / p.n_tiles * kTile + cta * 128;
         const int x_b = local % p.n_tiles * kTile + cta * 128;
         const int row0 = slot_bound(p.offsets, e, p.slots), row1 = slot_bound(p.offsets, e + 1, p.slots);
-        for (int r0 = row0; r0 < row1; r0 += kBK) {
+        for (int r0 = row0; r0 + kBK <= row1; r0 += kBK) {
           if (!mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb)) {
             report_status(p.status, kStatusTimeoutMbarrier, 111, 0, r0, 0, t);
             ok = false;
@@ -687,17 +695,14 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
           }
           const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
           const uint32_t bar = mapa_shared(s.full + 8 * stage, 0);
-          const bool whole = r0 + kBK <= row1;
-          if (leader) mbar_expect_tx(s.full + 8 * stage, whole ? 2 * kStageBytes : 0);
+          if (leader) mbar_expect_tx(s.full + 8 * stage, 2 * kStageBytes);
           auto load = [&](uint32_t dst, const CUtensorMap* map, int x, bool halves) {
             tma_load_3d_pair(dst, map, halves ? x : 0, r0, halves ? 0 : x / 64, bar);
             if (halves) tma_load_3d_pair(dst + kHalfBytes, map, x + 64, r0, 0, bar);
           };
-          if (whole) {
-            load(sa, &p.tma_a, x_a, p.a_halves != 0);
-            load(sb, &p.tma_b, x_b, p.b_halves != 0);
-          }
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          load(sa, &p.tma_a, x_a, p.a_halves != 0);
+          load(sb, &p.tma_b, x_b, p.b_halves != 0);
+          if (++stage == kGradStages) { stage = 0; phase ^= 1u; }
         }
       }
     }
@@ -705,8 +710,7 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
     // ----------------------- MMA issuer (leader CTA only) -----------------------
     if (elect_one_sync()) {
       const uint32_t idesc = umma_idesc_f16(p.bf16, 1, 1, kTile, kTile);
-      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-      uint32_t tail_phases = 0;           // one bit per stage: copied blocks use it now and then
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, tail_phase = 0;
       bool ok = true;
       for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
         const int e = t / per_expert;
@@ -721,25 +725,22 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
         tcgen05_fence_after();
         const uint32_t d = tmem_base + acc * kAccCols;
         for (int kb = 0; kb < blocks; ++kb) {
-          bool full = mbar_wait(s.full + 8 * stage, phase, wb);
-          if (full && kb * kBK + kBK > rows) {           // the copied block
-            full = wait_cluster(s.tail + 8 * stage, (tail_phases >> stage) & 1u, wb);
-            tail_phases ^= 1u << stage;
-          }
-          if (!full) {
-            report_status(p.status, kStatusTimeoutMbarrier, 113, blocks, kb, 0, t);
+          const bool copied = kb * kBK + kBK > rows;
+          if (copied ? !wait_cluster(s.tail, tail_phase, wb) : !mbar_wait(s.full + 8 * stage, phase, wb)) {
+            report_status(p.status, kStatusTimeoutMbarrier, copied ? 117 : 113, blocks, kb, 0, t);
             ok = false;
             break;
           }
           tcgen05_fence_after();
-          const uint32_t sa = s.base + stage * kStageBytes, sb = sa + kOperandBytes;
+          const uint32_t sa = s.base + (copied ? kGradStages : stage) * kStageBytes, sb = sa + kOperandBytes;
 #pragma unroll
           for (int k = 0; k < kBK / kUmmaK; ++k)
             umma_f16_pair(d, umma_smem_desc_sw128(sa + k * kUmmaK * 128, kHalfBytes, 1024),
                           umma_smem_desc_sw128(sb + k * kUmmaK * 128, kHalfBytes, 1024), idesc,
                           (kb | k) != 0 ? 1u : 0u);
-          umma_commit_pair(s.empty + 8 * stage, 3);
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          umma_commit_pair(copied ? s.tail_empty : s.empty + 8 * stage, 3);
+          if (copied) tail_phase ^= 1u;
+          else if (++stage == kGradStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
         umma_commit_pair(s.acc_full + 8 * acc, 3);
@@ -754,43 +755,35 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
   } else if (warp >= kThreads / 32) {
     // ------------- copying warps: the partial block at the end of an expert -------------
     // Thread c copies 16-byte chunk c % 8 of one half of the columns (c / 8 % 2) of the rows
-    // c / 16, c / 16 + 8, ... of both operands.  The arrival at the other CTA is a release at
-    // cluster scope, about a microsecond; it comes once per tile and runs ahead of the MMAs.  It
-    // goes to a barrier of the stage: experts with few rows have copied blocks in several stages
-    // at a time, and the stage's own use keeps the phases of its barrier apart.
+    // c / 16, c / 16 + 8, ... of both operands.
     const int c = threadIdx.x - kThreads, chunk = c & 7, h = (c >> 3) & 1, row = c >> 4;
-    const uint32_t dst = h * kHalfBytes + row * 128 + ((chunk ^ row) << 4);
-    uint32_t stage = 0, phase = 0;
-    bool ok = true;
-    for (int t = blockIdx.x >> 1; ok && t < total; t += step) {
+    const uint32_t dst = s.base + kGradStages * kStageBytes + h * kHalfBytes + row * 128 + ((chunk ^ row) << 4);
+    uint32_t phase = 0;
+    for (int t = blockIdx.x >> 1; t < total; t += step) {
       const int e = t / per_expert, local = t % per_expert;
       const int x_a = local / p.n_tiles * kTile + cta * 128 + h * 64 + chunk * 8;
       const int x_b = local % p.n_tiles * kTile + cta * 128 + h * 64 + chunk * 8;
       const int row0 = slot_bound(p.offsets, e, p.slots), row1 = slot_bound(p.offsets, e + 1, p.slots);
-      for (int r0 = row0; r0 < row1; r0 += kBK) {
-        ok = copiers_all(mbar_wait(s.empty + 8 * stage, phase ^ 1u, wb));
-        if (!ok) {
-          if (c == 0) report_status(p.status, kStatusTimeoutMbarrier, 115, 0, r0, 0, t);
-          break;
-        }
-        if (r0 + kBK > row1) {
-          const uint32_t sa = s.base + stage * kStageBytes + dst;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int64_t r = r0 + row + 8 * i;
-            const bool in_a = r < row1 && x_a < p.m, in_b = r < row1 && x_b < p.n;
-            copy_16(sa + i * 1024,
-                    static_cast<const char*>(p.a) + (in_a ? 2 * (r * p.lda + x_a) : 0), in_a);
-            copy_16(sa + kOperandBytes + i * 1024,
-                    static_cast<const char*>(p.b) + (in_b ? 2 * (r * p.ldb + x_b) : 0), in_b);
-          }
-          copy_wait_all();
-          fence_proxy_async_smem();
-          copiers_all(true);
-          if (c == 0) mbar_arrive_cluster(mapa_shared(s.tail + 8 * stage, 0));
-        }
-        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      const int rows = max(row1 - row0, 0);
+      if (rows % kBK == 0) continue;
+      if (!copiers_all(mbar_wait(s.tail_empty, phase ^ 1u, wb))) {
+        if (c == 0) report_status(p.status, kStatusTimeoutMbarrier, 115, 0, 0, 0, t);
+        break;
       }
+      const int r0 = row0 + rows / kBK * kBK;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t r = r0 + row + 8 * i;
+        const bool in_a = r < row1 && x_a < p.m, in_b = r < row1 && x_b < p.n;
+        copy_16(dst + i * 1024, static_cast<const char*>(p.a) + (in_a ? 2 * (r * p.lda + x_a) : 0), in_a);
+        copy_16(dst + kOperandBytes + i * 1024,
+                static_cast<const char*>(p.b) + (in_b ? 2 * (r * p.ldb + x_b) : 0), in_b);
+      }
+      copy_wait_all();
+      fence_proxy_async_smem();
+      copiers_all(true);
+      if (c == 0) mbar_arrive_cluster(mapa_shared(s.tail, 0));
+      phase ^= 1u;
     }
   } else if (warp >= 4) {
     // --------------------------------- epilogue ---------------------------------
