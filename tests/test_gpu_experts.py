@@ -203,6 +203,27 @@ def test_route_backward_unrouted_rows_are_zero():
 
 
 # ------------------------------------------------------------------------------ slot map
+def test_slots_of_a_very_large_batch():
+    """Beyond 256 CTAs the counts are summed by a kernel of their own."""
+    from tileccl_b200 import ops
+
+    tokens, k, experts = 150_003, 8, 300
+    ids = torch.randint(-3, experts, (tokens, k), device="cuda", generator=_gen(77)).int()
+    s = ops.expert_slots(ids, 290, first_expert=5)
+    flat = ids.reshape(-1).long() - 5
+    here = (flat >= 0) & (flat < 290)
+    key = torch.where(here, flat, torch.full_like(flat, 290))
+    order = torch.sort(key, stable=True).indices
+    used = int(here.sum())
+    counts = torch.bincount(key, minlength=291)[:290]
+    assert s.offsets.tolist() == [0] + counts.cumsum(0).tolist()
+    assert torch.equal(s.token_of_slot[:used].long(), order[:used] // k)
+    assert (s.token_of_slot[used:] == -1).all()
+    want = torch.full_like(flat, -1)
+    want[order[:used]] = torch.arange(used, device="cuda")
+    assert torch.equal(s.slot_of.reshape(-1).long(), want)
+
+
 @pytest.mark.parametrize("tokens, k, experts, first, local", [
     (0, 2, 4, 0, 4), (1, 1, 1, 0, 1), (1, 8, 64, 0, 64), (37, 3, 5, 1, 3), (512, 8, 8, 0, 8),
     (513, 8, 8, 2, 2), (2049, 2, 1024, 0, 1024), (5000, 6, 61, 60, 1), (20011, 8, 256, 128, 128)])
@@ -820,3 +841,17 @@ def test_malformed_maps_stay_in_bounds():
     d = ops.route_experts_backward(torch.ones(1, 2, device="cuda"), torch.zeros(1, 8, device="cuda"),
                                    i32([[8, -9]]))
     assert (d == 0).all()
+
+
+def test_weights_with_interleaved_experts():
+    """W[e] may lie between the rows of the others ([K, E, N] in memory)."""
+    from tileccl_b200 import ops
+
+    g = _gen(61)
+    base = _randn(g, 64, 3, 72, dtype=torch.float16)
+    W = base.transpose(0, 1)
+    slots = _make_slots(g, 20, 2, 3)
+    X = _randn(g, 20, 64, std=0.125, dtype=torch.float16)
+    assert torch.equal(ops.expert_gemm(X, W, slots), ops.expert_gemm(X, W.contiguous(), slots))
+    gx, gw = ops.expert_gemm_backward(_randn(g, 40, 72, dtype=torch.float16), X, W, slots)
+    assert gw.is_contiguous() and gw.shape == W.shape

@@ -30,6 +30,7 @@ struct SlotParams {
   int32_t* token_of_slot;   // [entries]
   int32_t* slot_of;         // [entries]
   int32_t* counts;          // [CTAs][experts], null with a single CTA
+  int32_t* totals;          // [experts], null unless `counts` has been summed over the CTAs
 };
 
 // Entries a lane keeps: a warp's segment is 32 * kPerLane long, a CTA's run kRun.
@@ -78,6 +79,39 @@ __global__ void __launch_bounds__(kSlotThreads) expert_slot_count_kernel(const S
   }
 }
 
+// One CTA per expert: its counts become sums over the earlier CTAs, `totals` their total.  Up to
+// kSumInPlace CTAs the placing kernel adds the rows up itself, which grows with their square.
+constexpr int64_t kSumInPlace = 256;
+
+__global__ void __launch_bounds__(kSlotThreads) expert_slot_sum_kernel(const SlotParams p, int32_t ctas) {
+  __shared__ int32_t warp_total[kSlotWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int e = blockIdx.x;
+  int32_t base = 0;
+  for (int32_t c0 = 0; c0 < ctas; c0 += kSlotThreads) {
+    const int32_t c = c0 + threadIdx.x;
+    int32_t* const at = p.counts + static_cast<int64_t>(c) * p.experts + e;
+    const int32_t n = c < ctas ? *at : 0;
+    int32_t scan = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t v = __shfl_up_sync(kAll, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) warp_total[warp] = scan;
+    __syncthreads();
+    int32_t before = base, all = 0;
+    for (int w = 0; w < kSlotWarps; ++w) {
+      if (w < warp) before += warp_total[w];
+      all += warp_total[w];
+    }
+    if (c < ctas) *at = before + scan - n;
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.totals[e] = base;
+}
+
 __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const SlotParams p) {
   extern __shared__ int32_t cnt[];                 // [warps][experts], [experts], [experts]
   int32_t* const all = cnt + kSlotWarps * p.experts;      // per expert: all entries
@@ -93,7 +127,15 @@ __global__ void __launch_bounds__(kSlotThreads) expert_slot_place_kernel(const S
   const int column = threadIdx.x - row * p.experts;
   constexpr int kPer = kMaxExperts / kSlotThreads;
   int32_t sum_all[kPer] = {}, sum_before[kPer] = {};
-  if (p.counts != nullptr && row < rows) {
+  if (p.totals != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = column + i * kSlotThreads;
+      if (row != 0 || e >= p.experts) continue;
+      sum_all[i] = p.totals[e];
+      sum_before[i] = p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e];
+    }
+  } else if (p.counts != nullptr && row < rows) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int e = column + i * kSlotThreads;
@@ -206,6 +248,7 @@ int64_t slot_ctas(int64_t entries) { return entries <= kRun ? 1 : (entries + kRu
 cudaError_t preload_expert_slot_kernels() {
   cudaFuncAttributes a;
   cudaError_t e = cudaFuncGetAttributes(&a, expert_slot_count_kernel);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_slot_sum_kernel);
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, expert_slot_place_kernel);
   return e;
 }
@@ -217,7 +260,8 @@ using namespace tileccl;
 extern "C" int tccl_expert_slots_workspace(int64_t entries, int32_t experts, int64_t* bytes) {
   TCCL_CHECK_ARG(bytes != nullptr, "null argument");
   const int64_t ctas = slot_ctas(entries);
-  *bytes = ctas > 1 ? ctas * experts * static_cast<int64_t>(sizeof(int32_t)) : 0;
+  const int64_t rows = ctas <= 1 ? 0 : ctas <= kSumInPlace ? ctas : ctas + 1;
+  *bytes = rows * experts * static_cast<int64_t>(sizeof(int32_t));
   return kOk;
 }
 
@@ -247,6 +291,11 @@ extern "C" int tccl_expert_slots(uint64_t ids, int64_t tokens, int32_t top_k, in
   TCCL_CHECK_CUDA(attrs_once());
   if (ctas > 1) {
     expert_slot_count_kernel<<<static_cast<unsigned>(ctas), kSlotThreads, slot_smem(experts), s>>>(p);
+    TCCL_CHECK_CUDA(cudaGetLastError());
+  }
+  if (ctas > kSumInPlace) {
+    p.totals = p.counts + ctas * experts;
+    expert_slot_sum_kernel<<<static_cast<unsigned>(experts), kSlotThreads, 0, s>>>(p, static_cast<int32_t>(ctas));
     TCCL_CHECK_CUDA(cudaGetLastError());
   }
   expert_slot_place_kernel<<<static_cast<unsigned>(ctas), kSlotThreads, slot_smem(experts), s>>>(p);

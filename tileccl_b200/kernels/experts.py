@@ -448,8 +448,11 @@ def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
     d.offsets = slots.offsets.data_ptr()
     d.x, d.w, d.out, d.dh = X.data_ptr(), W.data_ptr(), out.data_ptr(), _ptr(dh)
     d.ldx, d.ldw, d.ldo = _aligned("X", X), _aligned("W", W), _aligned("out", out)
-    d.w_expert = W.stride(0) if E > 1 else W.shape[1] * d.ldw
-    if d.w_expert < (W.shape[1] - 1) * d.ldw + W.shape[2] or d.w_expert % 8:
+    rows_w, cols_w = W.shape[1], W.shape[2]
+    d.w_expert = W.stride(0) if E > 1 else rows_w * d.ldw
+    apart = d.w_expert >= (rows_w - 1) * d.ldw + cols_w
+    between = d.w_expert >= cols_w and d.ldw >= (E - 1) * d.w_expert + cols_w   # [K, E, N] in memory
+    if not (apart or between) or d.w_expert % 8:
         raise ValueError("W's experts overlap or are not 16-byte aligned")
     d.ld_dh = 0 if dh is None else _aligned("grad_out", dh)
     d.status, d.wait_budget_ns = _status_ptr(X.device), _fg._config().wait_budget_ns
