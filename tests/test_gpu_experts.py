@@ -855,3 +855,76 @@ def test_weights_with_interleaved_experts():
     assert torch.equal(ops.expert_gemm(X, W, slots), ops.expert_gemm(X, W.contiguous(), slots))
     gx, gw = ops.expert_gemm_backward(_randn(g, 40, 72, dtype=torch.float16), X, W, slots)
     assert gw.is_contiguous() and gw.shape == W.shape
+
+
+def test_offsets_beyond_32_bits():
+    """Matrices of more than 2^31 elements: their last rows are the ones that are computed."""
+    from tileccl_b200 import ops
+
+    g = _gen(71)
+    T, K, N = 75_000, 64, 28_672                          # 2.15e9 elements of 16 bits
+    ids = torch.zeros(T, 1, dtype=torch.int32, device="cuda")
+    slots = ops.expert_slots(ids, 1)
+    x, w = _randn(g, T, K, std=0.125, dtype=torch.float16), _randn(g, 1, K, N, dtype=torch.float16)
+    y = ops.expert_gemm(x, w, slots)
+    assert y.numel() > 1 << 31
+    want = x[-300:].double() @ w[0].double()
+    bound = _sum_bound(x[-300:].double(), w[0].double(), K)
+    _within(y[-300:], want, bound + (want.abs() + bound) * _half_step(torch.float16))
+    weights = torch.rand(T, 1, device="cuda", generator=g)
+    out = ops.expert_combine(y, slots, weights)
+    want = weights[-5:].double() * y[-5:].double()
+    _within(out[-5:], want, want.abs() * (_half_step(torch.float16) + 2 ** -23) + 2 ** -25)
+    dh, dw = ops.expert_combine_backward(out, y, slots, weights)
+    want = weights[-5:].double() * out[-5:].double()
+    _within(dh[-5:], want, want.abs() * (_half_step(torch.float16) + 2 ** -23) + 2 ** -25)
+    prod = out[-5:].double() * y[-5:].double()
+    _within(dw[-5:], prod.sum(1, keepdim=True), N * 2 ** -24 * prod.abs().sum(1, keepdim=True))
+    # the wide matrix as the left operand, gathered and in slot order, and in the weight gradient
+    back = w.transpose(1, 2).contiguous()
+    del dh, out
+    z = ops.expert_gemm(y, back, slots)
+    assert torch.equal(z[-300:], ops.expert_gemm(y, back, slots, rows="slots")[-300:])
+    want = y[-300:].double() @ back[0].double()
+    bound = _sum_bound(y[-300:].double(), back[0].double(), N)
+    _within(z[-300:], want, bound + (want.abs() + bound) * _half_step(torch.float16))
+    few = torch.zeros_like(z)
+    few[-3:] = 1.0                                        # only the last rows reach the gradient
+    _, gw = ops.expert_gemm_backward(few, y, back, slots, rows="slots")
+    want = y[-3:].double().sum(0)[:, None].expand(N, K)
+    _within(gw[0], want, 3 * 2 ** -23 * y[-3:].double().abs().sum(0)[:, None]
+            + want.abs() * _half_step(torch.float16) + 2 ** -25)
+
+
+def test_padded_batch():
+    """Masked tokens take no part: NaN in their logits and rows reaches nothing, their result is
+    the residual alone, and the unmasked ones are those of the batch without them."""
+    from tileccl_b200 import ops
+
+    g = _gen(73)
+    T, E, H, F, k = 50, 8, 128, 128, 3
+    keep = torch.rand(T, device="cuda", generator=g) < 0.6
+    logits, x = _randn(g, T, E), _randn(g, T, H, dtype=torch.bfloat16)
+    w_gu = _randn(g, E, H, 2 * F, std=H ** -0.5, dtype=torch.bfloat16)
+    w_down = _randn(g, E, F, H, std=F ** -0.5, dtype=torch.bfloat16)
+
+    def layer(logits, x, mask):
+        weights, ids = ops.route_experts(logits, k, score="sigmoid", mask=mask)
+        slots = ops.expert_slots(ids, E)
+        h = ops.expert_gemm(x, w_gu, slots, epilogue="silu_gate")
+        y = ops.expert_gemm(h, w_down, slots, rows="slots")
+        return weights, ids, slots, y, ops.expert_combine(y, slots, weights)
+
+    alone = layer(logits[keep], x[keep], None)
+    logits[~keep], x[~keep] = math.nan, math.nan
+    weights, ids, slots, y, out = layer(logits, x, keep)
+    assert torch.equal(out[keep], alone[4]) and (out[~keep] == 0).all()
+    assert (ids[~keep] == -1).all() and (weights[~keep] == 0).all()
+    dout = _randn(g, T, H, dtype=torch.bfloat16)
+    dout[~keep] = math.nan
+    dy, dw = ops.expert_combine_backward(dout, y, slots, weights)
+    gx, gw = ops.expert_gemm_backward(dy, torch.zeros(T * k, F, device="cuda").bfloat16(), w_down, slots,
+                                      rows="slots")
+    dl = ops.route_experts_backward(dw, logits, ids, score="sigmoid")
+    assert (dw[~keep] == 0).all() and (dl[~keep] == 0).all() and torch.isfinite(dl).all()
+    assert torch.isfinite(gw).all() and torch.isfinite(gx[:int(slots.offsets[-1])]).all()
