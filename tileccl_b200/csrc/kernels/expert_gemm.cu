@@ -408,10 +408,14 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
     const int wide = min(kBand, tiles - band * kBand);
     const int ti = band * kBand + local % wide;
     it.f0 = local / wide * kTile;
-    const int per = ((rows + tiles - 1) / tiles + 31) & ~31;   // even shares, a multiple of 32
-    it.row0 = s.start[it.e] + ti * per;
-    it.rows = min(per, rows - ti * per);
-    it.n = (max(it.rows, 1) + 31) & ~31;
+    // The expert's rows in blocks of 32, shared out evenly: no tile is padded but the last.  (With
+    // every tile rounded up from an equal share 8192 tokens x top 2 of 8 experts, 4096 x 28672,
+    // took 2.75 ms instead of 2.52.)
+    const int blocks = (rows + 31) / 32, share = blocks / tiles, more = blocks - share * tiles;
+    const int first = (ti * share + min(ti, more)) * 32;
+    it.row0 = s.start[it.e] + first;
+    it.n = (share + (ti < more ? 1 : 0)) * 32;
+    it.rows = min(it.n, rows - first);
     return true;
   };
   Walker w = walk();
