@@ -310,7 +310,8 @@ def expert_slots(ids: torch.Tensor, num_experts: int, *, first_expert: int = 0,
             2 * n + num_experts + 1 + need // 4).split((n, n, num_experts + 1, need // 4))
         slot_of = slot_of.view(tokens, top_k)
         _launch("tccl_expert_slots", ids.data_ptr(), tokens, top_k, num_experts, first_expert,
-                offsets.data_ptr(), token_of_slot.data_ptr(), slot_of.data_ptr(), scratch.data_ptr() if need else 0, raw)
+                offsets.data_ptr(), token_of_slot.data_ptr(), slot_of.data_ptr(),
+                scratch.data_ptr() if need else 0, raw)
     slots = object.__new__(ExpertSlots)           # (its parts need no second check)
     slots.__dict__.update(offsets=offsets, token_of_slot=token_of_slot, slot_of=slot_of)
     return slots
