@@ -312,7 +312,10 @@ __device__ __forceinline__ void store_row8(void* base, int64_t i, bool bf16, con
 // The weights are the M operand (256 features per pair, 128 per CTA) and the tokens the N
 // operand: M is fixed to 256 by the pair form of the instruction while N may be any multiple
 // of 32, so an expert's tile is as wide as its rows need.  With the gate a CTA's 128 features
-// are 64 gate columns and the 64 up columns that belong to them.
+// are 64 gate columns and the 64 up columns that belong to them.  Bound by the tensor cores with
+// many rows per expert (16384 rows of 8 experts, 4096 x 28672: 2.52 ms, 1530 TFLOP/s; 1270 in a
+// long run, at the power limit) and by the weights' way from DRAM with few (64 rows of 64 experts,
+// 4096 x 3584: 154 us; 6018 rows of 61, 1792 x 4096: 162 us, 5.9 TB/s).
 //
 // Schedule: tile t goes to pair t mod P.  With few tokens the time is that of streaming the
 // weights, and a third of the SMs nearly draws the full memory bandwidth: only a last round with
