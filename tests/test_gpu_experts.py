@@ -928,3 +928,38 @@ def test_padded_batch():
     dl = ops.route_experts_backward(dw, logits, ids, score="sigmoid")
     assert (dw[~keep] == 0).all() and (dl[~keep] == 0).all() and torch.isfinite(dl).all()
     assert torch.isfinite(gw).all() and torch.isfinite(gx[:int(slots.offsets[-1])]).all()
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """No call before the capture: kernels, counters and status words are not there yet."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from tileccl_b200 import ops
+g = torch.Generator(device='cuda'); g.manual_seed(0)
+r = lambda *s: torch.randn(*s, device='cuda', generator=g)
+logits, x = r(5, 8), r(5, 4096).bfloat16()
+w_gu, w_down = (r(8, 4096, 256) / 64).bfloat16(), (r(8, 128, 4096) / 12).bfloat16()
+def layer():
+    w, ids = ops.route_experts(logits, 2)
+    s = ops.expert_slots(ids, 8)
+    h = ops.expert_gemm(x, w_gu, s, epilogue='silu_gate')
+    y = ops.expert_gemm(h, w_down, s, rows='slots')
+    out = ops.expert_combine(y, s, w, add=x)
+    dy, dw = ops.expert_combine_backward(out, y, s, w)
+    dx, dg = ops.expert_gemm_backward(dy, h, w_down, s, rows='slots')
+    return out, dx, dg, ops.route_experts_backward(dw, logits, ids)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = layer()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(captured, layer()))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

@@ -76,54 +76,64 @@ def _pitch(name: str, t) -> int:
 _HALF = (torch.float16, torch.bfloat16)
 
 
-# The raw handle of a device's current stream, without the Python object around it (1.2 us).
+# The raw handle of a device's current stream and the current device, without the Python objects
+# around them (a microsecond of a call's fourteen).
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else lambda index: torch.cuda.current_stream(index).cuda_stream
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") \
+    else torch.cuda.current_device
 
 
-class _On:
-    """Current device and stream of a launch; yields the raw stream.  Inputs that are used on
-    another stream than the current one are reported to the caching allocator.  (A class: as a
-    generator it took 4 us of a call's 20.)"""
+class _Elsewhere:
+    """Makes another device or stream than the current one current; inputs used on ``stream``
+    are reported to the caching allocator."""
 
-    __slots__ = ("stream", "inputs", "dev", "device_guard", "stream_guard")
+    def __init__(self, dev, stream, inputs):
+        self.guards = [torch.cuda.device(dev)]
+        if stream is not None:
+            if stream.device != dev:
+                raise ValueError(f"stream is on {stream.device}, the tensors are on {dev}")
+            for t in inputs:
+                if t is not None:
+                    t.record_stream(stream)
+            self.guards.append(torch.cuda.stream(stream))
+        for g in self.guards:
+            g.__enter__()
 
-    def __init__(self, stream, inputs):
-        self.stream, self.inputs, self.dev = stream, inputs, inputs[0].device
-        if self.dev.type != "cuda":
-            raise ValueError(f"the expert operators take CUDA tensors, got tensors on {self.dev}")
-        if stream is not None and stream.device != self.dev:
-            raise ValueError(f"stream is on {stream.device}, the tensors are on {self.dev}")
-        self.device_guard = self.stream_guard = None
+    def leave(self) -> None:
+        for g in reversed(self.guards):
+            g.__exit__(None, None, None)
 
-    def __enter__(self) -> int:
-        index = self.dev.index
-        if torch.cuda.current_device() != index:
-            self.device_guard = torch.cuda.device(index)
-            self.device_guard.__enter__()
-        if self.stream is None:
-            return _raw_stream(index)
-        for t in self.inputs:
-            if t is not None:
-                t.record_stream(self.stream)
-        self.stream_guard = torch.cuda.stream(self.stream)
-        self.stream_guard.__enter__()
-        return self.stream.cuda_stream
 
-    def __exit__(self, *exc):
-        if self.stream_guard is not None:
-            self.stream_guard.__exit__(*exc)
-        if self.device_guard is not None:
-            self.device_guard.__exit__(*exc)
-        return False
+def _enter(stream, *inputs):
+    """``(raw stream, guard)`` of a call on ``inputs``' device; the guard is None in the common
+    case that device and stream are current, and otherwise left when the call is done."""
+    index = inputs[0].get_device()
+    if index < 0:
+        raise ValueError(f"the expert operators take CUDA tensors, got tensors on {inputs[0].device}")
+    guard = None
+    if stream is not None or _current_device() != index:
+        guard = _Elsewhere(inputs[0].device, stream, inputs)
+    return _raw_stream(index), guard
 
 
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+_ENTRIES: dict = {}
+
+
 def _launch(fn: str, *args) -> None:
-    _native.call(fn, *args)
+    entry = _ENTRIES.get(fn)
+    if entry is None:
+        entry = getattr(_native.load(), fn, None)
+        if entry is None:
+            raise _native.NativeError(fn, -1, "symbol not present in this build of libtileccl_b200")
+        _ENTRIES[fn] = entry
+    rc = entry(*args)
+    if rc != 0:
+        _native.check(fn, rc)
     _fg.count_launches(1)
 
 
@@ -203,13 +213,17 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
         if mask.shape[0] != tokens:
             raise ValueError(f"mask has {mask.shape[0]} entries for {tokens} tokens")
     ld = _pitch("logits", logits)
-    with _On(stream, (logits, bias, mask)) as raw:
+    raw, guard = _enter(stream, logits, bias, mask)
+    try:
         weights = logits.new_empty((tokens, top_k), dtype=torch.float32)
         ids = logits.new_empty((tokens, top_k), dtype=torch.int32)
         _launch("tccl_expert_route", logits.data_ptr(), ld, _ptr(bias), _ptr(mask),
                 weights.data_ptr(), ids.data_ptr(), tokens, experts, top_k,
                 _LOGIT_DTYPES[logits.dtype], sig, groups, top_groups, by_max,
                 1 if renormalize else 0, scale, raw)
+    finally:
+        if guard is not None:
+            guard.leave()
     return weights, ids
 
 
@@ -229,11 +243,15 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids
         raise ValueError(f"ids {tuple(ids.shape)} and grad_weights {tuple(grad_weights.shape)} "
                          f"must both be {(tokens, top_k)}")
     ld = _pitch("logits", logits)
-    with _On(stream, (logits, ids, grad_weights)) as raw:
+    raw, guard = _enter(stream, logits, ids, grad_weights)
+    try:
         grad = logits.new_empty((tokens, experts))
         _launch("tccl_expert_route_backward", grad_weights.data_ptr(), logits.data_ptr(), ld,
                 ids.data_ptr(), grad.data_ptr(), tokens, experts, top_k,
                 _LOGIT_DTYPES[logits.dtype], sig, 1 if renormalize else 0, scale, raw)
+    finally:
+        if guard is not None:
+            guard.leave()
     return grad
 
 
@@ -252,6 +270,15 @@ class ExpertSlots:
     slot_of: torch.Tensor
 
     def __post_init__(self) -> None:
+        o, t, s = self.offsets, self.token_of_slot, self.slot_of
+        try:                                      # the usual case in few steps
+            if (o.dtype is t.dtype is s.dtype is torch.int32 and o.device == t.device == s.device
+                    and o.dim() == t.dim() == 1 and s.dim() == 2 and s.is_contiguous()
+                    and o.is_contiguous() and t.is_contiguous()
+                    and 2 <= o.shape[0] <= MAX_EXPERTS + 1 and t.shape[0] == s.numel()):
+                return
+        except AttributeError:
+            pass
         _check_tensor("offsets", self.offsets, 1, (torch.int32,), contiguous=True)
         dev = self.offsets.device
         _check_tensor("token_of_slot", self.token_of_slot, 1, (torch.int32,), dev, contiguous=True)
@@ -301,8 +328,8 @@ def expert_slots(ids: torch.Tensor, num_experts: int, *, first_expert: int = 0,
         raise ValueError(f"first_expert={first_expert} must not be negative")
     if top_k < 1 or tokens * top_k >= 1 << 31:
         raise ValueError(f"ids have an unsupported shape {tuple(ids.shape)}")
-    dev = ids.device
-    with _On(stream, (ids,)) as raw:
+    raw, guard = _enter(stream, ids)
+    try:
         n = tokens * top_k
         need = _slots_scratch(n, num_experts)
         # one allocation for the three parts and the scratch
@@ -312,6 +339,9 @@ def expert_slots(ids: torch.Tensor, num_experts: int, *, first_expert: int = 0,
         _launch("tccl_expert_slots", ids.data_ptr(), tokens, top_k, num_experts, first_expert,
                 offsets.data_ptr(), token_of_slot.data_ptr(), slot_of.data_ptr(),
                 scratch.data_ptr() if need else 0, raw)
+    finally:
+        if guard is not None:
+            guard.leave()
     slots = object.__new__(ExpertSlots)           # (its parts need no second check)
     slots.__dict__.update(offsets=offsets, token_of_slot=token_of_slot, slot_of=slot_of)
     return slots
@@ -495,7 +525,8 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
     if out is not None:
         _check_rows("out", out, shape, X, out_dtype)
         _refuse_overlap(out, X=X, W=W)
-    with _On(stream, (X, W, slots.offsets, slots.token_of_slot, out)) as raw:
+    raw, guard = _enter(stream, X, W, slots.offsets, slots.token_of_slot, out)
+    try:
         if out is None:
             out = X.new_empty(shape, dtype=out_dtype)
         # Tokens' rows are put in slot order by a copy kernel first.  (The product gathering them
@@ -503,6 +534,9 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
         # every size: 209 against 200 us for 8 tokens, 8.1 against 2.5 ms for 8192.)
         xs = _gather(X, slots, raw) if rows == "tokens" else X
         _product(xs, W, slots, out, b_is_nk, epi, None, raw)
+    finally:
+        if guard is not None:
+            guard.leave()
     return out
 
 
@@ -520,7 +554,8 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
     E, K, N, epi = _check_product(X, W, slots, rows, b_is_nk, epilogue)
     _check_rows("grad_out", grad_out, (slots.capacity, N // 2 if epi else N), X)
     S = slots.capacity
-    with _On(stream, (X, W, grad_out, slots.offsets, slots.token_of_slot, slots.slot_of)) as raw:
+    raw, guard = _enter(stream, X, W, grad_out, slots.offsets, slots.token_of_slot, slots.slot_of)
+    try:
         # (once in slot order for both products that read X)
         xs = _gather(X, slots, raw) if rows == "tokens" else X
         dy = grad_out
@@ -547,6 +582,9 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
         d.lda, d.ldb = _aligned("X", a), _aligned("X", b)
         d.status, d.wait_budget_ns = _status_ptr(X.device), _fg._config().wait_budget_ns
         _launch("tccl_expert_weight_grad", C.byref(d), raw)
+    finally:
+        if guard is not None:
+            guard.leave()
     return grad_X, grad_W
 
 
@@ -592,10 +630,14 @@ def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.
         ld_out = _check_rows("out", out, shape, H)
         same = add is not None and out.data_ptr() == add.data_ptr() and out.stride() == add.stride()
         _refuse_overlap(out, H=H, add=None if same else add, weights=weights)
-    with _On(stream, (H, weights, add, slots.slot_of, out)) as raw:
+    raw, guard = _enter(stream, H, weights, add, slots.slot_of, out)
+    try:
         if out is None:
             out = H.new_empty(shape)
         _combine(H, ld_h, slots, weights, add, ld_add, out, ld_out, raw)
+    finally:
+        if guard is not None:
+            guard.leave()
     return out
 
 
@@ -609,11 +651,15 @@ def expert_combine_backward(grad_out: torch.Tensor, H: torch.Tensor, slots: Expe
         raise ValueError("weights must be a 2-D tensor")
     ld_h = _check_combine(H, slots, weights)
     ld_dy = _check_rows("grad_out", grad_out, (slots.tokens, H.shape[1]), H)
-    with _On(stream, (H, weights, grad_out, slots.slot_of)) as raw:
+    raw, guard = _enter(stream, H, weights, grad_out, slots.slot_of)
+    try:
         grad_H = H.new_empty(H.shape)
         grad_weights = weights.new_empty(weights.shape)
         _launch("tccl_expert_combine_backward", grad_out.data_ptr(), ld_dy, H.data_ptr(), ld_h,
                 slots.slot_of.data_ptr(), weights.data_ptr(), grad_H.data_ptr(), H.shape[1],
                 grad_weights.data_ptr(),
                 slots.tokens, slots.capacity, slots.top_k, H.shape[1], _fg.dtype_code(H.dtype), raw)
+    finally:
+        if guard is not None:
+            guard.leave()
     return grad_H, grad_weights
