@@ -165,11 +165,11 @@ def test_native_entries_check_their_arguments():
         assert lib.tccl_expert_route(*args) == 1, (i, v)
     d = _native.ExpertGemm()
     fields = dict(dtype=0, epilogue=0, experts=3, w_nk=0, k=16, n=24, slots=8, offsets=64, x=64, w=64, out=64, dh=0, ldx=16, ldw=24, w_expert=384, ldo=24, partial=0,
-                  counters=0)
+                  counters=0, token_of_slot=0, x_slots=0, x_rows=0)
     for name, bad in [("dtype", 2), ("epilogue", 4), ("epilogue", 1), ("experts", 0),
                       ("experts", 1025), ("k", 12), ("n", 20), ("k", 0), ("ldx", 12), ("x", 72),
                       ("slots", -1), ("slots", 1 << 31), ("x", 0), ("offsets", 0),
-                      ("partial", 64)]:
+                      ("partial", 64), ("token_of_slot", 64)]:
         for k, v in fields.items():
             setattr(d, k, v)
         setattr(d, name, bad)

@@ -168,6 +168,9 @@ class ExpertGemm(C.Structure):
         ("w", C.c_uint64),
         ("out", C.c_uint64),
         ("dh", C.c_uint64),
+        ("token_of_slot", C.c_uint64),
+        ("x_slots", C.c_uint64),
+        ("x_rows", C.c_int64),
         ("ldx", C.c_int64),
         ("ldw", C.c_int64),
         ("w_expert", C.c_int64),

@@ -331,7 +331,10 @@ typedef struct TcclExpertGemm {
   int32_t experts, w_nk;      // w_nk: W is [experts, N, K], else [experts, K, N]
   int64_t k, n, slots;
   uint64_t offsets;           // int32[experts + 1]
-  uint64_t x, w, out, dh;     // x: row s belongs to slot s; dh: epilogue 2 only
+  uint64_t x, w, out, dh;     // dh: epilogue 2 only
+  uint64_t token_of_slot;     // 0: row s of x belongs to slot s; else int32[slots], x has one row
+  uint64_t x_slots;           // per token (x_rows of them) and is copied to x_slots [slots, k] first
+  int64_t x_rows;
   int64_t ldx, ldw, w_expert, ldo, ld_dh;   // pitches in elements
   uint64_t status;            // uint32[8] status words (0 = a wait that gave up is not reported)
   uint64_t partial, counters; // scratch of tccl_expert_gemm_scratch's sizes, 0 = none

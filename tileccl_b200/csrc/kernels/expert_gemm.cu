@@ -1015,7 +1015,7 @@ extern "C" int tccl_expert_gemm_scratch(int64_t slots, int64_t k, int64_t* parti
 
 extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   TCCL_CHECK_ARG(desc != nullptr, "null argument");
-  const TcclExpertGemm& d = *desc;
+  TcclExpertGemm d = *desc;
   TCCL_CHECK_ARG(d.dtype == 0 || d.dtype == 1, "dtype must be 0 (fp16) or 1 (bf16)");
   TCCL_CHECK_ARG(d.epilogue >= kNone && d.epilogue <= kFloat, "epilogue must be 0..3");
   TCCL_CHECK_ARG(d.experts >= 1 && d.experts <= kMaxExperts, "experts must be 1..1024");
@@ -1034,10 +1034,20 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   if (d.slots == 0) return kOk;
   TCCL_CHECK_ARG(d.x != 0 && d.w != 0 && d.out != 0 && d.offsets != 0, "null argument");
   TCCL_CHECK_ARG(d.epilogue != kSiluGateGrad || d.dh != 0, "null argument");
+  TCCL_CHECK_ARG(d.token_of_slot == 0 || (d.x_slots != 0 && d.x_slots % 16 == 0 && d.x_rows >= 1),
+                 "gathered rows need scratch");
   TCCL_CHECK_ARG(d.partial == 0 || (d.counters != 0 && d.partial % 16 == 0), "bad scratch");
   const int64_t f_tiles = (d.n + kTile - 1) / kTile, tiles = most_tiles(d.slots, d.experts, d.n);
   TCCL_CHECK_ARG(tiles < (int64_t(1) << 31), "too many tiles");
   TCCL_REQUIRE_DRIVER();
+  if (d.token_of_slot != 0) {
+    // the tokens' rows in slot order first
+    const int rc = tccl_expert_gather(d.x, d.ldx, d.x_rows, d.token_of_slot, d.x_slots, d.k, d.slots,
+                                      static_cast<int32_t>(d.k), stream);
+    if (rc) return rc;
+    d.x = d.x_slots;
+    d.ldx = d.k;
+  }
   const bool bf16 = d.dtype == 1;
   GemmParams p;
   int rc = weight_map(d, &p);

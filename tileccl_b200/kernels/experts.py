@@ -469,8 +469,9 @@ def _refuse_overlap(out, **inputs) -> None:
         raise ValueError(f"out overlaps {name}")
 
 
-def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
-    """One launch of the grouped product; every argument is checked already."""
+def _product(X, W, slots, out, b_is_nk, epi, dh, raw, gathered=None):
+    """One launch of the grouped product; every argument is checked already.  ``gathered``: scratch
+    for the rows of ``X`` in slot order, when it has one row per token."""
     E = W.shape[0]
     N, K = (W.shape[1], W.shape[2]) if b_is_nk else (W.shape[2], W.shape[1])
     d = _native.ExpertGemm()
@@ -478,6 +479,10 @@ def _product(X, W, slots, out, b_is_nk, epi, dh, raw):
     d.k, d.n, d.slots = K, N, slots.capacity
     d.offsets = slots.offsets.data_ptr()
     d.x, d.w, d.out, d.dh = X.data_ptr(), W.data_ptr(), out.data_ptr(), _ptr(dh)
+    if gathered is not None:
+        d.token_of_slot, d.x_slots = slots.token_of_slot.data_ptr(), gathered.data_ptr()
+        d.x_rows = X.shape[0]
+        _fg.count_launches(1)
     d.ldx, d.ldw, d.ldo = _aligned("X", X), _aligned("W", W), _aligned("out", out)
     rows_w, cols_w = W.shape[1], W.shape[2]
     d.w_expert = W.stride(0) if E > 1 else rows_w * d.ldw
@@ -532,8 +537,8 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
         # Tokens' rows are put in slot order by a copy kernel first.  (The product gathering them
         # itself, with the TMA unit's four rows per copy or through the threads, measured slower at
         # every size: 209 against 200 us for 8 tokens, 8.1 against 2.5 ms for 8192.)
-        xs = _gather(X, slots, raw) if rows == "tokens" else X
-        _product(xs, W, slots, out, b_is_nk, epi, None, raw)
+        gathered = X.new_empty((slots.capacity, K)) if rows == "tokens" else None
+        _product(X, W, slots, out, b_is_nk, epi, None, raw, gathered)
     finally:
         if guard is not None:
             guard.leave()
