@@ -166,6 +166,8 @@ constexpr int kGatherRows = 4;
 __global__ void __launch_bounds__(kThreads) expert_gather_kernel(
     const uint4* x, int64_t x_ld, int64_t x_rows, const int32_t* token_of_slot, uint4* out,
     int64_t out_ld, int64_t slots, int32_t vecs) {
+  // a product that reads the rows may set itself up meanwhile (it waits for this kernel's end)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kGatherRows;
   const int v = blockIdx.y * kThreads + threadIdx.x;
   if (v >= vecs) return;

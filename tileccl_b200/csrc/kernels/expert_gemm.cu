@@ -364,6 +364,10 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
   list_tiles(s, p.offsets, p.slots, p.experts,
              [&](int rows) { return (rows + kTile - 1) / kTile * p.f_tiles; });
   const uint32_t tmem_base = pipe_meet(s);
+  // Behind the row copy this kernel may have been scheduled while that still runs (it touches
+  // nothing but x; what came before it, the offsets among it, was complete when it began).  One
+  // token of 2 experts of 4096 x 28672: 80 -> 78 us, of 8 of 4096 x 3584: 44.2 -> 43.7.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   WaitBudget wb;
   wb.start(p.budget_ns, s.words + 1);
 
@@ -954,19 +958,21 @@ cudaError_t attrs_once(int* sms) {
 
 template <typename P>
 cudaError_t launch_pairs(void (*kernel)(const P), const P& p, int pairs, int threads, int smem,
-                         cudaStream_t stream) {
+                         cudaStream_t stream, bool chained) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = chained ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -1082,7 +1088,7 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
       d.slots <= kFewTokens ? gemm_kernel<true>(d.epilogue) : gemm_kernel<false>(d.epilogue);
   TCCL_CHECK_CUDA(launch_pairs(kernel, p, pairs,
                                kThreads, kGemmSmem,
-                               reinterpret_cast<cudaStream_t>(stream)));
+                               reinterpret_cast<cudaStream_t>(stream), d.token_of_slot != 0));
   return kOk;
 }
 
@@ -1146,6 +1152,6 @@ extern "C" int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_
   TCCL_CHECK_CUDA(attrs_once(&sms));
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
   TCCL_CHECK_CUDA(launch_pairs(&expert_weight_grad_kernel, p, pairs, kThreads + kCopyThreads, kGradSmem,
-                               reinterpret_cast<cudaStream_t>(stream)));
+                               reinterpret_cast<cudaStream_t>(stream), false));
   return kOk;
 }
