@@ -4,6 +4,8 @@ Shapes, types and ranges are checked before the device is touched, so plain CPU 
 every refusal; a call that passes them all is refused for its device."""
 
 import ctypes as C
+import threading
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -198,3 +200,98 @@ def test_moe_block_refusals(change):
     args.update(change)
     with pytest.raises(ValueError):
         TPMoE(_Rank(), **args)
+
+
+# ----------------------------------------------------- state shared by host threads
+def _together(call, arguments):
+    """``call`` on every one of ``arguments``, each in a thread of its own."""
+    results = [None] * len(arguments)
+
+    def one(i):
+        results[i] = call(*arguments[i])
+
+    threads = [threading.Thread(target=one, args=(i,)) for i in range(len(arguments))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return results
+
+
+def _meet(barrier):
+    """Waits for the other thread, unless a lock keeps it away."""
+    try:
+        barrier.wait(0.5)
+    except threading.BrokenBarrierError:
+        pass
+
+
+@pytest.fixture
+def shared_state(monkeypatch):
+    from tileccl_b200.kernels import experts
+
+    monkeypatch.setattr(experts, "_ARENAS", {})
+    monkeypatch.setattr(experts, "_STATUS", {}, raising=False)
+    monkeypatch.setattr(experts, "_stream_key", lambda raw: raw, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return experts
+
+
+@pytest.mark.parametrize("streams", [(1001, 1001), (1001, 1002)])
+def test_first_products_of_two_threads_share_one_arena(shared_state, monkeypatch, streams):
+    """Both threads find no counters yet: one arena is made and kept, so that no address that was
+    handed out loses its memory."""
+    experts, made, meet = shared_state, [], threading.Barrier(2)
+
+    class Arena:
+        def __init__(self, *_):
+            made.append(self)
+            _meet(meet)
+            self.by_stream, self.used = {}, 1 << 20
+
+        def take(self, nbytes):
+            self.used += nbytes
+            return self.used
+
+    monkeypatch.setattr(experts, "_CounterArena", Arena)
+    got = _together(experts._counters, [(SimpleNamespace(index=7), raw, 128) for raw in streams])
+    assert len(made) == 1 and experts._ARENAS[7] is made[0]
+    kept = made[0].by_stream
+    assert [address for address, _ in got] == [kept[raw] for raw in streams]
+    assert (got[0][0] == got[1][0]) == (streams[0] == streams[1])
+
+
+def test_two_threads_never_get_the_same_counters(shared_state):
+    """A piece that one thread is about to take is not given to another."""
+    experts, meet = shared_state, threading.Barrier(2)
+
+    class Arena(experts._CounterArena):
+        def __init__(self):
+            self.words, self.address = torch.zeros(4096, dtype=torch.uint8), 1 << 20
+            self.by_stream, self.at = {}, 0
+
+        @property
+        def used(self):
+            at = self.at
+            _meet(meet)
+            return at
+
+        @used.setter
+        def used(self, value):
+            self.at = value
+
+    experts._ARENAS[7] = Arena()
+    got = _together(experts._counters, [(SimpleNamespace(index=7), raw, 128) for raw in (1001, 1002)])
+    assert abs(got[0][0] - got[1][0]) >= 128
+
+
+def test_status_words_of_two_threads_are_the_same(shared_state, monkeypatch):
+    experts, meet, zeros = shared_state, threading.Barrier(2), torch.zeros
+
+    def slow(*shape, device=None, **kw):
+        _meet(meet)
+        return zeros(*shape, **kw)
+
+    monkeypatch.setattr(torch, "zeros", slow)
+    got = _together(experts._status_ptr, [(SimpleNamespace(index=7),)] * 2)
+    assert got[0] == got[1] == experts._STATUS[7].data_ptr()

@@ -21,6 +21,7 @@ are allocated on that stream; the caller orders it behind the work that produced
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from dataclasses import dataclass
 from functools import lru_cache
 from typing import Optional
@@ -137,6 +138,9 @@ def _launch(fn: str, *args) -> None:
     _fg.count_launches(1)
 
 
+# Held while per-device state is made or handed out: host threads may make their first calls together.
+_STATE_LOCK = threading.Lock()
+
 _STATUS: dict = {}
 
 
@@ -146,7 +150,10 @@ def _status_ptr(dev: torch.device) -> int:
     if t is None:
         if torch.cuda.is_current_stream_capturing():
             return 0                      # (cannot be cleared inside a capture: not reported)
-        t = _STATUS[dev.index] = torch.zeros(_fg.STATUS_WORDS, dtype=torch.int32, device=dev)
+        with _STATE_LOCK:
+            t = _STATUS.get(dev.index)
+            if t is None:
+                t = _STATUS[dev.index] = torch.zeros(_fg.STATUS_WORDS, dtype=torch.int32, device=dev)
     return t.data_ptr()
 
 
@@ -408,7 +415,7 @@ class _CounterArena:
         self.used, self.by_stream = 0, {}
 
     def take(self, nbytes: int) -> int:
-        """Address of a new piece, 0 when none is left."""
+        """Address of a new piece, 0 when none is left (under the lock: no piece is given twice)."""
         at = self.used
         if at + nbytes > self.BYTES:
             return 0
@@ -422,22 +429,23 @@ _ARENAS: dict = {}
 def _counters(dev, raw, nbytes):
     """(address, tensor to keep until the launch) of zeroed counters for one product."""
     arena = _ARENAS.get(dev.index)
-    if torch.cuda.is_current_stream_capturing():
-        address = arena.take(nbytes) if arena is not None else 0
-        if address:
-            return address, None
-        t = torch.zeros(nbytes, dtype=torch.uint8, device=dev)      # zeroed by the graph itself
-        return t.data_ptr(), t
-    if arena is None:
-        arena = _ARENAS[dev.index] = _CounterArena(dev)
-    address = arena.by_stream.get(raw)
+    capturing = torch.cuda.is_current_stream_capturing()
+    address = None if capturing or arena is None else arena.by_stream.get(raw)
     if address is None:
-        address = arena.take(nbytes)
-        if not address:
-            t = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-            return t.data_ptr(), t
-        arena.by_stream[raw] = address
-    return address, None
+        with _STATE_LOCK:
+            arena = _ARENAS.get(dev.index)
+            if capturing:
+                address = arena.take(nbytes) if arena is not None else 0
+            else:
+                if arena is None:
+                    arena = _ARENAS[dev.index] = _CounterArena(dev)
+                address = arena.by_stream.get(raw) or arena.take(nbytes)
+                if address:
+                    arena.by_stream[raw] = address
+    if address:
+        return address, None
+    t = torch.zeros(nbytes, dtype=torch.uint8, device=dev)          # in a capture: by the graph itself
+    return t.data_ptr(), t
 
 
 def _gather(X, slots, raw):
