@@ -295,3 +295,22 @@ def test_status_words_of_two_threads_are_the_same(shared_state, monkeypatch):
     monkeypatch.setattr(torch, "zeros", slow)
     got = _together(experts._status_ptr, [(SimpleNamespace(index=7),)] * 2)
     assert got[0] == got[1] == experts._STATUS[7].data_ptr()
+
+
+@pytest.mark.parametrize("setting, budget", [("3000", 2_000_000_000), ("5000000", 5_000_000_000),
+                                             (None, 2_000_000_000)])
+def test_a_short_budget_for_peers_does_not_end_products(monkeypatch, setting, budget):
+    """Products wait for no peer: what the configuration grants a peer only ever lengthens them."""
+    from tileccl_b200.kernels import experts
+
+    if setting is None:
+        monkeypatch.delenv("TILECCL_WAIT_BUDGET_US", raising=False)
+    else:
+        monkeypatch.setenv("TILECCL_WAIT_BUDGET_US", setting)
+    seen = []
+    monkeypatch.setattr(experts, "_launch", lambda fn, desc, raw: seen.append(desc._obj.wait_budget_ns))
+    monkeypatch.setattr(experts, "_status_ptr", lambda dev: 0)
+    monkeypatch.setattr(experts, "_scratch_sizes", lambda *args: (0, 0))
+    half = lambda *shape: torch.zeros(*shape, dtype=torch.float16)
+    experts._product(half(4, 16), half(3, 16, 24), _slots(), half(8, 24), False, 0, None, 0)
+    assert seen == [budget]

@@ -963,3 +963,21 @@ assert all(torch.equal(a, b) for a, b in zip(captured, layer()))
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_waits_grow_with_the_work(monkeypatch):
+    """Products that run for far longer than the budget of their waits end well: the kernels add
+    100 us per K block and tile of an SM pair to it."""
+    from tileccl_b200 import ops
+    from tileccl_b200.kernels import experts
+
+    g = _gen(81)
+    dtype, T, E, K, N = torch.bfloat16, 4096, 4, 2048, 8192
+    slots = _make_slots(g, T, 2, E)
+    X, W = _randn(g, T, K, dtype=dtype), _randn(g, E, K, N, std=K ** -0.5, dtype=dtype)
+    dY = _randn(g, T * 2, N, dtype=dtype)
+    want = [ops.expert_gemm(X, W, slots), *ops.expert_gemm_backward(dY, X, W, slots)]
+    monkeypatch.setattr(experts, "_wait_budget_ns", lambda: 1)          # (0 would be two seconds)
+    got = [ops.expert_gemm(X, W, slots), *ops.expert_gemm_backward(dY, X, W, slots)]
+    ops.check_expert_status()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

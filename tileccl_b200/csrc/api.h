@@ -338,7 +338,8 @@ typedef struct TcclExpertGemm {
   int64_t ldx, ldw, w_expert, ldo, ld_dh;   // pitches in elements
   uint64_t status;            // uint32[8] status words (0 = a wait that gave up is not reported)
   uint64_t partial, counters; // scratch of tccl_expert_gemm_scratch's sizes, 0 = none
-  uint64_t wait_budget_ns;    // of every wait inside the kernel, 0 = 2 s
+  uint64_t wait_budget_ns;    // time until the kernel's waits give up, to which it adds 100 us per
+                              // K block and tile of an SM pair's share; 0 = 2 s
 } TcclExpertGemm;
 int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream);
 // Scratch with which a product shares its tiles evenly among the SMs (0 bytes: it would not
@@ -353,7 +354,7 @@ typedef struct TcclExpertWeightGrad {
   int64_t m, n, slots;
   uint64_t offsets, a, b, out;
   int64_t lda, ldb;
-  uint64_t status, wait_budget_ns;
+  uint64_t status, wait_budget_ns;  // as in TcclExpertGemm
 } TcclExpertWeightGrad;
 int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_t stream);
 

@@ -157,10 +157,21 @@ def _status_ptr(dev: torch.device) -> int:
     return t.data_ptr()
 
 
+_MIN_BUDGET_NS = 2_000_000_000
+
+
+def _wait_budget_ns() -> int:
+    """Budget of a product's waits.  They wait for the kernel's own copies and products, never for
+    a peer, so ``TILECCL_WAIT_BUDGET_US`` can only lengthen them: a budget that suits peers would
+    end long products that nothing is wrong with."""
+    return max(_fg._config().wait_budget_ns, _MIN_BUDGET_NS)
+
+
 def check_expert_status(device=None) -> None:
     """Synchronise and raise :class:`TileCCLTimeoutError` if a wait inside a grouped product on
-    ``device`` (default: the current one) ran out of its budget (two seconds, or
-    ``TILECCL_WAIT_BUDGET_US``) since the last check; the results of that call are undefined."""
+    ``device`` (default: the current one) gave up since the last check; the results of that call
+    are undefined.  A product gives up two seconds (``TILECCL_WAIT_BUDGET_US`` if that is longer)
+    and some hundred times its own running time after it began."""
     dev = torch.device("cuda" if device is None else device)
     t = _STATUS.get(torch.cuda.current_device() if dev.index is None else dev.index)
     if t is not None:
@@ -499,7 +510,7 @@ def _product(X, W, slots, out, b_is_nk, epi, dh, raw, gathered=None):
     if not (apart or between) or d.w_expert % 8:
         raise ValueError("W's experts overlap or are not 16-byte aligned")
     d.ld_dh = 0 if dh is None else _aligned("grad_out", dh)
-    d.status, d.wait_budget_ns = _status_ptr(X.device), _fg._config().wait_budget_ns
+    d.status, d.wait_budget_ns = _status_ptr(X.device), _wait_budget_ns()
     partial_bytes, counter_bytes = _scratch_sizes(X.device.index, d.slots, K)
     partial = None
     if partial_bytes:
@@ -593,7 +604,7 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
         d.m, d.n = a.shape[1], b.shape[1]
         d.a, d.b, d.out = a.data_ptr(), b.data_ptr(), grad_W.data_ptr()
         d.lda, d.ldb = _aligned("X", a), _aligned("X", b)
-        d.status, d.wait_budget_ns = _status_ptr(X.device), _fg._config().wait_budget_ns
+        d.status, d.wait_budget_ns = _status_ptr(X.device), _wait_budget_ns()
         _launch("tccl_expert_weight_grad", C.byref(d), raw)
     finally:
         if guard is not None:

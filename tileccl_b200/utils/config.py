@@ -35,7 +35,7 @@ class RuntimeConfig:
     dynamic_tiles: bool = False            # TILECCL_DYNAMIC_TILES: tiles handed to CTAs from a global counter
     rs_cta_pairs: Optional[bool] = None    # TILECCL_RS_CTA_PAIRS: kernel form of a multi-rank reduce-scatter (None = measured choice)
     rs_own_lag: Optional[int] = None       # TILECCL_RS_OWN_LAG: rounds the own rows trail (None = heuristic)
-    wait_budget_us: Optional[float] = None  # TILECCL_WAIT_BUDGET_US: budget of every device wait (None = 2 s)
+    wait_budget_us: Optional[float] = None  # TILECCL_WAIT_BUDGET_US: budget of every device wait (None = 2 s; the expert products' at least that)
     # NVLS / multicast
     disable_nvls: bool = False             # TILECCL_DISABLE_NVLS
     force_nvls: bool = False               # TILECCL_FORCE_NVLS: also with two ranks
