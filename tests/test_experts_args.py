@@ -239,23 +239,23 @@ def shared_state(monkeypatch):
 
 @pytest.mark.parametrize("streams", [(1001, 1001), (1001, 1002)])
 def test_first_products_of_two_threads_share_one_arena(shared_state, monkeypatch, streams):
-    """Both threads find no counters yet: one arena is made and kept, so that no address that was
-    handed out loses its memory."""
+    """Both threads find no counters yet: one arena is made and kept, so that no piece is handed out
+    twice."""
     experts, made, meet = shared_state, [], threading.Barrier(2)
 
-    class Arena:
-        def __init__(self, *_):
+    class Arena(experts._CounterArena):
+        def __init__(self, *args):
             made.append(self)
             _meet(meet)
-            self.by_stream, self.used = {}, 1 << 20
+            super().__init__(*args)
 
-        def take(self, nbytes):
-            self.used += nbytes
-            return self.used
+    def state(fn, status, counters, nbytes):
+        status._obj.value, counters._obj.value, nbytes._obj.value = 64, 4096, 4096
 
     monkeypatch.setattr(experts, "_CounterArena", Arena)
+    monkeypatch.setattr(experts._native, "call", state)
     got = _together(experts._counters, [(SimpleNamespace(index=7), raw, 128) for raw in streams])
-    assert len(made) == 1 and experts._ARENAS[7] is made[0]
+    assert len(made) == 1 and experts._ARENAS[7] is made[0] and experts._STATUS[7] == 64
     kept = made[0].by_stream
     assert [address for address, _ in got] == [kept[raw] for raw in streams]
     assert (got[0][0] == got[1][0]) == (streams[0] == streams[1])
@@ -267,8 +267,7 @@ def test_two_threads_never_get_the_same_counters(shared_state):
 
     class Arena(experts._CounterArena):
         def __init__(self):
-            self.words, self.address = torch.zeros(4096, dtype=torch.uint8), 1 << 20
-            self.by_stream, self.at = {}, 0
+            self.address, self.BYTES, self.by_stream, self.at = 1 << 20, 4096, {}, 0
 
         @property
         def used(self):
@@ -285,16 +284,35 @@ def test_two_threads_never_get_the_same_counters(shared_state):
     assert abs(got[0][0] - got[1][0]) >= 128
 
 
-def test_status_words_of_two_threads_are_the_same(shared_state, monkeypatch):
-    experts, meet, zeros = shared_state, threading.Barrier(2), torch.zeros
+def test_status_words_come_with_the_arena(shared_state, monkeypatch):
+    """Looked up once by whoever is first, and the arena that pieces were taken from stays."""
+    experts, calls, meet = shared_state, [], threading.Barrier(2)
 
-    def slow(*shape, device=None, **kw):
+    def state(fn, status, counters, nbytes):
+        calls.append(fn)
         _meet(meet)
-        return zeros(*shape, **kw)
+        status._obj.value, counters._obj.value, nbytes._obj.value = 64, 4096, 4096
 
-    monkeypatch.setattr(torch, "zeros", slow)
-    got = _together(experts._status_ptr, [(SimpleNamespace(index=7),)] * 2)
-    assert got[0] == got[1] == experts._STATUS[7].data_ptr()
+    monkeypatch.setattr(experts._native, "call", state)
+    dev = SimpleNamespace(index=7)
+    assert _together(experts._status_ptr, [(dev,)] * 2) == [64, 64]
+    arena = experts._ARENAS[7]
+    experts._counters(dev, 1001, 128)
+    assert experts._status_ptr(dev) == 64 and experts._ARENAS[7] is arena and len(calls) == 1
+
+
+def test_a_captured_first_product_reports_and_owns_its_counters(shared_state, monkeypatch):
+    experts = shared_state
+
+    def state(fn, status, counters, nbytes):
+        status._obj.value, counters._obj.value, nbytes._obj.value = 64, 4096, 4096
+
+    monkeypatch.setattr(experts._native, "call", state)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    dev = SimpleNamespace(index=7)
+    assert experts._status_ptr(dev) == 64
+    first, second = experts._counters(dev, 1001, 128), experts._counters(dev, 1001, 128)
+    assert first[0] != second[0] and 4096 <= min(first[0], second[0]) and experts._ARENAS[7].by_stream == {}
 
 
 @pytest.mark.parametrize("setting, budget", [("3000", 2_000_000_000), ("5000000", 5_000_000_000),

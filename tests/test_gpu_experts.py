@@ -981,3 +981,69 @@ def test_waits_grow_with_the_work(monkeypatch):
     got = [ops.expert_gemm(X, W, slots), *ops.expert_gemm_backward(dY, X, W, slots)]
     ops.check_expert_status()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_captured_first_product_has_status_words():
+    """A graph captured before any eager product reports to the words that eager calls report to,
+    and its counters are the device's own."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from tileccl_b200 import ops
+from tileccl_b200.kernels import experts
+x, w = torch.ones(2, 4096, device='cuda').half(), torch.ones(2, 4096, 256, device='cuda').half()
+slots = ops.expert_slots(torch.tensor([[0], [1]], dtype=torch.int32, device='cuda'), 2)
+seen, launch = [], experts._launch
+def record(fn, *args):
+    if fn == 'tccl_expert_gemm':
+        seen.append((args[0]._obj.status, args[0]._obj.counters))
+    launch(fn, *args)
+experts._launch = record
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ops.expert_gemm(x, w, slots)
+for _ in range(2):
+    graph.replay()
+z = ops.expert_gemm(x, w, slots)
+ops.check_expert_status()
+assert torch.equal(y, z) and (y == 4096).all()
+(s0, c0), (s1, c1) = seen
+assert s0 == s1 != 0 and c0 != c1 and abs(c0 - c1) < 1 << 20
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_a_reported_wait_is_raised_once_and_counters_are_cleared():
+    """What a product that gave up leaves behind (written here by hand: a status word and arrival
+    counters) is raised by the check and gone afterwards."""
+    from tileccl_b200 import ops
+    from tileccl_b200.kernels import experts
+
+    g = _gen(83)
+    x, W = _randn(g, 2, 4096, dtype=torch.float16), _randn(g, 4, 4096, 256, std=1 / 64, dtype=torch.float16)
+    slots = _make_slots(g, 2, 2, 4)
+    want = ops.expert_gemm(x, W, slots).clone()
+    ops.check_expert_status()
+
+    def words(address, n):
+        class Memory:
+            __cuda_array_interface__ = dict(shape=(n,), typestr="<i4", data=(address, False), version=3)
+
+        return torch.as_tensor(Memory(), device="cuda")
+
+    arena = experts._ARENAS[x.device.index]
+    counters = words(arena.address, arena.BYTES // 4)
+    assert (counters == 0).all()
+    counters[:arena.used // 4] = 1
+    words(experts._STATUS[x.device.index], 8)[0] = 2
+    with pytest.raises(ops.TileCCLTimeoutError):
+        ops.check_expert_status()
+    assert (counters == 0).all()
+    ops.check_expert_status()
+    assert torch.equal(ops.expert_gemm(x, W, slots), want)

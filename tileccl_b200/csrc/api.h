@@ -347,6 +347,12 @@ int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream);
 // calls that may run at the same time need scratch of their own.
 int tccl_expert_gemm_scratch(int64_t slots, int64_t k, int64_t* partial_bytes,
                              int64_t* counter_bytes);
+// The current device's status words (uint32[8]) and zeroed arrival counters, there from the start
+// and for good.
+int tccl_expert_state(uint64_t* status, uint64_t* counters, int64_t* counter_bytes);
+// Copies those status words to the host.  When a wait gave up, they and the counters, of which
+// the call may have left some behind, are cleared; nothing may be running then.
+int tccl_expert_status(uint32_t* words);
 
 // out[e] = sum over the slots s of expert e of a[s]^T b[s]: [experts, m, n] contiguous.
 typedef struct TcclExpertWeightGrad {

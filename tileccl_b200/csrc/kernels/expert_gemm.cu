@@ -59,6 +59,13 @@ constexpr int kGradStagingBytes = 4 * 2 * 4096;   // per epilogue warp two buffe
 constexpr int kGradSmem = kStages * kStageBytes + kGradStagingBytes + kCtlBytes + 1024;
 static_assert(kGemmSmem <= 232448 && kGradSmem <= 232448, "shared memory of one SM");
 
+// Status words and arrival counters of a device's products.  They are part of the module, zero when
+// it is loaded: a first call needs no allocation and may be captured.
+constexpr int kStatusWords = 8;
+constexpr int64_t kCounterBytes = 1 << 20;
+__device__ uint32_t g_status[kStatusWords];
+__device__ __align__(128) uint32_t g_counters[kCounterBytes / 4];
+
 struct GemmParams {
   CUtensorMap tma_w;          // five dimensions, see weight_map
   CUtensorMap tma_x[4];       // {K, rows}, boxes {64, 128}, {64, 64}, {64, 32}, {64, 16}
@@ -1026,6 +1033,35 @@ extern "C" int tccl_expert_gemm_scratch(int64_t slots, int64_t k, int64_t* parti
   if (slots <= 0 || slots > kSharedSlots || k < kSharedK) return kOk;
   *partial_bytes = pairs * 4 * 128 * partial_tokens(slots) * static_cast<int64_t>(sizeof(float));
   *counter_bytes = pairs * 4 * static_cast<int64_t>(sizeof(uint32_t));
+  return kOk;
+}
+
+extern "C" int tccl_expert_state(uint64_t* status, uint64_t* counters, int64_t* counter_bytes) {
+  TCCL_CHECK_ARG(status != nullptr && counters != nullptr && counter_bytes != nullptr, "null argument");
+  // (the first call may load the module, which a capture does not have to notice)
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  TCCL_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  void *s = nullptr, *c = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&s, g_status);
+  if (e == cudaSuccess) e = cudaGetSymbolAddress(&c, g_counters);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  TCCL_CHECK_CUDA(e);
+  *status = reinterpret_cast<uint64_t>(s);
+  *counters = reinterpret_cast<uint64_t>(c);
+  *counter_bytes = kCounterBytes;
+  return kOk;
+}
+
+extern "C" int tccl_expert_status(uint32_t* words) {
+  TCCL_CHECK_ARG(words != nullptr, "null argument");
+  TCCL_CHECK_CUDA(cudaMemcpyFromSymbol(words, g_status, sizeof(g_status)));
+  if (words[0] == 0) return kOk;
+  void *s = nullptr, *c = nullptr;
+  TCCL_CHECK_CUDA(cudaGetSymbolAddress(&s, g_status));
+  TCCL_CHECK_CUDA(cudaGetSymbolAddress(&c, g_counters));
+  TCCL_CHECK_CUDA(cudaMemset(s, 0, sizeof(g_status)));
+  TCCL_CHECK_CUDA(cudaMemset(c, 0, sizeof(g_counters)));
+  TCCL_CHECK_CUDA(cudaDeviceSynchronize());          // (other streams do not wait for these)
   return kOk;
 }
 

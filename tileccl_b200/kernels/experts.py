@@ -141,20 +141,45 @@ def _launch(fn: str, *args) -> None:
 # Held while per-device state is made or handed out: host threads may make their first calls together.
 _STATE_LOCK = threading.Lock()
 
-_STATUS: dict = {}
+_STATUS: dict = {}                        # device index -> address of its status words
+_ARENAS: dict = {}                        # device index -> its _CounterArena
+
+
+class _CounterArena:
+    """Zeroed arrival counters of one device's products.  Every call leaves its counters at zero.
+    Calls on one stream follow one another and share a piece; a captured call gets a piece of its
+    own for good, because its graph may be replayed beside anything else."""
+
+    def __init__(self, address: int, nbytes: int):
+        self.address, self.BYTES = address, nbytes        # (some 800 pieces)
+        self.used, self.by_stream = 0, {}
+
+    def take(self, nbytes: int) -> int:
+        """Address of a new piece, 0 when none is left (under the lock: no piece is given twice)."""
+        at = self.used
+        if at + nbytes > self.BYTES:
+            return 0
+        self.used = at + -(-nbytes // 128) * 128
+        return self.address + at
+
+
+def _device_state(index: int) -> None:
+    """Looks up the status words and counters of the current device, ``index`` (under the lock)."""
+    status, counters, nbytes = C.c_uint64(), C.c_uint64(), C.c_int64()
+    _native.call("tccl_expert_state", C.byref(status), C.byref(counters), C.byref(nbytes))
+    _ARENAS[index] = _CounterArena(counters.value, nbytes.value)
+    _STATUS[index] = status.value
 
 
 def _status_ptr(dev: torch.device) -> int:
     """Status words of a device's products (see :func:`check_expert_status`)."""
-    t = _STATUS.get(dev.index)
-    if t is None:
-        if torch.cuda.is_current_stream_capturing():
-            return 0                      # (cannot be cleared inside a capture: not reported)
+    address = _STATUS.get(dev.index)
+    if address is None:
         with _STATE_LOCK:
-            t = _STATUS.get(dev.index)
-            if t is None:
-                t = _STATUS[dev.index] = torch.zeros(_fg.STATUS_WORDS, dtype=torch.int32, device=dev)
-    return t.data_ptr()
+            if dev.index not in _STATUS:
+                _device_state(dev.index)
+            address = _STATUS[dev.index]
+    return address
 
 
 _MIN_BUDGET_NS = 2_000_000_000
@@ -173,12 +198,13 @@ def check_expert_status(device=None) -> None:
     are undefined.  A product gives up two seconds (``TILECCL_WAIT_BUDGET_US`` if that is longer)
     and some hundred times its own running time after it began."""
     dev = torch.device("cuda" if device is None else device)
-    t = _STATUS.get(torch.cuda.current_device() if dev.index is None else dev.index)
-    if t is not None:
-        torch.cuda.synchronize(t.device)
-        if int(t[0]) != 0 and t.device.index in _ARENAS:
-            _ARENAS[t.device.index].words.zero_()     # (an abandoned call may have left some behind)
-        _fg.raise_on_status(t)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    if index in _STATUS:
+        torch.cuda.synchronize(index)
+        words = (C.c_uint32 * _fg.STATUS_WORDS)()
+        with torch.cuda.device(index):
+            _native.call("tccl_expert_status", words)
+        _fg.raise_on_status(torch.tensor(list(words)))
 
 
 # -------------------------------------------------------------------------- routing
@@ -413,45 +439,20 @@ def _scratch_sizes(device: int, slots: int, k: int) -> tuple:
     return a.value, b.value
 
 
-class _CounterArena:
-    """Zeroed arrival counters of one device's products.  Every call leaves its counters at zero.
-    Calls on one stream follow one another and share a piece; a captured call gets a piece of its
-    own for good, because its graph may be replayed beside anything else."""
-
-    BYTES = 1 << 20                       # some 800 pieces
-
-    def __init__(self, dev):
-        self.words = torch.zeros(self.BYTES, dtype=torch.uint8, device=dev)
-        torch.cuda.current_stream(dev).synchronize()      # (once: other streams use it, too)
-        self.used, self.by_stream = 0, {}
-
-    def take(self, nbytes: int) -> int:
-        """Address of a new piece, 0 when none is left (under the lock: no piece is given twice)."""
-        at = self.used
-        if at + nbytes > self.BYTES:
-            return 0
-        self.used = at + -(-nbytes // 128) * 128
-        return self.words.data_ptr() + at
-
-
-_ARENAS: dict = {}
-
-
 def _counters(dev, raw, nbytes):
     """(address, tensor to keep until the launch) of zeroed counters for one product."""
-    arena = _ARENAS.get(dev.index)
     capturing = torch.cuda.is_current_stream_capturing()
+    arena = _ARENAS.get(dev.index)
     address = None if capturing or arena is None else arena.by_stream.get(raw)
     if address is None:
         with _STATE_LOCK:
-            arena = _ARENAS.get(dev.index)
-            if capturing:
-                address = arena.take(nbytes) if arena is not None else 0
-            else:
-                if arena is None:
-                    arena = _ARENAS[dev.index] = _CounterArena(dev)
-                address = arena.by_stream.get(raw) or arena.take(nbytes)
-                if address:
+            if dev.index not in _ARENAS:
+                _device_state(dev.index)
+            arena = _ARENAS[dev.index]
+            address = 0 if capturing else arena.by_stream.get(raw, 0)
+            if not address:
+                address = arena.take(nbytes)
+                if address and not capturing:
                     arena.by_stream[raw] = address
     if address:
         return address, None
