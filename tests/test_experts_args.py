@@ -232,7 +232,7 @@ def shared_state(monkeypatch):
 
     monkeypatch.setattr(experts, "_ARENAS", {})
     monkeypatch.setattr(experts, "_STATUS", {}, raising=False)
-    monkeypatch.setattr(experts, "_stream_key", lambda raw: raw, raising=False)
+    monkeypatch.setattr(experts, "_stream_key", lambda index, raw: raw, raising=False)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return experts
 
@@ -299,6 +299,22 @@ def test_status_words_come_with_the_arena(shared_state, monkeypatch):
     arena = experts._ARENAS[7]
     experts._counters(dev, 1001, 128)
     assert experts._status_ptr(dev) == 64 and experts._ARENAS[7] is arena and len(calls) == 1
+
+
+def test_streams_that_share_a_handle_do_not_share_counters(shared_state, monkeypatch):
+    """A handle that is given out again belongs to another stream, and the handle of the per-thread
+    default stream to one stream per thread."""
+    experts, numbers = shared_state, iter([41, 42, 41])
+    monkeypatch.setattr(experts, "_stream_key", lambda index, raw: (next(numbers),))
+    experts._ARENAS[7] = experts._CounterArena(4096, 4096)
+    dev = SimpleNamespace(index=7)
+    first, second, again = (experts._counters(dev, 1001, 128)[0] for _ in range(3))
+    assert first == again and abs(first - second) >= 128
+    zeros = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *shape, device=None, **kw: zeros(*shape, **kw))
+    (a, keep_a), (b, keep_b) = (experts._counters(dev, 2, 128) for _ in range(2))
+    assert a == keep_a.data_ptr() and b == keep_b.data_ptr() and a != b
+    assert experts._ARENAS[7].used == 256
 
 
 def test_a_captured_first_product_reports_and_owns_its_counters(shared_state, monkeypatch):

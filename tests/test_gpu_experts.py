@@ -1047,3 +1047,56 @@ def test_a_reported_wait_is_raised_once_and_counters_are_cleared():
     assert (counters == 0).all()
     ops.check_expert_status()
     assert torch.equal(ops.expert_gemm(x, W, slots), want)
+
+
+def test_streams_have_numbers_of_their_own():
+    """Also where the driver gives a destroyed stream's handle out again; products on the streams
+    of two host threads that are made and destroyed agree with the others."""
+    import ctypes as C
+    import threading
+
+    from tileccl_b200 import ops
+    from tileccl_b200.kernels import experts
+
+    torch.cuda.synchronize()
+    cudart = torch.cuda.cudart()
+
+    def key(stream):
+        with torch.cuda.stream(stream):
+            return experts._stream_key(stream.device.index, stream.cuda_stream)
+
+    lasting = [torch.cuda.default_stream(), torch.cuda.Stream(), torch.cuda.Stream(priority=-1)]
+    keys = [key(s) for s in lasting]
+    assert keys == [s.cuda_stream for s in lasting]
+    for _ in range(4):
+        handle = C.c_uint64()
+        assert int(cudart.cudaStreamCreate(C.addressof(handle))) == 0
+        stream = torch.cuda.ExternalStream(handle.value)
+        keys.append(key(stream))
+        assert key(stream) == keys[-1] != handle.value
+        assert int(cudart.cudaStreamDestroy(handle.value)) == 0
+    assert len(set(keys)) == len(keys)
+
+    g = _gen(87)
+    dtype, T, E, K, N = torch.bfloat16, 3, 8, 4608, 512
+    W = _randn(g, E, K, N, std=K ** -0.5, dtype=dtype)
+    data = [(_randn(g, T, K, dtype=dtype), _make_slots(g, T, 2, E)) for _ in range(2)]
+    want = [ops.expert_gemm(x, W, s).clone() for x, s in data]
+    torch.cuda.synchronize()
+    off = []
+
+    def work(i, stream):
+        with torch.cuda.stream(stream):
+            for _ in range(100):
+                got = ops.expert_gemm(data[i][0], W, data[i][1])
+                if not torch.equal(got, want[i]):
+                    off.append(i)
+
+    for streams in ([torch.cuda.Stream(), torch.cuda.Stream()], [torch.cuda.default_stream()] * 2):
+        threads = [threading.Thread(target=work, args=(i, s)) for i, s in enumerate(streams)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    assert off == []
+    ops.check_expert_status()

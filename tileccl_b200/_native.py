@@ -273,6 +273,7 @@ def _declare(lib: C.CDLL) -> None:
         "tccl_expert_gemm_scratch": [i64, i64, C.POINTER(i64), C.POINTER(i64)],
         "tccl_expert_state": [C.POINTER(u64), C.POINTER(u64), C.POINTER(i64)],
         "tccl_expert_status": [C.POINTER(u32)],
+        "tccl_stream_id": [u64, C.POINTER(u64)],
         "tccl_expert_weight_grad": [C.POINTER(ExpertWeightGrad), u64],
         "tccl_expert_gather": [u64, i64, i64, u64, u64, i64, i64, i32, u64],
         "tccl_expert_combine": [u64, i64, u64, u64, u64, i64, u64, i64, i64, i64, i32, i32, i32, i32,

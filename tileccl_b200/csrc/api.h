@@ -350,6 +350,8 @@ int tccl_expert_gemm_scratch(int64_t slots, int64_t k, int64_t* partial_bytes,
 // The current device's status words (uint32[8]) and zeroed arrival counters, there from the start
 // and for good.
 int tccl_expert_state(uint64_t* status, uint64_t* counters, int64_t* counter_bytes);
+// Number of a stream that no other stream of the process ever has (a handle may be given out again).
+int tccl_stream_id(uint64_t stream, uint64_t* id);
 // Copies those status words to the host.  When a wait gave up, they and the counters, of which
 // the call may have left some behind, are cleared; nothing may be running then.
 int tccl_expert_status(uint32_t* words);

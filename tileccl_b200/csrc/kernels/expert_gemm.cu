@@ -1052,6 +1052,14 @@ extern "C" int tccl_expert_state(uint64_t* status, uint64_t* counters, int64_t* 
   return kOk;
 }
 
+extern "C" int tccl_stream_id(uint64_t stream, uint64_t* id) {
+  TCCL_CHECK_ARG(id != nullptr, "null argument");
+  unsigned long long v = 0;
+  TCCL_CHECK_CUDA(cudaStreamGetId(reinterpret_cast<cudaStream_t>(stream), &v));
+  *id = v;
+  return kOk;
+}
+
 extern "C" int tccl_expert_status(uint32_t* words) {
   TCCL_CHECK_ARG(words != nullptr, "null argument");
   TCCL_CHECK_CUDA(cudaMemcpyFromSymbol(words, g_status, sizeof(g_status)));

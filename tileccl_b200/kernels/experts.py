@@ -439,21 +439,38 @@ def _scratch_sizes(device: int, slots: int, k: int) -> tuple:
     return a.value, b.value
 
 
+_PER_THREAD_STREAM = 2                    # the handle of every thread's own default stream
+
+
+def _stream_key(index: int, raw: int):
+    """What tells the current stream (handle ``raw``) of a device from every other one.  PyTorch
+    never destroys its own streams; the handle of another library's may be given out again while
+    the stream that had it is still at work, its number is not."""
+    if raw == 0 or torch.cuda.current_stream(index).stream_id != raw:
+        return raw
+    number = C.c_uint64()
+    _native.call("tccl_stream_id", raw, C.byref(number))
+    return (number.value,)
+
+
 def _counters(dev, raw, nbytes):
     """(address, tensor to keep until the launch) of zeroed counters for one product."""
     capturing = torch.cuda.is_current_stream_capturing()
     arena = _ARENAS.get(dev.index)
     address = None if capturing or arena is None else arena.by_stream.get(raw)
+    if address is None and raw == _PER_THREAD_STREAM and not capturing:
+        address = 0
     if address is None:
+        key = None if capturing else _stream_key(dev.index, raw)
         with _STATE_LOCK:
             if dev.index not in _ARENAS:
                 _device_state(dev.index)
             arena = _ARENAS[dev.index]
-            address = 0 if capturing else arena.by_stream.get(raw, 0)
+            address = 0 if capturing else arena.by_stream.get(key, 0)
             if not address:
                 address = arena.take(nbytes)
                 if address and not capturing:
-                    arena.by_stream[raw] = address
+                    arena.by_stream[key] = address
     if address:
         return address, None
     t = torch.zeros(nbytes, dtype=torch.uint8, device=dev)          # in a capture: by the graph itself
