@@ -156,6 +156,23 @@ def test_results_may_lie_beside_their_inputs_but_not_over_them():
         ops.expert_combine(H, s, None, pair[:, :16], add=pair[:, 8:])
 
 
+@pytest.mark.parametrize("part", ["offsets", "token_of_slot", "slot_of"])
+def test_results_may_not_lie_over_the_slot_map(part):
+    memory = torch.zeros(256, dtype=torch.int32)
+    parts = dict(offsets=torch.zeros(4, dtype=torch.int32), token_of_slot=torch.zeros(8, dtype=torch.int32),
+                 slot_of=torch.zeros(4, 2, dtype=torch.int32))
+    parts[part] = memory[20:20 + parts[part].numel()].view(parts[part].shape)
+    s = ops.ExpertSlots(**parts)
+    over = memory.view(torch.float16)
+    with pytest.raises(ValueError, match=f"overlaps slots.{part}"):
+        ops.expert_gemm(torch.zeros(4, 16).half(), torch.zeros(3, 16, 24).half(), s, over[:8 * 24].view(8, 24))
+    with pytest.raises(ValueError, match=f"overlaps slots.{part}"):
+        ops.expert_combine(torch.zeros(8, 16).half(), s, None, over[:4 * 16].view(4, 16))
+    with pytest.raises(ValueError, match="CUDA"):                # beside it
+        ops.expert_gemm(torch.zeros(4, 16).half(), torch.zeros(3, 16, 24).half(), s,
+                        over[64:64 + 8 * 24].view(8, 24))
+
+
 def test_native_entries_check_their_arguments():
     """The C entries refuse on their own (another binding may call them)."""
     lib = _native.load()

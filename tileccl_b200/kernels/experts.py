@@ -492,11 +492,12 @@ def _refuse_overlap(out, **inputs) -> None:
     a0, pitch = out.data_ptr(), out.stride(0) * out.element_size()
     a1 = a0 + ((out.shape[0] - 1) * out.stride(0) + out.shape[1]) * out.element_size()
     for name, t in inputs.items():
-        if t is None or t.numel() == 0 or out.numel() == 0:
+        if t is None:
             continue
-        b0 = t.data_ptr()
-        b1 = b0 + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-        if a0 >= b1 or b0 >= a1:
+        b0, count = t.data_ptr(), t.numel()
+        if count and not t.is_contiguous():
+            count = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+        if a0 >= b0 + count * t.element_size() or b0 >= a1 or count == 0 or out.numel() == 0:
             continue
         if t.dim() == 2 and t.shape[0] > 1 and out.shape[0] > 1 and t.stride(0) * t.element_size() == pitch:
             shift = (b0 - a0) % pitch
@@ -504,6 +505,11 @@ def _refuse_overlap(out, **inputs) -> None:
                     shift + t.shape[1] * t.element_size() <= pitch:
                 continue
         raise ValueError(f"out overlaps {name}")
+
+
+def _maps(slots) -> dict:
+    return {"slots.offsets": slots.offsets, "slots.token_of_slot": slots.token_of_slot,
+            "slots.slot_of": slots.slot_of}
 
 
 def _product(X, W, slots, out, b_is_nk, epi, dh, raw, gathered=None):
@@ -550,7 +556,7 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
     K]`` with ``b_is_nk``.  ``epilogue="silu_gate"`` takes every 256 columns of the product as
     128 gate columns followed by 128 up columns (``models.pack_gate_up`` of every expert) and
     writes ``silu(gate) * up``, half as wide.  Rows of ``out [tokens * top_k, N]`` behind the
-    last slot keep what they held.  ``out`` must not overlap an input.  ``out_dtype``:
+    last slot keep what they held.  ``out`` must not overlap an input, the slot map included.  ``out_dtype``:
     ``X.dtype`` (default, or that of ``out``) or, without the gate, ``torch.float32``.
     ``rows="tokens"`` takes scratch memory for ``tokens * top_k`` rows of ``X``.
     """
@@ -566,7 +572,7 @@ def expert_gemm(X: torch.Tensor, W: torch.Tensor, slots: ExpertSlots,
         epi = _EPI_FLOAT
     if out is not None:
         _check_rows("out", out, shape, X, out_dtype)
-        _refuse_overlap(out, X=X, W=W)
+        _refuse_overlap(out, X=X, W=W, **_maps(slots))
     raw, guard = _enter(stream, X, W, slots.offsets, slots.token_of_slot, out)
     try:
         if out is None:
@@ -662,7 +668,7 @@ def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.
     ``H [tokens * top_k, N]`` is slot-ordered (fp16 / bf16), ``weights`` fp32 ``[tokens,
     top_k]`` (None: all ones), ``add [tokens, N]`` a residual or a shared expert's output.
     Choices without a slot add nothing.  ``out`` may be ``add`` (in place) but must not overlap
-    ``H``.
+    another input, the slot map included.
     """
     ld_h = _check_combine(H, slots, weights)
     shape = (slots.tokens, H.shape[1])
@@ -671,7 +677,7 @@ def expert_combine(H: torch.Tensor, slots: ExpertSlots, weights: Optional[torch.
     if out is not None:
         ld_out = _check_rows("out", out, shape, H)
         same = add is not None and out.data_ptr() == add.data_ptr() and out.stride() == add.stride()
-        _refuse_overlap(out, H=H, add=None if same else add, weights=weights)
+        _refuse_overlap(out, H=H, add=None if same else add, weights=weights, **_maps(slots))
     raw, guard = _enter(stream, H, weights, add, slots.slot_of, out)
     try:
         if out is None:
