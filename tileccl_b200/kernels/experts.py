@@ -235,11 +235,12 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     experts, divided by their sum if ``renormalize``.
 
     Returns ``(weights, ids)``: fp32 and int32 ``[tokens, top_k]``, best first, ties to the
-    lower index.  The choice is exact (made in 64 bits where 32 cannot tell).  A logit or bias
-    of ``-inf`` takes an expert out; a token whose ``mask`` (bool ``[tokens]``) is false, or
-    that has fewer than ``top_k`` experts left, gets id -1 and weight 0 in the places that
-    stay empty.  A NaN among an unmasked row's logits makes the row's weights NaN (its ids
-    stay distinct and in range).
+    lower index.  The choice is exact (made in 64 bits where 32 cannot tell); weights are
+    computed in 32 bits, within a few 2^-24.  A logit or bias of ``-inf`` takes an expert out; a
+    token whose ``mask`` (bool ``[tokens]``) is false, or that has fewer than ``top_k`` experts
+    left, gets id -1 and weight 0 in the places that stay empty.  A NaN among an unmasked row's
+    logits makes the row's weights NaN (its ids stay distinct and in range).  Group counts that
+    are no power of two are right but slower: every row is then decided on 64-bit keys.
     """
     tokens, experts, sig, scale = _check_routing(logits, top_k, score, scale)
     if groups < 1 or groups > 32 or experts % groups:
@@ -594,10 +595,14 @@ def expert_gemm_backward(grad_out: torch.Tensor, X: torch.Tensor, W: torch.Tenso
     """``(grad_X, grad_W)`` of :func:`expert_gemm` for ``grad_out`` (shaped like its result).
 
     With ``epilogue="silu_gate"`` gate and up are computed again from ``X`` and ``W``, so the
-    forward pass keeps nothing.  ``grad_X`` has ``X``'s shape: with ``rows="tokens"`` the sum
-    over a token's slots (zero for a token without one), with ``rows="slots"`` one row per
-    slot, undefined behind the last slot.  ``grad_W`` has ``W``'s shape and is contiguous;
-    experts without a slot get zeros.
+    forward pass keeps nothing.  Their gradients are rounded to the operands' 16 bits before the two
+    products that read them, half a step per element (the tensor cores take no wider operand
+    beside a 16-bit one): in bf16 ``grad_X`` and ``grad_W`` are then 2.4e-3 off on the whole
+    instead of 1.7e-3, and in fp16 they have to stay below 65504.
+
+    ``grad_X`` has ``X``'s shape: with ``rows="tokens"`` the sum over a token's slots (zero for a
+    token without one), with ``rows="slots"`` one row per slot, undefined behind the last slot.
+    ``grad_W`` has ``W``'s shape and is contiguous; experts without a slot get zeros.
     """
     E, K, N, epi = _check_product(X, W, slots, rows, b_is_nk, epilogue)
     _check_rows("grad_out", grad_out, (slots.capacity, N // 2 if epi else N), X)
