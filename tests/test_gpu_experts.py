@@ -1100,3 +1100,208 @@ def test_streams_have_numbers_of_their_own():
             t.join()
     assert off == []
     ops.check_expert_status()
+
+
+# ------------------------------------------- the larger forms of every launch, and their seams
+def _pairs_of_sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count // 2
+
+
+@pytest.mark.parametrize("extra", [0.0, 0.2, 0.34])
+@pytest.mark.parametrize("form", ["plain", "float", "silu_gate"])
+@pytest.mark.parametrize("b_is_nk", [False, True])
+def test_shared_tiles_before_whole_ones(extra, form, b_is_nk):
+    """A few tiles more than pairs of SMs: the tiles of a round and of the rest are cut up, so that
+    a pair's run may hold the end of a tile, whole tiles and the start of another.  From a third
+    of the pairs more they stay whole."""
+    from tileccl_b200 import ops
+
+    P = _pairs_of_sms()
+    tiles = P + max(1, int(extra * P))
+    dtype, T, K, N = torch.bfloat16, 3, 4096, 256 * tiles
+    gate = form == "silu_gate"
+    g = _gen(91)
+    slots = _make_slots(g, T, 1, 1)
+    X = _randn(g, T, K, std=K ** -0.5, dtype=dtype)
+    W = _randn(g, 1, N, K, dtype=dtype) if b_is_nk else _randn(g, 1, K, N, dtype=dtype)
+    kw = dict(b_is_nk=b_is_nk, epilogue="silu_gate" if gate else "none",
+              out_dtype=torch.float32 if form == "float" else None)
+    got = ops.expert_gemm(X, W, slots, **kw)
+    for _ in range(3):
+        assert torch.equal(ops.expert_gemm(X, W, slots, **kw), got)
+    want, bound = _ref_product(X[slots.token_of_slot.long()], W[0].t() if b_is_nk else W[0], gate)
+    if form != "float":
+        bound = bound + (want.abs() + bound) * _half_step(dtype) + 2 ** -25
+    _within(got, want, bound)
+    ops.check_expert_status()
+
+
+@pytest.mark.parametrize("more", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ["tokens", "slots"])
+@pytest.mark.parametrize("epilogue", ["none", "silu_gate"])
+def test_backward_of_shared_tiles(more, dtype, rows, epilogue):
+    """Few rows, contractions of 4096 and more: the gate's gradient (16 tiles, or one more than there
+    are pairs) and the token gradients come from shared tiles, too."""
+    tiles = _pairs_of_sms() + 1 if more else 17
+    test_expert_gemm_backward((3, 1, 1, 4096, 256 * tiles, 0.0), dtype, False, rows, epilogue)
+
+
+@pytest.fixture
+def many_choices(monkeypatch):
+    """Lets the tests above take more choices than they have experts for, with room for sums of that
+    many terms in the bounds of the products."""
+    slots, bound = _make_slots, _sum_bound
+    here = globals()
+    monkeypatch.setitem(here, "_make_slots", lambda g, t, k, e, lost=0.0: slots(g, t, k, max(e, k), lost))
+    # (|a sum of k products' results| <= sum of |a| |b|: k additions of 2^-24 each)
+    monkeypatch.setitem(here, "_sum_bound", lambda a, b, terms: bound(a, b, terms + 16))
+
+
+@pytest.mark.parametrize("tokens, k, n, lost", [
+    (300, 2, 9000, 0.1), (300, 4, 4104, 0.0), (300, 3, 264, 0.3), (256, 4, 8, 0.0), (5, 11, 1032, 0.2),
+    (300, 20, 264, 0.1), (257, 9, 2056, 0.0), (2, 32, 8200, 0.0)])
+@pytest.mark.parametrize("weighted, add", [(True, True), (False, False)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_combine_of_every_batch(many_choices, tokens, k, n, lost, weighted, add, dtype):
+    test_combine(tokens, k, n, lost, weighted, add, dtype)
+
+
+@pytest.mark.parametrize("tokens, k, n, lost", [
+    (300, 3, 264, 0.0), (40, 4, 4104, 0.2), (300, 9, 1032, 0.0), (7, 20, 2056, 0.3), (2, 32, 8, 0.0)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_combine_backward_of_every_batch(many_choices, tokens, k, n, lost, dtype):
+    test_combine_backward(tokens, k, n, lost, dtype)
+
+
+@pytest.mark.parametrize("case", [(300, 2, 4, 2568, 256, 0.0),         # two choices, several pieces
+                                  (300, 3, 4, 1032, 256, 0.1), (40, 6, 8, 264, 256, 0.2),
+                                  (270, 12, 16, 136, 256, 0.0)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("epilogue", ["none", "silu_gate"])
+def test_backward_sums_of_many_choices(many_choices, case, dtype, epilogue):
+    """Token gradients summed over more choices than one batch of the fp32 combine holds."""
+    test_expert_gemm_backward(case, dtype, False, "tokens", epilogue)
+
+
+@pytest.mark.parametrize("case", [(300, 8, 64, 64, 256, 0.0), (90, 6, 200, 72, 512, 0.2),
+                                  (50, 4, 129, 4096, 256, 0.0), (700, 4, 1024, 64, 256, 0.1),
+                                  (3, 8, 1024, 136, 256, 0.0)])
+@pytest.mark.parametrize("b_is_nk", [False, True])
+@pytest.mark.parametrize("epilogue", ["none", "silu_gate"])
+def test_products_of_many_experts(case, b_is_nk, epilogue):
+    test_expert_gemm(case, torch.bfloat16, b_is_nk, "tokens", epilogue)
+    if case[3] < 4096:
+        test_expert_gemm_backward(case, torch.bfloat16, b_is_nk, "slots", epilogue)
+
+
+def test_products_of_a_part_of_the_experts():
+    """A rank that holds the experts 24 .. 40 of 64: the same rows as in the whole map, and nothing
+    behind the last of them."""
+    from tileccl_b200 import ops
+
+    g = _gen(93)
+    T, k, E, first, local, K, N, dtype = 120, 6, 64, 24, 16, 136, 256, torch.float16
+    ids = _randn(g, T, E).topk(k, 1).indices.int()
+    X, W = _randn(g, T, K, std=K ** -0.5, dtype=dtype), _randn(g, E, K, N, dtype=dtype)
+    dY = _randn(g, T * k, N, dtype=dtype)
+    whole, part = ops.expert_slots(ids, E), ops.expert_slots(ids, local, first_expert=first)
+    a, b = int(whole.offsets[first]), int(whole.offsets[first + local])
+    y = ops.expert_gemm(X, W, whole)
+    out = torch.full((T * k, N), 7.0, dtype=dtype, device="cuda")
+    ops.expert_gemm(X, W[first:first + local], part, out)
+    assert torch.equal(out[:b - a], y[a:b]) and (out[b - a:] == 7.0).all()
+    _, gw = ops.expert_gemm_backward(dY, X, W, whole)
+    dY_part = torch.full_like(dY, math.nan)
+    dY_part[:b - a] = dY[a:b]
+    gx, gw_part = ops.expert_gemm_backward(dY_part, X, W[first:first + local], part)
+    assert torch.equal(gw_part, gw[first:first + local]) and torch.isfinite(gx).all()
+    here = ((ids >= first) & (ids < first + local)).any(1)
+    assert (gx[~here] == 0).all() and (gx[here] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("E, k, kw", [
+    (8, 2, {}), (64, 8, {}), (256, 8, dict(groups=8, top_groups=3, group_score="max")),
+    (256, 8, dict(score="sigmoid", biased=True, groups=8, top_groups=4, scale=2.5)),
+    (33, 5, dict(biased=True, renormalize=False)), (500, 32, dict(score="sigmoid", biased=True)),
+    (40, 3, dict(score="sigmoid", groups=5, top_groups=2))])
+def test_route_of_a_large_batch(dtype, E, k, kw):
+    """More tokens than there are warps in a launch: every row as in a small batch."""
+    from tileccl_b200 import ops
+
+    g = _gen(95 + E)
+    kw = dict(kw)
+    T, step = 10_007, 251
+    logits = _randn(g, T, E, std=1.5).to(dtype)
+    logits[::7, 1] = -math.inf
+    mask = torch.rand(T, device="cuda", generator=g) < 0.9
+    bias = _randn(g, E, std=0.1) if kw.pop("biased", False) else None
+    w, ids = ops.route_experts(logits, k, bias=bias, mask=mask, **kw)
+    assert (ids[~mask] == -1).all() and (ids[mask][:, 0] >= 0).all()
+    grad = _randn(g, T, k)
+    options = {n: kw[n] for n in ("score", "renormalize", "scale") if n in kw}
+    dl = ops.route_experts_backward(grad, logits, ids, **options)
+    for a in range(0, T, step):
+        b = a + step
+        w1, ids1 = ops.route_experts(logits[a:b], k, bias=bias, mask=mask[a:b], **kw)
+        assert torch.equal(ids1, ids[a:b]) and torch.equal(w1, w[a:b])
+        assert torch.equal(ops.route_experts_backward(grad[a:b], logits[a:b], ids1, **options), dl[a:b])
+
+
+@pytest.mark.parametrize("b_is_nk", [False, True])
+@pytest.mark.parametrize("N, epilogue", [(72, "none"), (192, "none"), (512, "silu_gate")])
+def test_interleaved_experts_give_the_results_of_separate_ones(b_is_nk, N, epilogue):
+    """W[e] between the rows of the others, in every form of the weights' map, forward and back."""
+    from tileccl_b200 import ops
+
+    g = _gen(97)
+    dtype, T, k, E, K = torch.float16, 40, 2, 3, 136
+    slots = _make_slots(g, T, k, E)
+    X = _randn(g, T, K, std=K ** -0.5, dtype=dtype)
+    W = _randn(g, *((N, E, K) if b_is_nk else (K, E, N)), dtype=dtype).transpose(0, 1)
+    dY = _randn(g, T * k, N // 2 if epilogue == "silu_gate" else N, dtype=dtype)
+    kw = dict(b_is_nk=b_is_nk, epilogue=epilogue)
+    assert not W.is_contiguous()
+    assert torch.equal(ops.expert_gemm(X, W, slots, **kw), ops.expert_gemm(X, W.contiguous(), slots, **kw))
+    got = ops.expert_gemm_backward(dY, X, W, slots, **kw)
+    want = ops.expert_gemm_backward(dY, X, W.contiguous(), slots, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[1].is_contiguous()
+
+
+def test_layers_of_two_host_threads():
+    """Whole layers and their gradients, on a stream per thread and on one for both."""
+    import threading
+
+    from tileccl_b200 import ops
+
+    dtype, k, E, H, F, T = torch.bfloat16, 2, 8, 4096, 256, 24
+    g = _gen(99)
+    w_gu, w_down = _randn(g, E, H, 2 * F, std=H ** -0.5, dtype=dtype), _randn(g, E, F, H, std=F ** -0.5, dtype=dtype)
+    data = [(_randn(g, T, E), _randn(g, T, H, dtype=dtype)) for _ in range(2)]
+
+    def step(l, x):
+        out, weights, slots, h, y = _layer(ops, l, x, w_gu, w_down, k)
+        dy, dw = ops.expert_combine_backward(out, y, slots, weights)
+        dh, dw_down = ops.expert_gemm_backward(dy, h, w_down, slots, rows="slots")
+        dx, dw_gu = ops.expert_gemm_backward(dh, x, w_gu, slots, epilogue="silu_gate")
+        return out, dw, dh, dw_down, dx, dw_gu
+
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    off = []
+
+    def work(i, stream):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = step(*data[i])
+                off.extend((i, n) for n, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a, b))
+
+    for streams in ([torch.cuda.Stream(), torch.cuda.Stream()], [torch.cuda.default_stream()] * 2):
+        threads = [threading.Thread(target=work, args=(i, s)) for i, s in enumerate(streams)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    assert off == []
+    ops.check_expert_status()
