@@ -51,9 +51,6 @@ constexpr int kStagingBytes = 2 * kChunk * kStageLd * 4;
 constexpr int kCtlBytes = 512;
 constexpr int kListBytes = 2 * 4 * (kMaxExperts + 2);
 constexpr int kGemmSmem = kStages * kStageBytes + kStagingBytes + kCtlBytes + kListBytes + 1024;
-// Time that the waits of a launch have, on top of their budget, for every K block and every tile
-// that a pair can be given.  A block takes 0.15 - 0.4 us, an empty tile's zeros 3.
-constexpr uint64_t kNsPerBlock = 100000;
 constexpr int kGradStages = kStages - 1; // the sixth stage takes the copied blocks
 constexpr int kGradStagingBytes = 4 * 2 * 4096;   // per epilogue warp two buffers of 32 x 64
 constexpr int kGradSmem = kStages * kStageBytes + kGradStagingBytes + kCtlBytes + 1024;
@@ -378,14 +375,11 @@ expert_gemm_kernel(const __grid_constant__ GemmParams p) {
   // nothing but x; what came before it, the offsets among it, was complete when it began).  One
   // token of 2 experts of 4096 x 28672: 80 -> 78 us, of 8 of 4096 x 3584: 44.2 -> 43.7.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  WaitBudget wb;
+  wb.start(p.budget_ns, s.words + 1);
+
   const int total = s.tiles[p.experts];
   const int pairs = static_cast<int>(gridDim.x >> 1), pair = static_cast<int>(blockIdx.x >> 1);
-  // One deadline for all waits of the launch: nothing waits for a peer, so it grows with the work
-  // and only a fault can reach it.
-  WaitBudget wb;
-  wb.start(p.budget_ns + kNsPerBlock * (static_cast<uint64_t>(max(total, 0) / pairs) + 2) *
-                             (static_cast<uint64_t>(p.k_blocks) + 1),
-           s.words + 1);
   auto walk = [&]() {
     Walker w;
     const int over = total % pairs;
@@ -696,14 +690,10 @@ expert_weight_grad_kernel(const __grid_constant__ GradParams p) {
   }
   pipe_start(s);
   const uint32_t tmem_base = pipe_meet(s);
+  WaitBudget wb;
+  wb.start(p.budget_ns, s.words + 1);
   const int total = p.experts * per_expert;
   const int step = static_cast<int>(gridDim.x >> 1);
-  // (one deadline, see expert_gemm_kernel: a pair has at most per_expert / step + 1 tiles of an
-  // expert, and the experts together slots / kBK + experts blocks of rows)
-  WaitBudget wb;
-  wb.start(p.budget_ns + kNsPerBlock * (static_cast<uint64_t>(per_expert / step) + 1) *
-                             (static_cast<uint64_t>(p.slots / kBK) + 2 * static_cast<uint64_t>(p.experts)),
-           s.words + 1);
 
   if (warp == 0) {
     // ------------------------------- TMA producer -------------------------------
@@ -1001,7 +991,14 @@ int32_t partial_tokens(int64_t slots) {
   return static_cast<int32_t>(slots < kTile ? (slots + 31) / 32 * 32 : kTile);
 }
 
-constexpr uint64_t kWaitBudgetNs = 2000000000ull;      // before the share of the work
+// All waits of a launch have one deadline.  Nothing waits for a peer, so it grows with the work and
+// only a fault can reach it: on top of the budget 100 us for every step (K block, or tile of zeros)
+// that an SM pair can be given, which takes 0.15 - 3 us.
+constexpr uint64_t kWaitBudgetNs = 2000000000ull, kNsPerStep = 100000;
+uint64_t deadline_ns(uint64_t budget, int64_t steps) {
+  const int64_t most = int64_t(1) << 30;       // (a day; the product stays far below 2^64)
+  return (budget ? budget : kWaitBudgetNs) + kNsPerStep * static_cast<uint64_t>(steps < most ? steps : most);
+}
 
 }  // namespace
 
@@ -1132,12 +1129,12 @@ extern "C" int tccl_expert_gemm(const TcclExpertGemm* desc, uint64_t stream) {
   p.f_tiles = static_cast<int32_t>(f_tiles);
   p.bf16 = bf16 ? 1 : 0;
   p.status = reinterpret_cast<uint32_t*>(d.status);
-  p.budget_ns = d.wait_budget_ns ? d.wait_budget_ns : kWaitBudgetNs;
   int sms = 0;
   TCCL_CHECK_CUDA(attrs_once(&sms));
   // (a shared tile is cut into runs of kMinBlocks K blocks at least)
   const int64_t runs = p.partial == nullptr ? tiles : tiles * ((p.k_blocks + kMinBlocks - 1) / kMinBlocks);
   const int pairs = static_cast<int>(runs < sms / 2 ? runs : sms / 2);
+  p.budget_ns = deadline_ns(d.wait_budget_ns, (tiles / pairs + 2) * (p.k_blocks + int64_t(1)));
   const GemmKernel kernel =
       d.slots <= kFewTokens ? gemm_kernel<true>(d.epilogue) : gemm_kernel<false>(d.epilogue);
   TCCL_CHECK_CUDA(launch_pairs(kernel, p, pairs,
@@ -1201,10 +1198,13 @@ extern "C" int tccl_expert_weight_grad(const TcclExpertWeightGrad* desc, uint64_
   p.n_tiles = static_cast<int32_t>(n_tiles);
   p.bf16 = bf16 ? 1 : 0;
   p.status = reinterpret_cast<uint32_t*>(d.status);
-  p.budget_ns = d.wait_budget_ns ? d.wait_budget_ns : kWaitBudgetNs;
   int sms = 0;
   TCCL_CHECK_CUDA(attrs_once(&sms));
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+  // (a pair has at most m_tiles * n_tiles / pairs + 1 tiles of an expert; the experts together have
+  // slots / kBK blocks of rows and one more each)
+  p.budget_ns = deadline_ns(d.wait_budget_ns,
+                            (m_tiles * n_tiles / pairs + 1) * (d.slots / kBK + 2 * int64_t(d.experts)));
   TCCL_CHECK_CUDA(launch_pairs(&expert_weight_grad_kernel, p, pairs, kThreads + kCopyThreads, kGradSmem,
                                reinterpret_cast<cudaStream_t>(stream), false));
   return kOk;
