@@ -1016,8 +1016,19 @@ cudaError_t preload_expert_gemm_kernels() {
 
 using namespace tileccl;
 
-// Tiles are shared for at most this many slots, and at least this long a contraction (see the
-// schedule of expert_gemm_kernel).
+// Tiles may be shared for at most this many slots, and at least this long a contraction (see the
+// schedule of expert_gemm_kernel).  What sharing gains grows with the contraction, what it costs
+// with the rows of an expert (partial sums) and the parts of a tile.  Weights from DRAM, us shared /
+// whole, K x N with the rows of every expert in front:
+//   1 row    1024 x 4096 10.9 / 10.1   1792 x 4096 11.7 / 12.2   2048 x 4096 14.1 / 12.8
+//            3584 x 4096 15.9 / 17.0   4096 x 4096 16.4 / 18.4   4096 x 19200 33.6 / 38.3
+//   16 rows  2048 x 4096 14.6 / 13.1   3584 x 4096 17.2 / 17.2   4096 x 4096 16.7 / 18.7
+//   32 rows  4096 x 4096 18.4 / 19.1   of each of 4 experts: 4096 x 1024 18.3 / 20.1
+//   64 rows  4096 x 4096 22.1 / 19.9   6144 x 4096 25.6 / 25.5   8192 x 4096 27.7 / 31.2
+//   128 rows 4096 x 4096 29.0 / 23.1   8192 x 4096 35.4 / 36.2   14336 x 4096 45.1 / 57.0
+//            4096 x 1024 39.4 / 22.1   8192 x 1024 48.4 / 34.3   14336 x 1024 47.7 / 52.7
+// The limits are those of the sum over experts, which the host knows: more than 32 rows of a single
+// expert lose below K = 6144, and 3584 would gain with one row.
 constexpr int64_t kSharedSlots = 128, kSharedK = 4096;
 
 extern "C" int tccl_expert_gemm_scratch(int64_t slots, int64_t k, int64_t* partial_bytes,
